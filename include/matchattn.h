@@ -344,6 +344,82 @@ MATCHATTN_API int matchattn_flow_init(const void *correlation, void *prob, void 
                                       void *scratch, size_t scratch_bytes, int B, int H, int W, int dtype,
                                       void *cuda_stream);
 
+/*
+ * Dense attention of every query over every key that the masks leave, beside the windowed operator above: the attention of
+ * layers whose tokens look at the whole map or at a sequence.  No counterpart in the reference.
+ *
+ *   x_ij = scale * q_i.k_j;  with cap > 0: cap * tanh(x_ij / cap);  with slopes: - slopes[head] * (|dx| + |dy|)
+ *   out_i = sum_j softmax_j(x_ij) v_j over the keys that query i sees; zeros where it sees none
+ *
+ * Key j of item b exists if j < lengths[b] (M without lengths; clamped to 0..M).  Query n stands at key position
+ * lengths[b] - N + n: the last query at the last key.  It sees key j if j exists, and (with causal) j is not behind its own
+ * position or j < prefix[b], and (with documents) both ids are equal and not negative.  dx, dy: columns and rows between the
+ * two positions on a map `width` tokens wide (width 1: their distance in a sequence).
+ * What no query may see does not reach a result, infinite and NaN values included.
+ *
+ *   q [B, N, h, d], k and v [B, M, hk, d] with the strides given (elements; item, token, head; channels are contiguous)
+ *   out [B, N, h, d], contiguous, written.  h is a multiple of hk: query heads [i*h/hk, (i+1)*h/hk) share key head i.
+ *   lse [B, h, N] float32, written: log2 of the sum of 2^(x log2 e) of a row, for the backward pass; may be NULL without one
+ *   d <= MATCHATTN_MAX_DENSE_D; 0 <= M <= 2^24; 0 < N <= 2^24; scale > 0; cap >= 0 (0: none); prefix needs causal.
+ * Scores, softmax and sums are float32.  The sums do not depend on timing: equal calls give equal bits.
+ */
+#define MATCHATTN_MAX_DENSE_D 256
+typedef struct matchattn_global_args {
+    const void *q, *k, *v;
+    void *out;
+    float *lse;
+    long long q_stride[3], k_stride[3], v_stride[3];
+    const float *slopes;               /* [h] or NULL                          */
+    const int *prefix, *lengths;       /* [B] or NULL                          */
+    const int *q_docs, *k_docs;        /* [B, N] and [B, M], both or neither   */
+    int B, N, M, h, hk, d;
+    int dtype, causal, width;
+    float scale, cap;
+} matchattn_global_args;
+
+/* Scratch bytes that the forward (backward = 0) or the backward call needs for these arguments (possibly 0); 0 if they are refused. */
+MATCHATTN_API size_t matchattn_global_scratch_bytes(const matchattn_global_args *args, int backward);
+MATCHATTN_API int matchattn_global_forward(const matchattn_global_args *args, void *scratch, size_t scratch_bytes, void *cuda_stream);
+/* Gradients to q, k and v, contiguous as [B, N, h, d] and [B, M, hk, d], from that of out (contiguous); args->out and args->lse
+ * are the forward call's.  The probabilities are recomputed; scratch is 16-byte aligned, as in the forward call. */
+MATCHATTN_API int matchattn_global_backward(const matchattn_global_args *args, const void *d_out, void *d_q, void *d_k, void *d_v,
+                                            void *scratch, size_t scratch_bytes, void *cuda_stream);
+
+/*
+ * RMS norm of every head of q and k, and its rotation by the token's position, in one pass: what stands between the
+ * projections and a dense attention.  No counterpart in the reference.
+ *
+ *   g = x * rsqrt(mean(x^2) + eps) * weight                      per token and head, over its d channels
+ *   pairs (i, i + rot/2), i < rot/2, turned by position[axis(i)] * freqs[i]; channels from rot on are left as they are
+ *
+ *   q [B, N, h, d], k [B, N, hk, d] with the strides given (elements; item, token, head); hk = 0: no k
+ *   q_out, k_out: contiguous, written
+ *   q_weight, k_weight [d] in weight_dtype (float32 or dtype); NULL: ones
+ *   positions: int32 or (positions_64) int64, [N, axes] for all items (positions_per_item 0) or [B, N, axes] (N * axes)
+ *   freqs [rot/2]: turns per position in units of 2^-64, as 64-bit integers; with axes = 2 the first half belongs to the
+ *     first coordinate of a position, the second half to the other (angles are exact to 2^-32 turns at any position)
+ *   d <= MATCHATTN_MAX_DENSE_D; rot <= d, a multiple of 2 * axes; rot = 0: no rotation (positions and freqs may be NULL)
+ */
+typedef struct matchattn_norm_args {
+    const void *q, *k;
+    long long q_stride[3], k_stride[3];
+    const void *q_weight, *k_weight;
+    const void *positions, *freqs;
+    long long positions_per_item;
+    int positions_64, axes, rot;
+    int B, N, h, hk, d;
+    int dtype, weight_dtype;
+    float eps;
+} matchattn_norm_args;
+
+MATCHATTN_API int matchattn_norm_rotary_forward(const matchattn_norm_args *args, void *q_out, void *k_out, void *cuda_stream);
+/* Gradients of q and k (contiguous) and, where the pointer is not NULL, of the weights (in weight_dtype), from those of q_out
+ * and k_out (contiguous).  scratch: matchattn_norm_rotary_scratch_bytes(d), asked for on the device of the call; not read without weight gradients. */
+MATCHATTN_API size_t matchattn_norm_rotary_scratch_bytes(int d);
+MATCHATTN_API int matchattn_norm_rotary_backward(const matchattn_norm_args *args, const void *d_q_out, const void *d_k_out, void *d_q,
+                                                 void *d_k, void *d_q_weight, void *d_k_weight, void *scratch, size_t scratch_bytes,
+                                                 void *cuda_stream);
+
 /* Name of the kernel variant that matchattn_fused_forward runs for these sizes ("fast cpl=2 lph=1": chunks of
  * eight channels per lane, lanes per head; "generic") or NULL if they are rejected.  pointers_32B_aligned: q, k, v
  * and out are (else 16-byte aligned); attn_out is taken to be aligned as its kernel needs.  Launches nothing. */

@@ -7,6 +7,8 @@ Public surface:
 * ``match_attention`` -- functional form with the row-band and skip-attn options;
 * ``cross_attention_core`` / ``self_attention_core`` -- the operator with the caller's
   clamp, gate and concatenation folded in;
+* ``global_attention`` -- dense attention over all tokens, with capped scores, distance bias and masks; trains;
+  ``norm_rotary`` (with ``rotary_frequencies``) -- norm and rotation of its queries and keys;
 * ``install_dropin()`` -- makes ``import match_attention`` resolve to this
   implementation so that the unmodified reference model runs on it with
   ``--mat_impl cuda``.
@@ -20,7 +22,8 @@ import importlib
 
 _OPS = ("MF_FusedForwardOps", "describe_dispatch", "fused_forward", "fused_forward_ops", "launch",
         "match_attention", "workspace_bytes", "cross_attention_core", "self_attention_core", "launch_glue",
-        "upsample_field", "stereo_volume", "consistency_mask", "local_disparity_estimator", "flow_init", "match_attention_autograd")
+        "upsample_field", "stereo_volume", "consistency_mask", "local_disparity_estimator", "flow_init", "match_attention_autograd",
+        "global_attention", "norm_rotary", "rotary_frequencies")
 __all__ = list(_OPS) + ["install_dropin", "abi_version"]
 
 

@@ -20,15 +20,34 @@ EXPORTS = ("matchattn_fused_forward", "matchattn_fused_forward_ex", "matchattn_f
            "matchattn_upsample_field",
            "matchattn_stereo_volume", "matchattn_consistency_mask", "matchattn_local_disparity",
            "matchattn_flow_init", "matchattn_flow_init_scratch_bytes", "matchattn_copy_blocks",
+           "matchattn_global_forward", "matchattn_global_backward", "matchattn_global_scratch_bytes",
+           "matchattn_norm_rotary_forward", "matchattn_norm_rotary_backward", "matchattn_norm_rotary_scratch_bytes",
            "matchattn_workspace_bytes", "matchattn_describe_dispatch", "matchattn_version", "matchattn_strerror")
 
 F32, F16, BF16 = 0, 1, 2
+MAX_DENSE_D = 256
 ERR_WINDOW = 6
 L1_NORM = 0
 DOT_PRODUCT = 1
 ATTN_TYPE_CODE = {"l1_norm": L1_NORM, "dot_product": DOT_PRODUCT}
 
 _vp, _i, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+_strides = ctypes.c_longlong * 3
+
+
+class GlobalArgs(ctypes.Structure):
+    """matchattn_global_args"""
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "out", "lse")] + \
+        [(n, _strides) for n in ("q_stride", "k_stride", "v_stride")] + \
+        [(n, _vp) for n in ("slopes", "prefix", "lengths", "q_docs", "k_docs")] + \
+        [(n, _i) for n in ("B", "N", "M", "h", "hk", "d", "dtype", "causal", "width")] + [("scale", _f), ("cap", _f)]
+
+
+class NormArgs(ctypes.Structure):
+    """matchattn_norm_args"""
+    _fields_ = [("q", _vp), ("k", _vp), ("q_stride", _strides), ("k_stride", _strides)] + \
+        [(n, _vp) for n in ("q_weight", "k_weight", "positions", "freqs")] + [("positions_per_item", ctypes.c_longlong)] + \
+        [(n, _i) for n in ("positions_64", "axes", "rot", "B", "N", "h", "hk", "d", "dtype", "weight_dtype")] + [("eps", _f)]
 
 
 def _load() -> ctypes.CDLL:
@@ -75,6 +94,19 @@ def _load() -> ctypes.CDLL:
     lib.matchattn_describe_dispatch.argtypes = [_i] * 5
     lib.matchattn_copy_blocks.restype = _i
     lib.matchattn_copy_blocks.argtypes = [ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_size_t), _i, _i, _vp]
+    _global, _norm = ctypes.POINTER(GlobalArgs), ctypes.POINTER(NormArgs)
+    lib.matchattn_global_scratch_bytes.restype = ctypes.c_size_t
+    lib.matchattn_global_scratch_bytes.argtypes = [_global, _i]
+    lib.matchattn_global_forward.restype = _i
+    lib.matchattn_global_forward.argtypes = [_global, _vp, ctypes.c_size_t, _vp]
+    lib.matchattn_global_backward.restype = _i
+    lib.matchattn_global_backward.argtypes = [_global] + [_vp] * 5 + [ctypes.c_size_t, _vp]
+    lib.matchattn_norm_rotary_scratch_bytes.restype = ctypes.c_size_t
+    lib.matchattn_norm_rotary_scratch_bytes.argtypes = [_i]
+    lib.matchattn_norm_rotary_forward.restype = _i
+    lib.matchattn_norm_rotary_forward.argtypes = [_norm] + [_vp] * 3
+    lib.matchattn_norm_rotary_backward.restype = _i
+    lib.matchattn_norm_rotary_backward.argtypes = [_norm] + [_vp] * 7 + [ctypes.c_size_t, _vp]
     lib.matchattn_version.restype = _i
     lib.matchattn_version.argtypes = []
     lib.matchattn_strerror.restype = ctypes.c_char_p

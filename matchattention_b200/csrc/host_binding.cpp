@@ -22,6 +22,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <optional>
@@ -233,6 +234,177 @@ struct MatchAttentionFn : torch::autograd::Function<MatchAttentionFn> {
                                               static_cast<float *>(data(d_v)), dmo, B, H, W, h, C / h, r, r, dtype_code(q), MATCHATTN_L1_NORM,
                                               scale, 0, H, stream));
         return {d_mo, d_q, d_k.to(k.scalar_type()), d_v.to(v.scalar_type()), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// ---- dense attention and the norm and rotation before it ---------------------------------------------------
+
+constexpr const char *kGlobalName = "matchattn_b200::global_attention_op";
+constexpr const char *kNormName = "matchattn_b200::norm_rotary_op";
+
+// A tensor whose channels lie side by side, as the kernels read them.
+Tensor with_rows(const Tensor &t) { return t.numel() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+
+template <typename P>
+P *data_as(const Tensor &t) { return t.defined() ? static_cast<P *>(t.data_ptr()) : nullptr; }
+
+struct GlobalCall {
+    Tensor q, k, v, slopes, prefix, lengths, q_docs, k_docs;
+    double scale, cap;
+    int64_t width;
+    bool causal;
+
+    matchattn_global_args args(const Tensor &out, const Tensor &lse) const
+    {
+        matchattn_global_args a{};
+        a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr(), a.out = out.data_ptr(), a.lse = data_as<float>(lse);
+        for (int i = 0; i < 3; ++i) a.q_stride[i] = q.stride(i), a.k_stride[i] = k.stride(i), a.v_stride[i] = v.stride(i);
+        a.slopes = data_as<float>(slopes), a.prefix = data_as<int>(prefix), a.lengths = data_as<int>(lengths);
+        a.q_docs = data_as<int>(q_docs), a.k_docs = data_as<int>(k_docs);
+        a.B = q.size(0), a.N = q.size(1), a.M = k.size(1), a.h = q.size(2), a.hk = k.size(2), a.d = q.size(3);
+        a.dtype = dtype_code(q), a.causal = causal, a.width = width;
+        a.scale = static_cast<float>(scale), a.cap = static_cast<float>(cap);
+        return a;
+    }
+
+    // The output, and lse where it is wanted; the tensors' device is current.
+    Tensor forward(Tensor *lse) const
+    {
+        const int64_t B = q.size(0), N = q.size(1), h = q.size(2);
+        Tensor out = at::empty({B, N, h, q.size(3)}, q.options());
+        if (lse != nullptr) *lse = at::empty({B, h, N}, q.options().dtype(at::kFloat));
+        if (out.numel() == 0) return out;
+        const matchattn_global_args a = args(out, lse != nullptr ? *lse : Tensor());
+        const size_t bytes = matchattn_global_scratch_bytes(&a, 0);
+        Tensor scratch;
+        if (bytes != 0) scratch = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+        check_status(matchattn_global_forward(&a, data_as<void>(scratch), bytes, c10::cuda::getCurrentCUDAStream(q.device().index()).stream()));
+        return out;
+    }
+};
+
+struct GlobalAttentionFn : torch::autograd::Function<GlobalAttentionFn> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const GlobalCall &call)
+    {
+        GlobalCall c = call;
+        c.q = with_rows(q), c.k = with_rows(k), c.v = with_rows(v);
+        const c10::cuda::CUDAGuard device(q.device());
+        RECORD_FUNCTION(kGlobalName, std::vector<c10::IValue>({q, k, v}));
+        Tensor lse, out = c.forward(&lse);
+        ctx->save_for_backward({q, k, v, out, lse, c.slopes, c.prefix, c.lengths, c.q_docs, c.k_docs});
+        ctx->saved_data["scale"] = c.scale;
+        ctx->saved_data["cap"] = c.cap;
+        ctx->saved_data["width"] = c.width;
+        ctx->saved_data["causal"] = c.causal;
+        return out;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        GlobalCall c{with_rows(s[0]), with_rows(s[1]), with_rows(s[2]), s[5], s[6], s[7], s[8], s[9], ctx->saved_data["scale"].toDouble(),
+                     ctx->saved_data["cap"].toDouble(), ctx->saved_data["width"].toInt(), ctx->saved_data["causal"].toBool()};
+        const Tensor &out = s[3], &lse = s[4];
+        const c10::cuda::CUDAGuard device(out.device());
+        const Tensor d_out = grads[0].contiguous().resolve_neg();
+        const auto like = [](const Tensor &t) { return at::empty(t.sizes(), t.options()); };
+        Tensor d_q = like(s[0]), d_k = like(s[1]), d_v = like(s[2]);
+        if (out.numel() == 0) {
+            d_k.zero_();
+            d_v.zero_();
+        } else {
+            const matchattn_global_args a = c.args(out, lse);
+            const size_t bytes = matchattn_global_scratch_bytes(&a, 1);
+            Tensor scratch;
+            if (bytes != 0) scratch = at::empty({static_cast<int64_t>(bytes)}, out.options().dtype(at::kByte));
+            check_status(matchattn_global_backward(&a, d_out.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), data_as<void>(scratch),
+                                                   bytes, c10::cuda::getCurrentCUDAStream(out.device().index()).stream()));
+        }
+        return {d_q, d_k, d_v, Tensor()};
+    }
+};
+
+struct NormCall {
+    Tensor q, k, q_weight, k_weight, freqs, positions;
+    double eps;
+
+    matchattn_norm_args args() const
+    {
+        matchattn_norm_args a{};
+        a.q = q.data_ptr(), a.k = data_as<void>(k);
+        for (int i = 0; i < 3; ++i) {
+            a.q_stride[i] = q.stride(i);
+            a.k_stride[i] = k.defined() ? k.stride(i) : 0;
+        }
+        a.q_weight = data_as<void>(q_weight), a.k_weight = data_as<void>(k_weight);
+        a.positions = data_as<void>(positions), a.freqs = data_as<void>(freqs);
+        a.axes = freqs.defined() ? freqs.size(0) : 1, a.rot = freqs.defined() ? 2 * freqs.numel() : 0;
+        a.positions_per_item = positions.defined() && positions.dim() == (a.axes == 1 ? 2 : 3) && positions.size(0) > 1 ? q.size(1) * a.axes : 0;
+        a.positions_64 = positions.defined() && positions.scalar_type() == at::kLong;
+        a.B = q.size(0), a.N = q.size(1), a.h = q.size(2), a.hk = k.defined() ? k.size(2) : 0, a.d = q.size(3);
+        a.dtype = dtype_code(q);
+        const Tensor &w = q_weight.defined() ? q_weight : k_weight;
+        a.weight_dtype = w.defined() ? dtype_code(w) : a.dtype;
+        a.eps = static_cast<float>(eps);
+        return a;
+    }
+
+    torch::autograd::variable_list forward() const
+    {
+        Tensor yq = at::empty(q.sizes(), q.options()), yk = k.defined() ? at::empty(k.sizes(), k.options()) : Tensor();
+        if (q.numel() != 0) {
+            const matchattn_norm_args a = args();
+            check_status(matchattn_norm_rotary_forward(&a, yq.data_ptr(), data_as<void>(yk), c10::cuda::getCurrentCUDAStream(q.device().index()).stream()));
+        }
+        return k.defined() ? torch::autograd::variable_list{yq, yk} : torch::autograd::variable_list{yq};
+    }
+};
+
+struct NormRotaryFn : torch::autograd::Function<NormRotaryFn> {
+    using Maybe = std::optional<Tensor>;
+
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Maybe &k, const Maybe &q_weight,
+                                                  const Maybe &k_weight, const NormCall &call)
+    {
+        NormCall c = call;
+        c.q = with_rows(c.q);
+        if (c.k.defined()) c.k = with_rows(c.k);
+        const c10::cuda::CUDAGuard device(q.device());
+        RECORD_FUNCTION(kNormName, std::vector<c10::IValue>({q}));
+        ctx->save_for_backward({call.q, call.k, c.q_weight, c.k_weight, c.freqs, c.positions});
+        ctx->saved_data["eps"] = c.eps;
+        ctx->saved_data["q_weight"] = c.q_weight.defined() && c.q_weight.requires_grad();
+        ctx->saved_data["k_weight"] = c.k_weight.defined() && c.k_weight.requires_grad();
+        return c.forward();
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        const bool both = s[1].defined();
+        const NormCall c{with_rows(s[0]), both ? with_rows(s[1]) : s[1], s[2], s[3], s[4], s[5], ctx->saved_data["eps"].toDouble()};
+        const c10::cuda::CUDAGuard device(c.q.device());
+        const auto like = [](const Tensor &t) { return t.defined() ? at::empty(t.sizes(), t.options()) : Tensor(); };
+        const auto whole = [](const Tensor &t) { return t.contiguous().resolve_neg(); };
+        Tensor d_q = like(s[0]), d_k = like(s[1]);
+        Tensor d_qw = ctx->saved_data["q_weight"].toBool() ? like(s[2]) : Tensor(), d_kw = ctx->saved_data["k_weight"].toBool() ? like(s[3]) : Tensor();
+        if (c.q.numel() == 0) {
+            if (d_qw.defined()) d_qw.zero_();
+            if (d_kw.defined()) d_kw.zero_();
+        } else {
+            const Tensor g_q = whole(grads[0]), g_k = both ? whole(grads[1]) : Tensor();
+            const matchattn_norm_args a = c.args();
+            Tensor scratch;
+            size_t bytes = 0;
+            if (d_qw.defined() || d_kw.defined()) {
+                bytes = matchattn_norm_rotary_scratch_bytes(a.d);
+                scratch = at::empty({static_cast<int64_t>(bytes)}, c.q.options().dtype(at::kByte));
+            }
+            check_status(matchattn_norm_rotary_backward(&a, g_q.data_ptr(), data_as<void>(g_k), d_q.data_ptr(), data_as<void>(d_k),
+                                                        data_as<void>(d_qw), data_as<void>(d_kw), data_as<void>(scratch), bytes,
+                                                        c10::cuda::getCurrentCUDAStream(c.q.device().index()).stream()));
+        }
+        return {d_q, d_k, d_qw, d_kw, Tensor()};
     }
 };
 
@@ -471,10 +643,109 @@ PyObject *flow_init(PyObject *const *a, Py_ssize_t n)
     return Py_BuildValue("(NN)", THPVariable_Wrap(flow), THPVariable_Wrap(prob));
 }
 
+// A tensor or None; false for anything else, or a tensor on another device than `like`.
+bool optional_tensor(PyObject *o, const Tensor &like, Tensor &t)
+{
+    if (o == Py_None) return true;
+    return cuda_tensor(o, t) && t.device() == like.device();
+}
+
+bool sized(const Tensor &t, at::ScalarType type, std::initializer_list<int64_t> shape)
+{
+    return !t.defined() || (t.scalar_type() == type && t.sizes() == at::IntArrayRef(shape.begin(), shape.size()) && t.is_contiguous());
+}
+
+// [B, N, h, d] of sizes that the entry points of the C ABI take (or empty)
+bool head_rows(const Tensor &t) { return t.dim() == 4 && dtype_code(t) >= 0 && t.size(3) > 0 && t.size(3) <= MATCHATTN_MAX_DENSE_D && t.size(2) > 0; }
+
+// global_attention(q, k, v, scale, cap, slopes, width, causal, prefix, lengths, q_docs, k_docs) -> out
+PyObject *global_attention(PyObject *const *a, Py_ssize_t n)
+{
+    GlobalCall c;
+    if (n != 12 || !eager() || !cuda_tensor(a[0], c.q) || !cuda_tensor(a[1], c.k) || !cuda_tensor(a[2], c.v) || !to_float(a[3], c.scale) ||
+        !to_float(a[4], c.cap) || !optional_tensor(a[5], c.q, c.slopes) || !to_int(a[6], c.width) || !optional_tensor(a[8], c.q, c.prefix) ||
+        !optional_tensor(a[9], c.q, c.lengths) || !optional_tensor(a[10], c.q, c.q_docs) || !optional_tensor(a[11], c.q, c.k_docs))
+        return not_covered();
+    const int causal = PyObject_IsTrue(a[7]);
+    if (causal < 0) {
+        PyErr_Clear();
+        return not_covered();
+    }
+    c.causal = causal != 0;
+    if (!head_rows(c.q) || !head_rows(c.k) || c.k.sizes() != c.v.sizes() || c.k.scalar_type() != c.q.scalar_type() ||
+        c.v.scalar_type() != c.q.scalar_type() || c.k.device() != c.q.device() || c.v.device() != c.q.device() || c.k.size(0) != c.q.size(0) ||
+        c.k.size(3) != c.q.size(3) || c.q.size(2) % c.k.size(2) != 0 || c.width <= 0)
+        return not_covered();
+    const int64_t B = c.q.size(0), N = c.q.size(1), M = c.k.size(1);
+    if (!sized(c.slopes, at::kFloat, {c.q.size(2)}) || (c.slopes.defined() && c.slopes.requires_grad()) || !sized(c.prefix, at::kInt, {B}) ||
+        !sized(c.lengths, at::kInt, {B}) || c.q_docs.defined() != c.k_docs.defined() || !sized(c.q_docs, at::kInt, {B, N}) ||
+        !sized(c.k_docs, at::kInt, {B, M}) || (c.prefix.defined() && !c.causal) || !(c.scale > 0) || !(c.cap >= 0) || !std::isfinite(c.scale) || !std::isfinite(c.cap) || N > (1 << 24) || M > (1 << 24))
+        return not_covered();
+    Tensor out;
+    {
+        pybind11::gil_scoped_release release;
+        if (at::GradMode::is_enabled() && (c.q.requires_grad() || c.k.requires_grad() || c.v.requires_grad())) {
+            const Tensor q = c.q, k = c.k, v = c.v;
+            out = GlobalAttentionFn::apply(q, k, v, c);
+        } else {
+            const c10::cuda::CUDAGuard device(c.q.device());
+            RECORD_FUNCTION(kGlobalName, std::vector<c10::IValue>({c.q, c.k, c.v}));
+            c.q = with_rows(c.q), c.k = with_rows(c.k), c.v = with_rows(c.v);
+            out = c.forward(nullptr);
+        }
+    }
+    return THPVariable_Wrap(out);
+}
+
+// norm_rotary(q, k or None, freqs, positions, q_weight, k_weight, eps) -> (q, k) or (q,)
+PyObject *norm_rotary(PyObject *const *a, Py_ssize_t n)
+{
+    NormCall c;
+    if (n != 7 || !eager() || !cuda_tensor(a[0], c.q) || !optional_tensor(a[1], c.q, c.k) || !optional_tensor(a[2], c.q, c.freqs) ||
+        !optional_tensor(a[3], c.q, c.positions) || !optional_tensor(a[4], c.q, c.q_weight) || !optional_tensor(a[5], c.q, c.k_weight) ||
+        !to_float(a[6], c.eps) || !(c.eps >= 0) || !std::isfinite(c.eps) || !head_rows(c.q))
+        return not_covered();
+    const int64_t B = c.q.size(0), N = c.q.size(1), d = c.q.size(3);
+    if (c.k.defined() && (!head_rows(c.k) || c.k.scalar_type() != c.q.scalar_type() || c.k.size(0) != B || c.k.size(1) != N || c.k.size(3) != d))
+        return not_covered();
+    if (c.freqs.defined() != c.positions.defined()) return not_covered();
+    if (c.freqs.defined()) {
+        const Tensor &f = c.freqs, &p = c.positions;
+        if (f.dim() != 2 || f.scalar_type() != at::kLong || !f.is_contiguous() || f.size(0) < 1 || f.size(0) > 2 || 2 * f.numel() > d ||
+            (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong) || !p.is_contiguous())
+            return not_covered();
+        const int64_t lead = p.dim() - (f.size(0) == 2 ? 2 : 1);
+        if (lead < 0 || lead > 1 || (lead == 1 && p.size(0) != B && p.size(0) != 1) || p.size(lead) != N || (f.size(0) == 2 && p.size(lead + 1) != 2))
+            return not_covered();
+    }
+    for (const Tensor *w : {&c.q_weight, &c.k_weight})
+        if (w->defined() && (w->dim() != 1 || w->size(0) != d || !w->is_contiguous() || (w->scalar_type() != at::kFloat && w->scalar_type() != c.q.scalar_type())))
+            return not_covered();
+    if (c.q_weight.defined() && c.k_weight.defined() && c.q_weight.scalar_type() != c.k_weight.scalar_type()) return not_covered();
+    if (c.k_weight.defined() && !c.k.defined()) return not_covered();
+    torch::autograd::variable_list out;
+    const auto trained = [](const Tensor &t) { return t.defined() && t.requires_grad(); };
+    {
+        pybind11::gil_scoped_release release;
+        if (at::GradMode::is_enabled() && (trained(c.q) || trained(c.k) || trained(c.q_weight) || trained(c.k_weight))) {
+            const auto maybe = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+            const Tensor q = c.q;
+            out = NormRotaryFn::apply(q, maybe(c.k), maybe(c.q_weight), maybe(c.k_weight), c);
+        } else {
+            const c10::cuda::CUDAGuard device(c.q.device());
+            RECORD_FUNCTION(kNormName, std::vector<c10::IValue>({c.q}));
+            c.q = with_rows(c.q);
+            if (c.k.defined()) c.k = with_rows(c.k);
+            out = c.forward();
+        }
+    }
+    return out.size() == 2 ? Py_BuildValue("(NN)", THPVariable_Wrap(out[0]), THPVariable_Wrap(out[1])) : Py_BuildValue("(N)", THPVariable_Wrap(out[0]));
+}
+
 #define MA_ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MA_ENTRY(module_forward),   MA_ENTRY(autograd),        MA_ENTRY(launch),    MA_ENTRY(cross_core), MA_ENTRY(self_core),
                          MA_ENTRY(upsample_field),   MA_ENTRY(stereo_volume),   MA_ENTRY(consistency_mask), MA_ENTRY(local_disparity),
-                         MA_ENTRY(flow_init),        {nullptr, nullptr, 0, nullptr}};
+                         MA_ENTRY(flow_init),        MA_ENTRY(global_attention), MA_ENTRY(norm_rotary), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,572 @@
+// Dense attention on the ordinary arithmetic units: float32, and head widths and alignments that the matrix kernels do not take.
+//
+// A block of 16 x 16 threads owns a tile of query rows of one key head (the g query heads that share it side by side: row
+// r is query r / g of head r % g, so K and V are read once for all of them) and walks the keys.  Tiles lie in shared memory
+// channel by channel ([channel][row], rows 16 bytes aligned, pitch + 4), so that a thread of the score product reads its rows and
+// its keys as one 16-byte word each per channel and the value product reads four keys of a channel at once.  All sums are
+// float32.  Bound by the multiply-add rate and the shared-memory reads behind it (one 16-byte read per 8 multiply-adds in the
+// scores, 10.7 in the value products).
+//
+// A value that no row of a tile may see can still be infinite or NaN, and 0 * NaN is NaN: a tile that holds such a value is
+// accumulated term by term, leaving out the terms of weight zero.
+#include "matchattn_global.cuh"
+
+#include <type_traits>
+
+namespace matchattn {
+namespace {
+
+constexpr int kAnyThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ void load_four(const T *p, int n, bool vec, float (&x)[4])
+{
+    if (vec && n >= 4) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 t = *reinterpret_cast<const float4 *>(p);
+            x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+        } else {
+            const uint2 t = *reinterpret_cast<const uint2 *>(p);
+            x[0] = DT<T>::unpack(t.x, 0), x[1] = DT<T>::unpack(t.x, 1), x[2] = DT<T>::unpack(t.y, 0), x[3] = DT<T>::unpack(t.y, 1);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = i < n ? load_one<T>(p + i) : 0.0f;
+    }
+}
+
+// dst[channel][row] = row(r)[channel]; rows that `row` has no address for, and channels from d on, are zero.  True if a value is
+// infinite or NaN.
+template <typename T, int DP, int ROWS, typename Row>
+__device__ __forceinline__ bool load_transposed(float *dst, int d, bool vec, Row row)
+{
+    bool bad = false;
+    for (int i = threadIdx.x; i < ROWS * (DP / 4); i += kAnyThreads) {
+        const int r = i % ROWS, c = i / ROWS * 4;
+        const T *src = row(r);
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (src != nullptr && c < d) load_four<T>(src + c, d - c, vec, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bad |= !(fabsf(x[j]) <= 3.402823466e38f);
+            dst[(c + j) * (ROWS + 4) + r] = x[j];
+        }
+    }
+    return bad;
+}
+
+template <int R>
+__device__ __forceinline__ void read_run(const float *p, float (&x)[R])
+{
+    if constexpr (R == 4) {
+        const float4 t = *reinterpret_cast<const float4 *>(p);
+        x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+    } else if constexpr (R == 2) {
+        const float2 t = *reinterpret_cast<const float2 *>(p);
+        x[0] = t.x, x[1] = t.y;
+    } else {
+        x[0] = *p;
+    }
+}
+
+// s[i][j] += sum over the channels of a[channel][RA * ty + i] * b[channel][RB * tx + j]
+template <int RA, int RB, int PA, int PB>
+__device__ __forceinline__ void products(float (&s)[RA][RB], const float *a, const float *b, int d, int ty, int tx)
+{
+    a += RA * ty;
+    b += RB * tx;
+#pragma unroll 4
+    for (int c = 0; c < d; ++c) {
+        float x[RA], y[RB];
+        read_run<RA>(a + c * PA, x);
+        read_run<RB>(b + c * PB, y);
+#pragma unroll
+        for (int i = 0; i < RA; ++i)
+#pragma unroll
+            for (int j = 0; j < RB; ++j) s[i][j] = fmaf(x[i], y[j], s[i][j]);
+    }
+}
+
+// acc[i][c] += sum over the K columns of w[RA * ty + i][column] * b[tx + 16 c][column]
+template <int RA, int NC, int K>
+__device__ __forceinline__ void accumulate(float (&acc)[RA][NC], const float *w, const float *b, int ty, int tx, bool bad)
+{
+    constexpr int P = K + 4;
+    w += RA * ty * P;
+    b += tx * P;
+    if (!bad) {
+#pragma unroll 2
+        for (int j = 0; j < K; j += 4) {
+            float4 x[RA];
+#pragma unroll
+            for (int i = 0; i < RA; ++i) x[i] = *reinterpret_cast<const float4 *>(w + i * P + j);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float4 y = *reinterpret_cast<const float4 *>(b + 16 * c * P + j);
+#pragma unroll
+                for (int i = 0; i < RA; ++i)
+                    acc[i][c] = fmaf(x[i].w, y.w, fmaf(x[i].z, y.z, fmaf(x[i].y, y.y, fmaf(x[i].x, y.x, acc[i][c]))));
+            }
+        }
+        return;
+    }
+    for (int j = 0; j < K; ++j) {
+#pragma unroll
+        for (int i = 0; i < RA; ++i) {
+            const float x = w[i * P + j];
+            if (x == 0.0f) continue;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) acc[i][c] = fmaf(x, b[16 * c * P + j], acc[i][c]);
+        }
+    }
+}
+
+// The score in units of log2 of a pair whose scaled product is x, and the slope of the cap there.
+__device__ __forceinline__ float any_score(const GlobalParams &p, float product, float &slant)
+{
+    float x = product * p.scale;
+    slant = 1.0f;
+    if (p.cap != 0.0f) {
+        const float t = tanhf(x / p.cap);
+        slant = 1.0f - t * t;
+        x = p.cap * t;
+    }
+    return x * kLog2e;
+}
+
+struct RowOf {
+    int n, head;
+};
+
+__device__ __forceinline__ RowOf row_of(const GlobalParams &p, int kh, int r)
+{
+    const int n = r / p.g;
+    return {n, kh * p.g + r - n * p.g};
+}
+
+template <typename T>
+__device__ __forceinline__ const T *at(const void *base, const long long (&s)[3], int b, int n, int head)
+{
+    return static_cast<const T *>(base) + b * s[0] + n * s[1] + head * s[2];
+}
+
+// lowest and highest document of the block's rows, in shared memory
+__device__ __forceinline__ void row_documents(const GlobalParams &p, int b, int r0, int rows, int *range)
+{
+    if (threadIdx.x == 0) range[0] = 0x7fffffff, range[1] = -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows; i += kAnyThreads) {
+        const int n = (r0 + i) / p.g;
+        if (n >= p.N) continue;
+        const int doc = p.q_docs[static_cast<long long>(b) * p.N + n];
+        if (doc < 0) continue;
+        atomicMin(range, doc);
+        atomicMax(range + 1, doc);
+    }
+    __syncthreads();
+}
+
+template <typename T, int DP, int RM, int RN>
+__global__ void __launch_bounds__(kAnyThreads) global_any_forward_kernel(const GlobalParams p)
+{
+    chain_begin();
+    constexpr int BM = 16 * RM, BN = 16 * RN, PM = BM + 4, PN = BN + 4, NC = DP / 16;
+    extern __shared__ __align__(16) float smem[];
+    float *qt = smem, *kvt = qt + DP * PM, *w = kvt + DP * PN;
+    float2 *place = reinterpret_cast<float2 *>(w + BM * PN);
+    int *doc = reinterpret_cast<int *>(place + BN), *range = doc + BN;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int r0 = blockIdx.x * BM, kh = blockIdx.y, b = blockIdx.z % p.B, split = blockIdx.z / p.B;
+    const int rows = p.N * p.g;
+    const GlobalMask mask = global_mask(p, b);
+
+    load_transposed<T, DP, BM>(qt, p.d, p.vec, [&](int r) -> const T * {
+        if (r0 + r >= rows) return nullptr;
+        const RowOf t = row_of(p, kh, r0 + r);
+        return at<T>(p.q, p.qs, b, t.n, t.head);
+    });
+    if (p.q_docs) row_documents(p, b, r0, BM, range);
+
+    float acc[RM][NC] = {}, top[RM], sum[RM], slope[RM];
+    float2 here[RM];
+    int n_of[RM], doc_of[RM];
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+        const int r = min(r0 + RM * ty + i, rows - 1);
+        const RowOf t = row_of(p, kh, r);
+        top[i] = -INFINITY;
+        sum[i] = 0.0f;
+        n_of[i] = t.n;
+        slope[i] = p.slopes ? p.slopes[t.head] * kLog2e : 0.0f;
+        here[i] = map_place(t.n + mask.shift, p.width);
+        doc_of[i] = p.q_docs ? p.q_docs[static_cast<long long>(b) * p.N + t.n] : 0;
+    }
+    const int end = key_end(mask, (min(r0 + BM, rows) - 1) / p.g);
+    const int t_end = p.splits > 1 ? min((end + BN - 1) / BN, (split + 1) * p.tiles_per_split) : (end + BN - 1) / BN;
+    for (int t = split * p.tiles_per_split; t < t_end; ++t) {
+        const int j0 = t * BN;
+        __syncthreads();
+        bool any = true;
+        if (tid < BN) {
+            const int j = j0 + tid;
+            place[tid] = map_place(j, p.width);
+            if (p.k_docs) {
+                const int dk = j < p.M ? p.k_docs[static_cast<long long>(b) * p.M + j] : -1;
+                doc[tid] = dk;
+                any = dk >= range[0] && dk <= range[1];
+            }
+        } else if (p.k_docs) {
+            any = false;
+        }
+        if (p.k_docs && !__syncthreads_or(any)) continue;
+        load_transposed<T, DP, BN>(kvt, p.d, p.vec, [&](int r) -> const T * {
+            return j0 + r < mask.len ? at<T>(p.k, p.ks, b, j0 + r, kh) : nullptr;
+        });
+        __syncthreads();
+        float s[RM][RN] = {};
+        products<RM, RN, PM, PN>(s, qt, kvt, p.d, ty, tx);
+        float high[RM];
+#pragma unroll
+        for (int i = 0; i < RM; ++i) {
+            high[i] = top[i];
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                const int c = RN * tx + j;
+                float slant;
+                float x = any_score(p, s[i][j], slant);
+                if (p.slopes) x -= slope[i] * map_distance(here[i], place[c]);
+                const bool seen = sees(mask, n_of[i], j0 + c) && (!p.k_docs || (doc[c] == doc_of[i] && doc[c] >= 0));
+                s[i][j] = seen ? x : -INFINITY;
+                high[i] = fmaxf(high[i], s[i][j]);
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], o));
+            const float ref = high[i] == -INFINITY ? 0.0f : high[i];
+            const float shrink = exp2f(top[i] - ref);
+            top[i] = high[i];
+            sum[i] *= shrink;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) acc[i][c] *= shrink;
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                const float e = exp2f(s[i][j] - ref);
+                sum[i] += e;
+                w[(RM * ty + i) * PN + RN * tx + j] = e;
+            }
+        }
+        __syncthreads();
+        const bool odd = load_transposed<T, DP, BN>(kvt, p.d, p.vec, [&](int r) -> const T * {
+            return j0 + r < mask.len ? at<T>(p.v, p.vs, b, j0 + r, kh) : nullptr;
+        });
+        const bool bad = __syncthreads_or(odd);
+        accumulate<RM, NC, BN>(acc, w, kvt, ty, tx, bad);
+    }
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+        const int r = r0 + RM * ty + i;
+        if (r >= rows) continue;
+        const RowOf t = row_of(p, kh, r);
+        const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
+        const bool empty = sum[i] == 0.0f;
+        const long long row = (static_cast<long long>(b) * p.h + t.head) * p.N + t.n;
+        const float lse = top[i] + log2f(sum[i]);
+        if (p.splits > 1) {
+            const long long part = static_cast<long long>(split) * p.B * p.h * p.N + row;
+            if (tx == 0) p.part_lse[part] = empty ? -INFINITY : lse;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (tx + 16 * c < p.d) p.part_out[part * p.d + tx + 16 * c] = empty ? 0.0f : acc[i][c] * inv;
+        } else {
+            if (p.lse && tx == 0) p.lse[row] = empty ? INFINITY : lse;
+            T *out = static_cast<T *>(p.out) + ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (tx + 16 * c < p.d) store_one<T>(out + tx + 16 * c, empty ? 0.0f : acc[i][c] * inv);
+        }
+    }
+}
+
+// dS of a pair from its scaled product, dP and the row's figures; p is the probability.
+__device__ __forceinline__ float any_slope(const GlobalParams &p, float product, float dp, float bias, float lse, float delta, bool seen,
+                                           float &prob)
+{
+    float slant;
+    const float x = any_score(p, product, slant) - bias;
+    prob = seen ? exp2f(x - lse) : 0.0f;
+    return seen ? prob * slant * (dp - delta) : 0.0f;
+}
+
+// dQ: the rows of the forward kernel, scores and probabilities recomputed.
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(kAnyThreads) global_any_dq_kernel(const GlobalParams p)
+{
+    chain_begin();
+    constexpr int BT = 16 * R, P = BT + 4, NC = DP / 16;
+    extern __shared__ __align__(16) float smem[];
+    float *qt = smem, *dot = qt + DP * P, *kt = dot + DP * P, *vt = kt + DP * P, *w = vt + DP * P;
+    float2 *place = reinterpret_cast<float2 *>(w + BT * P);
+    int *doc = reinterpret_cast<int *>(place + BT), *range = doc + BT;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int r0 = blockIdx.x * BT, kh = blockIdx.y, b = blockIdx.z, rows = p.N * p.g;
+    const GlobalMask mask = global_mask(p, b);
+    load_transposed<T, DP, BT>(qt, p.d, p.vec, [&](int r) -> const T * {
+        if (r0 + r >= rows) return nullptr;
+        const RowOf t = row_of(p, kh, r0 + r);
+        return at<T>(p.q, p.qs, b, t.n, t.head);
+    });
+    load_transposed<T, DP, BT>(dot, p.d, p.vec, [&](int r) -> const T * {
+        if (r0 + r >= rows) return nullptr;
+        const RowOf t = row_of(p, kh, r0 + r);
+        return static_cast<const T *>(p.d_out) + ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
+    });
+    if (p.q_docs) row_documents(p, b, r0, BT, range);
+    float acc[R][NC] = {}, lse[R], delta[R], slope[R];
+    float2 here[R];
+    int n_of[R], doc_of[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const RowOf t = row_of(p, kh, min(r0 + R * ty + i, rows - 1));
+        const long long row = (static_cast<long long>(b) * p.h + t.head) * p.N + t.n;
+        lse[i] = p.lse[row];
+        delta[i] = p.delta[row];
+        n_of[i] = t.n;
+        slope[i] = p.slopes ? p.slopes[t.head] * kLog2e : 0.0f;
+        here[i] = map_place(t.n + mask.shift, p.width);
+        doc_of[i] = p.q_docs ? p.q_docs[static_cast<long long>(b) * p.N + t.n] : 0;
+    }
+    const int end = key_end(mask, (min(r0 + BT, rows) - 1) / p.g);
+    for (int j0 = 0; j0 < end; j0 += BT) {
+        __syncthreads();
+        bool any = true;
+        if (tid < BT) {
+            const int j = j0 + tid;
+            place[tid] = map_place(j, p.width);
+            if (p.k_docs) {
+                const int dk = j < p.M ? p.k_docs[static_cast<long long>(b) * p.M + j] : -1;
+                doc[tid] = dk;
+                any = dk >= range[0] && dk <= range[1];
+            }
+        } else if (p.k_docs) {
+            any = false;
+        }
+        if (p.k_docs && !__syncthreads_or(any)) continue;
+        const bool odd = load_transposed<T, DP, BT>(kt, p.d, p.vec, [&](int r) -> const T * {
+            return j0 + r < mask.len ? at<T>(p.k, p.ks, b, j0 + r, kh) : nullptr;
+        });
+        load_transposed<T, DP, BT>(vt, p.d, p.vec, [&](int r) -> const T * {
+            return j0 + r < mask.len ? at<T>(p.v, p.vs, b, j0 + r, kh) : nullptr;
+        });
+        const bool bad = __syncthreads_or(odd);
+        float s[R][R] = {}, dp[R][R] = {};
+        products<R, R, P, P>(s, qt, kt, p.d, ty, tx);
+        products<R, R, P, P>(dp, dot, vt, p.d, ty, tx);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const int c = R * tx + j;
+                const float bias = p.slopes ? slope[i] * map_distance(here[i], place[c]) : 0.0f;
+                const bool seen = sees(mask, n_of[i], j0 + c) && (!p.k_docs || (doc[c] == doc_of[i] && doc[c] >= 0));
+                float prob;
+                w[(R * ty + i) * P + c] = any_slope(p, s[i][j], dp[i][j], bias, lse[i], delta[i], seen, prob);
+            }
+        __syncthreads();
+        accumulate<R, NC, BT>(acc, w, kt, ty, tx, bad);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = r0 + R * ty + i;
+        if (r >= rows) continue;
+        const RowOf t = row_of(p, kh, r);
+        T *out = static_cast<T *>(p.d_q) + ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if (tx + 16 * c < p.d) store_one<T>(out + tx + 16 * c, acc[i][c] * p.scale);
+    }
+}
+
+// dK and dV: a block owns a tile of keys of one key head and walks the query rows of all heads that share it.
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const GlobalParams p)
+{
+    chain_begin();
+    constexpr int BT = 16 * R, P = BT + 4, NC = DP / 16;
+    extern __shared__ __align__(16) float smem[];
+    float *qt = smem, *dot = qt + DP * P, *kt = dot + DP * P, *vt = kt + DP * P, *w = vt + DP * P;
+    float2 *place = reinterpret_cast<float2 *>(w + BT * P);
+    float *lse = reinterpret_cast<float *>(place + BT), *delta = lse + BT, *slope = delta + BT;
+    int *n_of = reinterpret_cast<int *>(slope + BT), *doc = n_of + BT, *range = doc + BT;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int j0 = blockIdx.x * BT, kh = blockIdx.y, b = blockIdx.z, rows = p.N * p.g;
+    const GlobalMask mask = global_mask(p, b);
+    const bool odd_k = load_transposed<T, DP, BT>(kt, p.d, p.vec, [&](int r) -> const T * {
+        return j0 + r < mask.len ? at<T>(p.k, p.ks, b, j0 + r, kh) : nullptr;
+    });
+    static_cast<void>(odd_k);
+    load_transposed<T, DP, BT>(vt, p.d, p.vec, [&](int r) -> const T * {
+        return j0 + r < mask.len ? at<T>(p.v, p.vs, b, j0 + r, kh) : nullptr;
+    });
+    float acc_k[R][NC] = {}, acc_v[R][NC] = {};
+    float2 here[R];
+    int doc_of[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int j = j0 + R * ty + i;
+        here[i] = map_place(j, p.width);
+        doc_of[i] = p.k_docs && j < p.M ? p.k_docs[static_cast<long long>(b) * p.M + j] : p.k_docs ? -1 : 0;
+    }
+    if (p.k_docs) {
+        if (tid == 0) range[0] = 0x7fffffff, range[1] = -1;
+        __syncthreads();
+        if (tx == 0) {
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (doc_of[i] >= 0) {
+                    atomicMin(range, doc_of[i]);
+                    atomicMax(range + 1, doc_of[i]);
+                }
+        }
+        __syncthreads();
+    }
+    const long long first = static_cast<long long>(query_begin(mask, j0)) * p.g;
+    for (int r0 = first < rows ? static_cast<int>(first) / BT * BT : rows; r0 < rows; r0 += BT) {
+        __syncthreads();
+        bool any = true;
+        if (tid < BT) {
+            const bool in = r0 + tid < rows;
+            const RowOf t = row_of(p, kh, min(r0 + tid, rows - 1));
+            const long long row = (static_cast<long long>(b) * p.h + t.head) * p.N + t.n;
+            place[tid] = map_place(t.n + mask.shift, p.width);
+            lse[tid] = p.lse[row];
+            delta[tid] = p.delta[row];
+            slope[tid] = p.slopes ? p.slopes[t.head] * kLog2e : 0.0f;
+            n_of[tid] = in ? t.n : -1;
+            if (p.q_docs) {
+                const int dq = in ? p.q_docs[static_cast<long long>(b) * p.N + t.n] : -1;
+                doc[tid] = dq;
+                any = dq >= range[0] && dq <= range[1];
+            }
+        } else if (p.q_docs) {
+            any = false;
+        }
+        if (p.q_docs && !__syncthreads_or(any)) continue;
+        const bool odd_q = load_transposed<T, DP, BT>(qt, p.d, p.vec, [&](int r) -> const T * {
+            if (r0 + r >= rows) return nullptr;
+            const RowOf t = row_of(p, kh, r0 + r);
+            return at<T>(p.q, p.qs, b, t.n, t.head);
+        });
+        const bool odd_o = load_transposed<T, DP, BT>(dot, p.d, p.vec, [&](int r) -> const T * {
+            if (r0 + r >= rows) return nullptr;
+            const RowOf t = row_of(p, kh, r0 + r);
+            return static_cast<const T *>(p.d_out) + ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
+        });
+        const bool bad = __syncthreads_or(odd_q || odd_o);
+        float s[R][R] = {}, dp[R][R] = {};
+        products<R, R, P, P>(s, kt, qt, p.d, ty, tx);
+        products<R, R, P, P>(dp, vt, dot, p.d, ty, tx);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const int c = R * tx + j;
+                const float bias = p.slopes ? slope[c] * map_distance(here[i], place[c]) : 0.0f;
+                const bool seen = n_of[c] >= 0 && sees(mask, n_of[c], j0 + R * ty + i) && (!p.k_docs || (doc[c] == doc_of[i] && doc[c] >= 0));
+                float prob;
+                dp[i][j] = any_slope(p, s[i][j], dp[i][j], bias, lse[c], delta[c], seen, prob);
+                w[(R * ty + i) * P + c] = prob;
+            }
+        __syncthreads();
+        accumulate<R, NC, BT>(acc_v, w, dot, ty, tx, bad);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < R; ++j) w[(R * ty + i) * P + R * tx + j] = dp[i][j];
+        __syncthreads();
+        accumulate<R, NC, BT>(acc_k, w, qt, ty, tx, bad);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int j = j0 + R * ty + i;
+        if (j >= p.M) continue;
+        const long long o = ((static_cast<long long>(b) * p.M + j) * p.hk + kh) * p.d;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if (tx + 16 * c < p.d) {
+                store_one<T>(static_cast<T *>(p.d_k) + o + tx + 16 * c, acc_k[i][c] * p.scale);
+                store_one<T>(static_cast<T *>(p.d_v) + o + tx + 16 * c, acc_v[i][c]);
+            }
+    }
+}
+
+template <typename... A>
+cudaError_t launch_any(void (*kernel)(GlobalParams), dim3 grid, size_t smem, cudaStream_t stream, const GlobalParams &p)
+{
+    // per device and cheap; more than 48 KB needs the attribute
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (err != cudaSuccess) return err;
+    return launch_chained(kernel, grid, kAnyThreads, smem, stream, p);
+}
+
+template <typename T, int DP, int RM, int RN>
+cudaError_t forward_one(const GlobalParams &p, cudaStream_t stream)
+{
+    constexpr int BM = 16 * RM, BN = 16 * RN;
+    constexpr size_t smem = sizeof(float) * (DP * (BM + 4) + DP * (BN + 4) + BM * (BN + 4) + 2 * BN + BN + 2);
+    static_assert(smem <= 227 * 1024, "shared memory of a block");
+    const dim3 grid((p.N * p.g + BM - 1) / BM, p.hk, p.B * p.splits);
+    return launch_any(global_any_forward_kernel<T, DP, RM, RN>, grid, smem, stream, p);
+}
+
+template <typename T, int DP>
+cudaError_t forward_width(const GlobalParams &p, cudaStream_t stream)
+{
+    // sixteen rows or fewer (single tokens): a block of sixteen rows
+    if (p.N * p.g <= 16) return forward_one<T, DP, 1, 4>(p, stream);
+    if constexpr (DP > 128) return forward_one<T, DP, 2, 2>(p, stream);
+    else return forward_one<T, DP, 4, 4>(p, stream);
+}
+
+template <typename T, int DP>
+cudaError_t backward_width(const GlobalParams &p, cudaStream_t stream)
+{
+    constexpr int R = DP > 128 ? 2 : 4, BT = 16 * R;
+    constexpr size_t smem = sizeof(float) * (4 * DP * (BT + 4) + BT * (BT + 4) + 7 * BT + 2);
+    static_assert(smem <= 227 * 1024, "shared memory of a block");
+    cudaError_t err = launch_any(global_any_dq_kernel<T, DP, R>, dim3((p.N * p.g + BT - 1) / BT, p.hk, p.B), smem, stream, p);
+    if (err != cudaSuccess) return err;
+    return launch_any(global_any_dkv_kernel<T, DP, R>, dim3((p.M + BT - 1) / BT, p.hk, p.B), smem, stream, p);
+}
+
+template <typename T>
+cudaError_t any_type(const GlobalParams &p, bool back, cudaStream_t stream)
+{
+    if (p.d <= 32) return back ? backward_width<T, 32>(p, stream) : forward_width<T, 32>(p, stream);
+    if (p.d <= 64) return back ? backward_width<T, 64>(p, stream) : forward_width<T, 64>(p, stream);
+    if (p.d <= 128) return back ? backward_width<T, 128>(p, stream) : forward_width<T, 128>(p, stream);
+    return back ? backward_width<T, 256>(p, stream) : forward_width<T, 256>(p, stream);
+}
+
+}  // namespace
+
+cudaError_t run_global_any_forward(const GlobalParams &p, int dtype, cudaStream_t stream)
+{
+    switch (dtype) {
+    case MATCHATTN_F32: return any_type<float>(p, false, stream);
+    case MATCHATTN_F16: return any_type<__half>(p, false, stream);
+    default: return any_type<__nv_bfloat16>(p, false, stream);
+    }
+}
+
+cudaError_t run_global_any_backward(const GlobalParams &p, int dtype, cudaStream_t stream)
+{
+    switch (dtype) {
+    case MATCHATTN_F32: return any_type<float>(p, true, stream);
+    case MATCHATTN_F16: return any_type<__half>(p, true, stream);
+    default: return any_type<__nv_bfloat16>(p, true, stream);
+    }
+}
+
+}  // namespace matchattn

@@ -1,0 +1,206 @@
+// Dense attention: entry points, the choice of kernels, and the small kernels around them.
+#include "matchattn_global.cuh"
+
+namespace matchattn {
+namespace {
+
+// out = sum over the splits of 2^(lse_s - lse) * part_s: a warp per row of a head.  Reads the parts once (float32), bound by
+// their latency: a row has few of them.
+template <typename T>
+__global__ void __launch_bounds__(256) global_join_kernel(const GlobalParams p)
+{
+    chain_begin();
+    const long long rows = static_cast<long long>(p.B) * p.h * p.N;
+    const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 31;
+    float top = -INFINITY;
+    for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_lse[s * rows + row]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.0f, acc[8] = {};
+    const float ref = top == -INFINITY ? 0.0f : top;
+    for (int s = 0; s < p.splits; ++s) {
+        const float x = p.part_lse[s * rows + row];
+        if (x == -INFINITY) continue;          // that share of the keys holds none that the row sees
+        const float w = exp2f(x - ref);
+        sum += w;
+        const float *part = p.part_out + (s * rows + row) * p.d;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (lane + 32 * i < p.d) acc[i] = fmaf(w, part[lane + 32 * i], acc[i]);
+    }
+    const int n = static_cast<int>(row % p.N);
+    const long long bh = row / p.N, b = bh / p.h, head = bh - b * p.h;
+    const bool empty = sum == 0.0f;
+    if (p.lse && lane == 0) p.lse[row] = empty ? INFINITY : ref + log2f(sum);
+    T *out = static_cast<T *>(p.out) + ((b * p.N + n) * p.h + head) * p.d;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < p.d) store_one<T>(out + lane + 32 * i, empty ? 0.0f : acc[i] / sum);
+}
+
+// delta = sum over the channels of d_out * out: a warp per row.  Bound by memory.
+template <typename T>
+__global__ void __launch_bounds__(256) global_delta_kernel(const GlobalParams p)
+{
+    chain_begin();
+    const long long rows = static_cast<long long>(p.B) * p.N * p.h;
+    const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 31;
+    const T *o = static_cast<const T *>(p.out) + row * p.d, *g = static_cast<const T *>(p.d_out) + row * p.d;
+    float sum = 0.0f;
+    for (int c = lane; c < p.d; c += 32) sum = fmaf(load_one<T>(o + c), load_one<T>(g + c), sum);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    const long long bn = row / p.h, head = row - bn * p.h, b = bn / p.N, n = bn - b * p.N;
+    if (lane == 0) p.delta[(b * p.h + head) * p.N + n] = sum;
+}
+
+template <typename F>
+cudaError_t by_type(int dtype, F f)
+{
+    switch (dtype) {
+    case MATCHATTN_F32: return f(float());
+    case MATCHATTN_F16: return f(__half());
+    default: return f(__nv_bfloat16());
+    }
+}
+
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int check_global(const matchattn_global_args *a)
+{
+    if (a == nullptr || !a->q || !a->out || (a->M > 0 && (!a->k || !a->v))) return MATCHATTN_ERR_NULL;
+    if ((a->q_docs == nullptr) != (a->k_docs == nullptr)) return MATCHATTN_ERR_NULL;
+    if (a->B <= 0 || a->N <= 0 || a->M < 0 || a->h <= 0 || a->hk <= 0 || a->h % a->hk != 0 || a->d <= 0 || a->d > MATCHATTN_MAX_DENSE_D ||
+        a->width <= 0)
+        return MATCHATTN_ERR_SHAPE;
+    // written so that NaN fails
+    if (!(a->scale > 0.0f && a->scale <= 3.402823466e38f && a->cap >= 0.0f && a->cap <= 3.402823466e38f)) return MATCHATTN_ERR_SHAPE;
+    if (a->prefix && !a->causal) return MATCHATTN_ERR_SHAPE;
+    if (a->dtype < MATCHATTN_F32 || a->dtype > MATCHATTN_BF16) return MATCHATTN_ERR_DTYPE;
+    const size_t size = a->dtype == MATCHATTN_F32 ? 4 : 2;
+    if (!aligned(a->q, size) || !aligned(a->k, size) || !aligned(a->v, size) || !aligned(a->out, size) || !aligned(a->lse, 4) ||
+        !aligned(a->slopes, 4) || !aligned(a->prefix, 4) || !aligned(a->lengths, 4) || !aligned(a->q_docs, 4) || !aligned(a->k_docs, 4))
+        return MATCHATTN_ERR_ALIGN;
+    // positions are exact in float32; rows of a key head and grid dimensions are 32- and 16-bit
+    if (a->N > (1 << 24) || a->M > (1 << 24) || a->h > 65535 || a->B > 65535 || 1LL * a->N * (a->h / a->hk) > (1LL << 30))
+        return MATCHATTN_ERR_TOO_LARGE;
+    return MATCHATTN_OK;
+}
+
+// Shares of the keys of a forward call with few blocks: enough to fill the SMs, none shorter than four tiles.
+int splits_of(long long blocks, int tiles, int B)
+{
+    const long long fill = sm_count();
+    if (blocks >= fill / 2 || tiles < 8) return 1;
+    long long s = (2 * fill) / blocks;
+    if (s > tiles / 4) s = tiles / 4;
+    if (s > 64) s = 64;
+    while (s > 1 && s * B > 65535) --s;
+    return s < 2 ? 1 : static_cast<int>(s);
+}
+
+struct Plan {
+    int splits, tiles_per_split;
+    size_t part_out, part_lse;      // floats
+};
+
+Plan plan_forward(const matchattn_global_args *a)
+{
+    const int g = a->h / a->hk, rows = a->N * g;
+    const int bm = any_forward_rows(rows, a->d), bn = any_forward_keys(rows, a->d);
+    const long long blocks = 1LL * ((rows + bm - 1) / bm) * a->hk * a->B;
+    const int tiles = (a->M + bn - 1) / bn;
+    Plan p{};
+    p.splits = splits_of(blocks, tiles, a->B);
+    p.tiles_per_split = p.splits > 1 ? (tiles + p.splits - 1) / p.splits : tiles;
+    if (p.splits > 1) {
+        p.splits = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
+        p.part_lse = static_cast<size_t>(p.splits) * a->B * a->h * a->N;
+        p.part_out = p.part_lse * a->d;
+    }
+    return p;
+}
+
+GlobalParams params_of(const matchattn_global_args *a)
+{
+    GlobalParams p{};
+    p.q = a->q, p.k = a->k, p.v = a->v, p.out = a->out, p.lse = a->lse;
+    for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i], p.ks[i] = a->k_stride[i], p.vs[i] = a->v_stride[i];
+    p.slopes = a->slopes, p.prefix = a->prefix, p.lengths = a->lengths, p.q_docs = a->q_docs, p.k_docs = a->k_docs;
+    p.B = a->B, p.N = a->N, p.M = a->M, p.h = a->h, p.hk = a->hk, p.g = a->h / a->hk, p.d = a->d;
+    p.causal = a->causal != 0, p.width = a->width, p.scale = a->scale, p.cap = a->cap;
+    p.splits = 1;
+    const size_t run = 4 * (a->dtype == MATCHATTN_F32 ? 4 : 2);
+    bool vec = a->d % 4 == 0 && aligned(a->q, run) && aligned(a->k, run) && aligned(a->v, run);
+    for (int i = 0; i < 3; ++i) vec = vec && a->q_stride[i] % 4 == 0 && a->k_stride[i] % 4 == 0 && a->v_stride[i] % 4 == 0;
+    p.vec = vec;
+    return p;
+}
+
+size_t backward_floats(const matchattn_global_args *a) { return static_cast<size_t>(a->B) * a->h * a->N; }
+
+}  // namespace
+}  // namespace matchattn
+
+using namespace matchattn;
+
+extern "C" size_t matchattn_global_scratch_bytes(const matchattn_global_args *a, int backward)
+{
+    if (check_global(a) != MATCHATTN_OK || a->M == 0) return 0;
+    if (backward) return sizeof(float) * backward_floats(a);
+    const Plan plan = plan_forward(a);
+    return sizeof(float) * (plan.part_out + plan.part_lse);
+}
+
+extern "C" int matchattn_global_forward(const matchattn_global_args *a, void *scratch, size_t scratch_bytes, void *cuda_stream)
+{
+    const int bad = check_global(a);
+    if (bad != MATCHATTN_OK) return bad;
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    const size_t size = a->dtype == MATCHATTN_F32 ? 4 : 2;
+    GlobalParams p = params_of(a);
+    if (a->M == 0) {        // no key at all: zeros (lse, for the backward pass, is not read then)
+        return status_of(cudaMemsetAsync(a->out, 0, static_cast<size_t>(a->B) * a->N * a->h * a->d * size, stream));
+    }
+    const Plan plan = plan_forward(a);
+    p.splits = plan.splits, p.tiles_per_split = plan.tiles_per_split;
+    if (plan.splits > 1) {
+        if (scratch == nullptr) return MATCHATTN_ERR_NULL;
+        if (scratch_bytes < sizeof(float) * (plan.part_out + plan.part_lse)) return MATCHATTN_ERR_SCRATCH_LIMIT;
+        if (!aligned(scratch, 16)) return MATCHATTN_ERR_ALIGN;
+        p.part_out = static_cast<float *>(scratch);
+        p.part_lse = p.part_out + plan.part_out;
+    }
+    cudaError_t err = run_global_any_forward(p, a->dtype, stream);
+    if (err == cudaSuccess && plan.splits > 1) {
+        const unsigned blocks = static_cast<unsigned>((plan.part_lse / plan.splits + 7) / 8);
+        err = by_type(a->dtype, [&](auto t) { return launch_chained(global_join_kernel<decltype(t)>, dim3(blocks), 256, 0, stream, p); });
+    }
+    return status_of(err);
+}
+
+extern "C" int matchattn_global_backward(const matchattn_global_args *a, const void *d_out, void *d_q, void *d_k, void *d_v, void *scratch,
+                                         size_t scratch_bytes, void *cuda_stream)
+{
+    const int bad = check_global(a);
+    if (bad != MATCHATTN_OK) return bad;
+    if (!d_out || !d_q || (a->M > 0 && (!d_k || !d_v || !a->lse || !scratch))) return MATCHATTN_ERR_NULL;
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    const size_t size = a->dtype == MATCHATTN_F32 ? 4 : 2;
+    if (!aligned(d_out, size) || !aligned(d_q, size) || !aligned(d_k, size) || !aligned(d_v, size)) return MATCHATTN_ERR_ALIGN;
+    if (a->M == 0) return status_of(cudaMemsetAsync(d_q, 0, static_cast<size_t>(a->B) * a->N * a->h * a->d * size, stream));
+    if (scratch_bytes < sizeof(float) * backward_floats(a)) return MATCHATTN_ERR_SCRATCH_LIMIT;
+    if (!aligned(scratch, 16)) return MATCHATTN_ERR_ALIGN;
+    GlobalParams p = params_of(a);
+    p.vec = p.vec && aligned(d_out, 4 * size);
+    p.d_out = d_out, p.d_q = d_q, p.d_k = d_k, p.d_v = d_v;
+    p.delta = static_cast<float *>(scratch);
+    const unsigned blocks = static_cast<unsigned>((backward_floats(a) + 7) / 8);
+    cudaError_t err = by_type(a->dtype, [&](auto t) { return launch_chained(global_delta_kernel<decltype(t)>, dim3(blocks), 256, 0, stream, p); });
+    if (err == cudaSuccess) err = run_global_any_backward(p, a->dtype, stream);
+    return status_of(err);
+}

@@ -1,0 +1,450 @@
+// Norm of every head of q and k and its rotation by the token's position, one pass over both (matchattn_norm_rotary_*).
+//
+//   u = x * rsqrt(mean(x^2) + eps),  g = u * weight
+//   y[i]         = g[i] cos(a_i) - g[i + rot/2] sin(a_i)        i < rot/2
+//   y[i + rot/2] = g[i + rot/2] cos(a_i) + g[i] sin(a_i)        channels from rot on: y = g
+//
+// The angle a_i is position * frequency.  A frequency is a 64-bit fraction of a turn per position: the product with the
+// position wraps at whole turns by itself, so what is left is exact to 2^-32 turns however far the position lies (a float32
+// product is off by 0.06 rad at position 10^6); its upper half goes to sincospif.
+//
+// Backward, from dy and x: dg = dy rotated back, dw = sum dg * u, e = dg * weight, dx = r (e - u mean(e u)).
+//
+// Bound by memory: x in, y out (backward: x, dy in, dx out).  A group of lanes owns a token's row of a head: a lane holds V
+// channels and the V they are paired with, so the rotation stays in the lane, a row is read once, and mean and rotation work from
+// registers; V channels are one load of up to 16 bytes.  The group takes several heads of its token in turn, because the angles (a
+// sincospif per pair, as many instructions as a head's row altogether) are the token's.  All sums are float32, results are rounded once.
+// The weights' gradients are summed per lane over the rows of a block, then over the block, then over the blocks by a second
+// kernel, always in the same order: no atomics.
+#include "matchattn_kernels.cuh"
+
+#include <type_traits>
+
+namespace matchattn {
+namespace {
+
+constexpr int kNormThreads = 128;
+constexpr int kNormHeads = 8;            // heads that a group takes in turn at most
+
+struct NormSide {            // queries or keys
+    const void *x, *w, *dy;
+    void *y, *dw;            // forward: the result; backward: dx
+    float *partial;          // [blocks, d]
+    long long stride[3];
+    int heads, chunks, per;  // heads of a token: `chunks` groups of `per`
+    int blocks;
+};
+
+struct NormParams {
+    NormSide side[2];
+    const void *positions;
+    const unsigned long long *freqs;
+    long long pos_item;      // positions per item (0: all items share them)
+    int pos64, axes, rot, B, N, d, w32;
+    float eps, inv_d;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_run(const T *p, float (&x)[V])
+{
+    constexpr int bytes = V * sizeof(T);
+    if constexpr (V == 1) {
+        x[0] = load_one<T>(p);
+    } else {
+        uint32_t w[bytes / 4];
+        if constexpr (bytes == 16) {
+            const uint4 t = *reinterpret_cast<const uint4 *>(p);
+            w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+        } else {
+            const uint2 t = *reinterpret_cast<const uint2 *>(p);
+            w[0] = t.x, w[1] = t.y;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = DT<T>::unpack(w[i / DT<T>::kElemsPerWord], i % DT<T>::kElemsPerWord);
+    }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_run(T *p, const float (&x)[V])
+{
+    constexpr int bytes = V * sizeof(T);
+    if constexpr (V == 1) {
+        store_one<T>(p, x[0]);
+    } else {
+        uint32_t w[bytes / 4];
+#pragma unroll
+        for (int i = 0; i < bytes / 4; ++i) w[i] = DT<T>::pack(x + i * DT<T>::kElemsPerWord);
+        if constexpr (bytes == 16) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+    }
+}
+
+// V channels of a weight in T or float32
+template <typename T, int V>
+__device__ __forceinline__ void load_weight(const NormParams &p, const void *w, int c, float (&x)[V])
+{
+    if (w == nullptr) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = 1.0f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = p.w32 ? static_cast<const float *>(w)[c + i] : load_one<T>(static_cast<const T *>(w) + c + i);
+    }
+}
+
+template <int S, int V>
+struct Turns {
+    float cosine[S][V], sine[S][V];
+};
+
+// first channel of a slot's two runs; slots below `paired` are rotated
+struct Slot {
+    int a, b;
+};
+template <int V>
+__device__ __forceinline__ Slot slot_of(int s, int paired, int rot)
+{
+    return s < paired ? Slot{s * V, s * V + rot / 2} : Slot{rot + 2 * (s - paired) * V, rot + (2 * (s - paired) + 1) * V};
+}
+
+template <int V, int S>
+__device__ __forceinline__ void load_turns(const NormParams &p, int b, int n, int lane, int lanes, int paired, Turns<S, V> &t)
+{
+    long long pos[2] = {0, 0};
+    for (int a = 0; a < p.axes && p.rot > 0; ++a) {
+        const long long i = b * p.pos_item + static_cast<long long>(n) * p.axes + a;
+        pos[a] = p.pos64 ? static_cast<const long long *>(p.positions)[i] : static_cast<const int *>(p.positions)[i];
+    }
+    const int per_axis = p.rot / 2 / max(p.axes, 1);
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+        const int s = lane + k * lanes;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            t.cosine[k][i] = 1.0f;
+            t.sine[k][i] = 0.0f;
+            if (s < paired) {
+                const int pair = s * V + i;
+                const unsigned long long turn = p.freqs[pair] * static_cast<unsigned long long>(pair >= per_axis ? pos[1] : pos[0]);
+                sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077393e-10f, &t.sine[k][i], &t.cosine[k][i]);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float group_sum(float v, int lanes)
+{
+    for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// T: element, V: channels per run, S: slots per lane, BACK: the backward pass
+template <typename T, int V, int S, bool BACK>
+__global__ void __launch_bounds__(kNormThreads) norm_rotary_kernel(const NormParams p, int lanes)
+{
+    chain_begin();
+    __shared__ float reduced[BACK ? kNormThreads * 2 * V : 1];
+    const int second = blockIdx.x >= p.side[0].blocks;
+    const NormSide &s = p.side[second];
+    const int block = blockIdx.x - (second ? p.side[0].blocks : 0);
+    const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = kNormThreads / lanes;
+    const int paired = p.rot / (2 * V);
+    const long long items = static_cast<long long>(p.B) * p.N * s.chunks;
+    float wa[S][V], wb[S][V], dwa[S][V], dwb[S][V];
+    bool has_a[S], has_b[S];
+    Slot at[S];
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+        at[k] = slot_of<V>(lane + k * lanes, paired, p.rot);
+        has_a[k] = at[k].a + V <= p.d && (lane + k * lanes < paired || at[k].a >= p.rot);
+        has_b[k] = at[k].b + V <= p.d;
+#pragma unroll
+        for (int i = 0; i < V; ++i) wa[k][i] = wb[k][i] = dwa[k][i] = dwb[k][i] = 0.0f;
+        if (has_a[k]) load_weight<T, V>(p, s.w, at[k].a, wa[k]);
+        if (has_b[k]) load_weight<T, V>(p, s.w, at[k].b, wb[k]);
+    }
+    // every group of a warp makes the same number of rounds (their sums are taken by the whole warp)
+    const long long step = static_cast<long long>(s.blocks) * groups;
+    for (long long first = static_cast<long long>(block) * groups; first < items; first += step) {
+        const long long item = first + group;
+        const bool on = item < items;
+        const long long token = on ? item / s.chunks : 0;
+        const int h0 = on ? static_cast<int>(item - token * s.chunks) * s.per : 0;
+        const int b = static_cast<int>(token / p.N), n = static_cast<int>(token - static_cast<long long>(b) * p.N);
+        Turns<S, V> t;
+        load_turns<V, S>(p, b, n, lane, lanes, paired, t);
+        const T *row = static_cast<const T *>(s.x) + b * s.stride[0] + n * s.stride[1];
+        const long long flat = token * s.heads * p.d;
+#pragma unroll 2
+        for (int i0 = 0; i0 < s.per; ++i0) {
+            const int head = h0 + i0;
+            const bool live = on && head < s.heads;
+            float xa[S][V], xb[S][V], ga[S][V], gb[S][V], square = 0.0f;
+#pragma unroll
+            for (int k = 0; k < S; ++k) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) xa[k][i] = xb[k][i] = ga[k][i] = gb[k][i] = 0.0f;
+                if (live && has_a[k]) load_run<T, V>(row + head * s.stride[2] + at[k].a, xa[k]);
+                if (live && has_b[k]) load_run<T, V>(row + head * s.stride[2] + at[k].b, xb[k]);
+                if constexpr (BACK) {
+                    const T *dy = static_cast<const T *>(s.dy) + flat + static_cast<long long>(head) * p.d;
+                    if (live && has_a[k]) load_run<T, V>(dy + at[k].a, ga[k]);
+                    if (live && has_b[k]) load_run<T, V>(dy + at[k].b, gb[k]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < S; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) square = fmaf(xa[k][i], xa[k][i], fmaf(xb[k][i], xb[k][i], square));
+            const float r = rsqrtf(fmaf(group_sum(square, lanes), p.inv_d, p.eps));
+            T *out = static_cast<T *>(s.y) + flat + static_cast<long long>(head) * p.d;
+            if constexpr (!BACK) {
+#pragma unroll
+                for (int k = 0; k < S; ++k) {
+                    float ya[V], yb[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float u = xa[k][i] * r * wa[k][i], v = xb[k][i] * r * wb[k][i];
+                        ya[i] = lane + k * lanes < paired ? u * t.cosine[k][i] - v * t.sine[k][i] : u;
+                        yb[i] = lane + k * lanes < paired ? v * t.cosine[k][i] + u * t.sine[k][i] : v;
+                    }
+                    if (live && has_a[k]) store_run<T, V>(out + at[k].a, ya);
+                    if (live && has_b[k]) store_run<T, V>(out + at[k].b, yb);
+                }
+            } else {
+                float dot = 0.0f;
+#pragma unroll
+                for (int k = 0; k < S; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const bool turned = lane + k * lanes < paired;
+                        const float da = turned ? ga[k][i] * t.cosine[k][i] + gb[k][i] * t.sine[k][i] : ga[k][i];
+                        const float db = turned ? gb[k][i] * t.cosine[k][i] - ga[k][i] * t.sine[k][i] : gb[k][i];
+                        xa[k][i] *= r, xb[k][i] *= r;
+                        if (live) {
+                            dwa[k][i] = fmaf(da, xa[k][i], dwa[k][i]);
+                            dwb[k][i] = fmaf(db, xb[k][i], dwb[k][i]);
+                        }
+                        ga[k][i] = da * wa[k][i], gb[k][i] = db * wb[k][i];
+                        dot = fmaf(ga[k][i], xa[k][i], fmaf(gb[k][i], xb[k][i], dot));
+                    }
+                const float mean = group_sum(dot, lanes) * p.inv_d;
+#pragma unroll
+                for (int k = 0; k < S; ++k) {
+                    float da[V], db[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        da[i] = r * (ga[k][i] - xa[k][i] * mean);
+                        db[i] = r * (gb[k][i] - xb[k][i] * mean);
+                    }
+                    if (live && has_a[k]) store_run<T, V>(out + at[k].a, da);
+                    if (live && has_b[k]) store_run<T, V>(out + at[k].b, db);
+                }
+            }
+        }
+    }
+    if constexpr (BACK) {
+        if (s.partial == nullptr) return;
+#pragma unroll
+        for (int k = 0; k < S; ++k) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                reduced[i * kNormThreads + threadIdx.x] = dwa[k][i];
+                reduced[(V + i) * kNormThreads + threadIdx.x] = dwb[k][i];
+            }
+            __syncthreads();
+            // thread (run element, lane): the sum over the groups
+            for (int e = threadIdx.x; e < 2 * V * lanes; e += kNormThreads) {
+                const int l = e & (lanes - 1), i = e / lanes;
+                const Slot c = slot_of<V>(l + k * lanes, paired, p.rot);
+                const int channel = i < V ? c.a + i : c.b + i - V;
+                float sum = 0.0f;
+                for (int g = 0; g < groups; ++g) sum += reduced[i * kNormThreads + g * lanes + l];
+                if (channel < p.d) s.partial[static_cast<long long>(block) * p.d + channel] = sum;
+            }
+        }
+    }
+}
+
+// dw[c] = sum over the blocks of partial[block][c], in a fixed order; 32 channels x 32 rows of threads
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_weight_kernel(const NormParams p)
+{
+    chain_begin();
+    __shared__ float sums[32][33];
+    const NormSide &s = p.side[blockIdx.y];
+    if (s.partial == nullptr) return;
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    float sum = 0.0f;
+    if (c < p.d)
+        for (int i = threadIdx.y; i < s.blocks; i += 32) sum += s.partial[static_cast<long long>(i) * p.d + c];
+    sums[threadIdx.y][threadIdx.x] = sum;
+    __syncthreads();
+    sum = sums[threadIdx.x][threadIdx.y];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int out = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && out < p.d) {
+        if (p.w32) static_cast<float *>(s.dw)[out] = sum;
+        else store_one<T>(static_cast<T *>(s.dw) + out, sum);
+    }
+}
+
+// The blocks of one side, and how its heads are cut.  Heads in turn share the angles; a small call spreads them instead, so
+// that the chip fills.  Backward blocks are few enough to keep the sums over them short.
+void lay_out(NormSide &s, long long tokens, int groups, bool back, long long wanted)
+{
+    s.per = s.heads < kNormHeads ? s.heads : kNormHeads;
+    while (s.per > 1 && tokens * ((s.heads + s.per - 1) / s.per) < wanted * groups) s.per = (s.per + 1) / 2;
+    s.chunks = (s.heads + s.per - 1) / s.per;
+    const long long items = tokens * s.chunks, blocks = (items + groups - 1) / groups;
+    const long long most = back ? wanted : 1LL << 30;
+    s.blocks = static_cast<int>(blocks < most ? blocks : most);
+}
+
+constexpr int kNormBackBlocks = 4;       // blocks per SM and side of the backward kernel at most
+
+template <typename T, int V, int S>
+cudaError_t run_norm_slots(NormParams &p, bool back, cudaStream_t stream)
+{
+    const int slots = ((p.d + V - 1) / V + 1) / 2;
+    int lanes = 1;
+    while (lanes < 32 && lanes * S < slots) lanes *= 2;
+    const int groups = kNormThreads / lanes;
+    int blocks = 0;
+    for (NormSide &s : p.side) {
+        if (s.heads > 0) lay_out(s, static_cast<long long>(p.B) * p.N, groups, back, 1LL * sm_count() * kNormBackBlocks);
+        blocks += s.blocks;
+    }
+    const cudaError_t err = back ? launch_chained(norm_rotary_kernel<T, V, S, true>, dim3(blocks), kNormThreads, 0, stream, p, lanes)
+                                 : launch_chained(norm_rotary_kernel<T, V, S, false>, dim3(blocks), kNormThreads, 0, stream, p, lanes);
+    if (err != cudaSuccess || (p.side[0].partial == nullptr && p.side[1].partial == nullptr)) return err;
+    return launch_chained(norm_weight_kernel<T>, dim3((p.d + 31) / 32, 2), dim3(32, 32), 0, stream, p);
+}
+
+bool fits(const NormParams &p, int V, size_t size, bool back)
+{
+    if (p.d % V != 0 || p.rot % (2 * V) != 0) return false;
+    for (const NormSide &s : p.side) {
+        if (s.heads == 0) continue;
+        for (const void *a : {s.x, static_cast<const void *>(s.y), back ? s.dy : s.x})
+            if (reinterpret_cast<uintptr_t>(a) % (V * size) != 0) return false;
+        for (long long t : s.stride)
+            if (t % V != 0) return false;
+    }
+    return true;
+}
+
+// The widest runs that the sizes and addresses allow: 16 bytes, 8, single elements.
+template <typename T>
+cudaError_t run_norm(NormParams &p, bool back, cudaStream_t stream)
+{
+    constexpr int wide = 16 / sizeof(T);
+    if (fits(p, wide, sizeof(T), back) && p.d <= 64 * wide) return run_norm_slots<T, wide, 1>(p, back, stream);
+    if constexpr (sizeof(T) == 2) {
+        if (fits(p, 4, sizeof(T), back)) return run_norm_slots<T, 4, 1>(p, back, stream);
+    }
+    return p.d <= 64 ? run_norm_slots<T, 1, 1>(p, back, stream) : run_norm_slots<T, 1, 4>(p, back, stream);
+}
+
+int check_norm(const matchattn_norm_args *a)
+{
+    if (a == nullptr || !a->q || (a->hk > 0 && !a->k)) return MATCHATTN_ERR_NULL;
+    if (a->rot > 0 && (!a->positions || !a->freqs)) return MATCHATTN_ERR_NULL;
+    if (a->B <= 0 || a->N <= 0 || a->h <= 0 || a->hk < 0 || a->d <= 0 || a->d > MATCHATTN_MAX_DENSE_D || a->rot < 0 || a->rot > a->d ||
+        a->axes < 1 || a->axes > 2 || a->rot % (2 * a->axes) != 0 || !(a->eps >= 0.0f) || a->eps > 3.402823466e38f)
+        return MATCHATTN_ERR_SHAPE;
+    if (a->dtype < MATCHATTN_F32 || a->dtype > MATCHATTN_BF16) return MATCHATTN_ERR_DTYPE;
+    if (a->weight_dtype != MATCHATTN_F32 && a->weight_dtype != a->dtype) return MATCHATTN_ERR_DTYPE;
+    const uintptr_t size = a->dtype == MATCHATTN_F32 ? 4 : 2, wsize = a->weight_dtype == MATCHATTN_F32 ? 4 : 2;
+    for (const void *t : {a->q, a->k})
+        if (reinterpret_cast<uintptr_t>(t) % size != 0) return MATCHATTN_ERR_ALIGN;
+    for (const void *t : {a->q_weight, a->k_weight})
+        if (reinterpret_cast<uintptr_t>(t) % wsize != 0) return MATCHATTN_ERR_ALIGN;
+    if (reinterpret_cast<uintptr_t>(a->freqs) % 8 != 0 || reinterpret_cast<uintptr_t>(a->positions) % (a->positions_64 ? 8 : 4) != 0)
+        return MATCHATTN_ERR_ALIGN;
+    if (a->h > (1 << 20) || a->hk > (1 << 20) || 1LL * a->B * a->N * ((a->h > a->hk ? a->h : a->hk)) > (1LL << 31) - 1)
+        return MATCHATTN_ERR_TOO_LARGE;
+    return MATCHATTN_OK;
+}
+
+NormParams norm_params(const matchattn_norm_args *a)
+{
+    NormParams p{};
+    const void *x[2] = {a->q, a->k}, *w[2] = {a->q_weight, a->k_weight};
+    const long long *stride[2] = {a->q_stride, a->k_stride};
+    const int heads[2] = {a->h, a->hk};
+    for (int i = 0; i < 2; ++i) {
+        p.side[i].x = x[i];
+        p.side[i].w = w[i];
+        p.side[i].heads = heads[i];
+        for (int j = 0; j < 3; ++j) p.side[i].stride[j] = stride[i][j];
+    }
+    p.positions = a->positions;
+    p.freqs = static_cast<const unsigned long long *>(a->freqs);
+    p.pos_item = a->positions_per_item;
+    p.pos64 = a->positions_64;
+    p.axes = a->axes;
+    p.rot = a->rot;
+    p.B = a->B, p.N = a->N, p.d = a->d;
+    p.w32 = a->weight_dtype == MATCHATTN_F32;
+    p.eps = a->eps;
+    p.inv_d = 1.0f / static_cast<float>(a->d);
+    return p;
+}
+
+cudaError_t run_norm_type(NormParams &p, int dtype, bool back, cudaStream_t stream)
+{
+    switch (dtype) {
+    case MATCHATTN_F32: return run_norm<float>(p, back, stream);
+    case MATCHATTN_F16: return run_norm<__half>(p, back, stream);
+    default: return run_norm<__nv_bfloat16>(p, back, stream);
+    }
+}
+
+}  // namespace
+}  // namespace matchattn
+
+extern "C" int matchattn_norm_rotary_forward(const matchattn_norm_args *a, void *q_out, void *k_out, void *cuda_stream)
+{
+    using namespace matchattn;
+    const int bad = check_norm(a);
+    if (bad != MATCHATTN_OK) return bad;
+    if (!q_out || (a->hk > 0 && !k_out)) return MATCHATTN_ERR_NULL;
+    NormParams p = norm_params(a);
+    p.side[0].y = q_out;
+    p.side[1].y = k_out;
+    return status_of(run_norm_type(p, a->dtype, false, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+extern "C" size_t matchattn_norm_rotary_scratch_bytes(int d)
+{
+    if (d <= 0 || d > MATCHATTN_MAX_DENSE_D) return 0;
+    return 2 * sizeof(float) * static_cast<size_t>(d) * matchattn::sm_count() * matchattn::kNormBackBlocks;
+}
+
+extern "C" int matchattn_norm_rotary_backward(const matchattn_norm_args *a, const void *d_q_out, const void *d_k_out, void *d_q, void *d_k,
+                                              void *d_q_weight, void *d_k_weight, void *scratch, size_t scratch_bytes, void *cuda_stream)
+{
+    using namespace matchattn;
+    const int bad = check_norm(a);
+    if (bad != MATCHATTN_OK) return bad;
+    if (!d_q_out || !d_q || (a->hk > 0 && (!d_k_out || !d_k))) return MATCHATTN_ERR_NULL;
+    if ((d_q_weight && !a->q_weight) || (d_k_weight && !a->k_weight)) return MATCHATTN_ERR_NULL;
+    if (d_q_weight || d_k_weight) {
+        if (!scratch) return MATCHATTN_ERR_NULL;
+        if (scratch_bytes < matchattn_norm_rotary_scratch_bytes(a->d)) return MATCHATTN_ERR_SCRATCH_LIMIT;
+        if (reinterpret_cast<uintptr_t>(scratch) % 4 != 0) return MATCHATTN_ERR_ALIGN;
+    }
+    NormParams p = norm_params(a);
+    p.side[0].dy = d_q_out, p.side[1].dy = d_k_out;
+    p.side[0].y = d_q, p.side[1].y = d_k;
+    p.side[0].dw = d_q_weight, p.side[1].dw = a->hk > 0 ? d_k_weight : nullptr;
+    float *room = static_cast<float *>(scratch);
+    for (NormSide &s : p.side) {
+        if (s.dw != nullptr) s.partial = room;
+        if (room != nullptr) room += static_cast<size_t>(a->d) * sm_count() * kNormBackBlocks;
+    }
+    return status_of(run_norm_type(p, a->dtype, true, static_cast<cudaStream_t>(cuda_stream)));
+}

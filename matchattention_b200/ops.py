@@ -24,6 +24,7 @@ cover; the Python code here then handles the call or words the error.
 from __future__ import annotations
 
 import contextlib
+import math
 import os
 from typing import List, Optional, Tuple
 
@@ -487,6 +488,194 @@ def flow_init(correlation: torch.Tensor, H: int, W: int, return_debug: bool = Fa
     return (flow, prob, blur, centre) if return_debug else (flow, prob)
 
 
+# ---- dense attention, and the norm and rotation of its queries and keys ------------------------------
+
+def _cuda_float(name: str, t, like=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise RuntimeError(f"matchattn_b200 runs on CUDA tensors only (no CPU fallback); got device {t.device} for {name}")
+    if t.dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {t.dtype} for {name}: float32, float16 or bfloat16")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise TypeError(f"{name} has dtype {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+
+
+def _head_rows(name: str, t):
+    if t.dim() != 4:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected [items, tokens, heads, channels]")
+    if t.size(2) < 1 or not 1 <= t.size(3) <= _lib.MAX_DENSE_D:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}: one head or more of 1 to {_lib.MAX_DENSE_D} channels")
+
+
+def _aside(name: str, t, dtypes, shapes, like):
+    """An argument beside the operands: type, shape (one of `shapes`) and device."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+        raise TypeError(f"{name} must be a tensor of {' or '.join(str(d) for d in dtypes)}")
+    if t.device != like.device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {like.device}")
+    if tuple(t.shape) not in shapes:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {' or '.join(str(s) for s in shapes)}")
+    return t.contiguous().resolve_neg()
+
+
+def _eager_values(tensors):
+    """Plain tensors with their values (for calls that a mode or a subclass kept from the extension)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError("gradients are not available under tensor subclasses, modes and functional transforms")
+    return [t if t is None else (t.resolve_neg() if t.numel() == 0 or t.size(-1) == 1 or t.stride(-1) == 1 else t.contiguous().resolve_neg())
+            for t in tensors]
+
+
+def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0, slopes=None, width: int = 1, causal: bool = False,
+                     prefix=None, lengths=None, documents=None):
+    """Dense softmax attention of every query over every key that the masks leave, with gradients to q, k and v.
+
+    q [B,N,h,d], k and v [B,M,hk,d]; h a multiple of hk (query heads ``[i*h/hk, (i+1)*h/hk)`` share key head i), d up to 256,
+    float32, float16 or bfloat16; any strides (rows whose channels do not lie side by side are copied).  Returns [B,N,h,d].
+
+    Score of query i and key j: ``scale * q_i.k_j`` (``scale`` defaults to ``d ** -0.5``), through ``cap * tanh(x / cap)`` with a
+    ``cap`` above 0, less ``slopes[head] * (|dx| + |dy|)`` with ``slopes`` (float32 [h], constant): dx and dy are the columns and
+    rows between the tokens on a map ``width`` tokens wide; width 1 is their distance in a sequence.
+
+    A key exists below ``lengths[b]`` (int32 [B], clamped to 0..M; all M without it), and query n stands at key position
+    ``lengths[b] - N + n``: new tokens at the end of a cache, or a whole sequence when N is its length.  ``causal`` hides keys
+    behind the query's position, except those below ``prefix[b]`` (int32 [B]).  ``documents``: int32 ids of the tokens, [B,N] for
+    N == M, or a pair for queries and keys; a query sees keys of its own id, and a negative id sees and shows nothing.
+    A query that sees no key gives zeros.  What no query sees, NaN included, does not reach a result.
+
+    Scores, softmax and sums are float32; 16-bit calls round the probabilities to the type for the product with v.  Equal calls
+    give equal bits."""
+    q_docs, k_docs = documents if isinstance(documents, (tuple, list)) and len(documents) == 2 else (documents, documents)
+    if scale is None:
+        scale = q.size(-1) ** -0.5
+    done = _host.global_attention(q, k, v, scale, cap, slopes, width, causal, prefix, lengths, q_docs, k_docs)
+    if done is not None:
+        return done
+    _cuda_float("q", q)
+    _head_rows("q", q)
+    for name, t in (("k", k), ("v", v)):
+        _cuda_float(name, t, q)
+        _head_rows(name, t)
+    B, N, h, d = q.shape
+    M, hk = k.size(1), k.size(2)
+    if tuple(k.shape) != (B, M, hk, d) or v.shape != k.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must both be [{B}, keys, key heads, {d}]")
+    if h % hk:
+        raise ValueError(f"{h} query heads cannot share {hk} key heads evenly")
+    scale, cap, width = float(scale), float(cap), int(width)
+    if not 0 < scale < float("inf") or not 0 <= cap < float("inf"):
+        raise ValueError(f"scale must be positive and finite and cap 0 or positive and finite, got {scale} and {cap}")
+    if width < 1:
+        raise ValueError(f"width must be at least 1, got {width}")
+    if prefix is not None and not causal:
+        raise ValueError("prefix needs causal=True: without it every key is seen already")
+    if slopes is not None and slopes.requires_grad:
+        raise NotImplementedError("slopes are constant: no gradient is formed for them")
+    if (q_docs is None) != (k_docs is None):
+        raise ValueError("documents are ids of the queries and of the keys, or of both at once")
+    slopes = _aside("slopes", slopes, (torch.float32,), [(h,)], q)
+    prefix = _aside("prefix", prefix, (torch.int32,), [(B,)], q)
+    lengths = _aside("lengths", lengths, (torch.int32,), [(B,)], q)
+    q_docs = _aside("documents of the queries", q_docs, (torch.int32,), [(B, N)], q)
+    k_docs = _aside("documents of the keys", k_docs, (torch.int32,), [(B, M)], q)
+    again = _host.global_attention(q, k, v, scale, cap, slopes, width, bool(causal), prefix, lengths, q_docs, k_docs)
+    if again is not None:
+        return again
+    q, k, v = _eager_values((q, k, v))
+    out = q.new_empty(q.shape)
+    if out.numel() == 0:
+        return out
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    args = _lib.GlobalArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), slopes=ptr(slopes), prefix=ptr(prefix),
+                           lengths=ptr(lengths), q_docs=ptr(q_docs), k_docs=ptr(k_docs), B=B, N=N, M=M, h=h, hk=hk, d=d,
+                           q_stride=tuple(q.stride()[:3]), k_stride=tuple(k.stride()[:3]), v_stride=tuple(v.stride()[:3]),
+                           dtype=_DTYPE_CODE[q.dtype], causal=int(bool(causal)), width=width, scale=scale, cap=cap)
+    with torch.cuda.device(q.device):
+        nbytes = int(_lib.lib.matchattn_global_scratch_bytes(args, 0))
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        status = _lib.lib.matchattn_global_forward(args, ptr(scratch), nbytes, torch.cuda.current_stream().cuda_stream)
+    _lib.check(status)
+    return out
+
+
+def rotary_frequencies(rot: int, theta: float = 10000.0, axes: int = 1, device=None) -> torch.Tensor:
+    """The table of norm_rotary for ``rot`` rotated channels: ``theta ** (-j / n)`` radians per position, j < n = rot / 2 / axes, for
+    each of the coordinates (1: sequences, 2: column and row of a map).  int64 [axes, n], turns per position in units of 2^-64
+    (frequencies that were scaled otherwise go into a table of the same form: ``round(f / (2 pi) * 2^64)``, wrapped)."""
+    if axes not in (1, 2) or rot < 0 or rot % (2 * axes):
+        raise ValueError(f"rot must be a multiple of {2 * axes if axes in (1, 2) else 2} for 1 or 2 axes, got rot={rot}, axes={axes}")
+    if not 0 < theta < float("inf"):
+        raise ValueError(f"theta must be positive and finite, got {theta}")
+    n = rot // 2 // axes
+    turns = [round(theta ** (-j / n) / (2 * math.pi) * 2.0 ** 64) % 2 ** 64 for j in range(n)]
+    row = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
+    return torch.tensor([row] * axes, dtype=torch.int64, device=device).view(axes, n)
+
+
+def norm_rotary(q, k=None, freqs=None, positions=None, *, q_weight=None, k_weight=None, eps: float = 1e-6):
+    """RMS norm of every head of q (and k), times a weight per channel, and the rotation by the token's position, in one pass over
+    both, with gradients to q, k and the weights: what stands between the projections and global_attention.
+
+    q [B,N,h,d], k [B,N,hk,d] or None (any strides, as in global_attention); weights [d] in q's dtype or float32, or None (ones).
+    ``freqs`` from rotary_frequencies(rot, axes=...) says how many channels turn: pairs ``(i, i + rot/2)`` by the angle of the token's
+    position, channels from ``rot`` on are left as the norm gives them.  ``positions``: int32 or int64, [N] or [B,N], with two axes
+    [N,2] or [B,N,2] (column, row).  Without ``freqs`` and ``positions`` nothing turns.  Angles are exact to 2^-32 turns at any
+    position.  Returns (q, k), or q alone without k; contiguous, rounded once."""
+    done = _host.norm_rotary(q, k, freqs, positions, q_weight, k_weight, eps)
+    if done is not None:
+        return done if k is not None else done[0]
+    _cuda_float("q", q)
+    _head_rows("q", q)
+    B, N, h, d = q.shape
+    if k is not None:
+        _cuda_float("k", k, q)
+        _head_rows("k", k)
+        if k.shape[:2] != q.shape[:2] or k.size(3) != d:
+            raise ValueError(f"k has shape {tuple(k.shape)}, expected [{B}, {N}, heads, {d}]")
+    elif k_weight is not None:
+        raise ValueError("k_weight without k")
+    eps = float(eps)
+    if not 0 <= eps < float("inf"):
+        raise ValueError(f"eps must be 0 or positive and finite, got {eps}")
+    if (freqs is None) != (positions is None):
+        raise ValueError("freqs and positions go together")
+    axes = 1
+    if freqs is not None:
+        if not isinstance(freqs, torch.Tensor) or freqs.dim() != 2 or freqs.size(0) not in (1, 2) or 2 * freqs.numel() > d:
+            raise ValueError(f"freqs must be a table of rotary_frequencies for at most {d} channels")
+        axes = freqs.size(0)
+        freqs = _aside("freqs", freqs, (torch.int64,), [tuple(freqs.shape)], q)
+        tail = (N,) if axes == 1 else (N, 2)
+        positions = _aside("positions", positions, (torch.int32, torch.int64), [tail, (B, *tail), (1, *tail)], q)
+    weights = tuple(dict.fromkeys((q.dtype, torch.float32)))
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        _aside(name, w, weights, [(d,)], q)
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise TypeError(f"q_weight is {q_weight.dtype}, k_weight {k_weight.dtype}: one type for both")
+    q_weight, k_weight = (w if w is None else w.contiguous().resolve_neg() for w in (q_weight, k_weight))
+    again = _host.norm_rotary(q, k, freqs, positions, q_weight, k_weight, eps)
+    if again is not None:
+        return again if k is not None else again[0]
+    q, k, q_weight, k_weight = _eager_values((q, k, q_weight, k_weight))
+    q_out, k_out = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    if q.numel():
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        weight = q_weight if q_weight is not None else k_weight
+        per_item = N * axes if positions is not None and positions.dim() == axes + 1 and positions.size(0) > 1 else 0
+        args = _lib.NormArgs(q=q.data_ptr(), k=ptr(k), q_stride=tuple(q.stride()[:3]), k_stride=(0, 0, 0) if k is None else tuple(k.stride()[:3]),
+                             q_weight=ptr(q_weight), k_weight=ptr(k_weight), positions=ptr(positions), freqs=ptr(freqs),
+                             positions_per_item=per_item, positions_64=int(positions is not None and positions.dtype == torch.int64),
+                             axes=axes, rot=0 if freqs is None else 2 * freqs.numel(), B=B, N=N, h=h, hk=0 if k is None else k.size(2), d=d,
+                             dtype=_DTYPE_CODE[q.dtype], weight_dtype=_DTYPE_CODE[q.dtype if weight is None else weight.dtype], eps=eps)
+        with torch.cuda.device(q.device):
+            status = _lib.lib.matchattn_norm_rotary_forward(args, q_out.data_ptr(), ptr(k_out), torch.cuda.current_stream().cuda_stream)
+        _lib.check(status)
+    return q_out if k is None else (q_out, k_out)
+
+
 # ---- the fused steps as opaque custom ops ------------------------------------------------------
 # torch.compile cannot trace a ctypes call.  These wrappers give the compiler the same thing the
 # reference gives it for its own extension (models/match_former_ops.py:6-62): an opaque op with a fake
@@ -572,3 +761,27 @@ def flow_init_op(correlation: torch.Tensor, H: int, W: int) -> List[torch.Tensor
 def _(correlation, H, W):
     B, N, _ = correlation.shape
     return [correlation.new_empty(2 * B, H, W, 2), correlation.new_empty(2 * B, H, W, N)]
+
+
+@torch.library.custom_op("matchattn_b200::global_attention_op", mutates_args=())
+def global_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, cap: float, slopes: Optional[torch.Tensor],
+                        width: int, causal: bool, prefix: Optional[torch.Tensor], lengths: Optional[torch.Tensor],
+                        q_documents: Optional[torch.Tensor], k_documents: Optional[torch.Tensor]) -> torch.Tensor:
+    return global_attention(q, k, v, scale=scale, cap=cap, slopes=slopes, width=width, causal=causal, prefix=prefix, lengths=lengths,
+                            documents=None if q_documents is None else (q_documents, k_documents))
+
+
+@global_attention_op.register_fake
+def _(q, k, v, scale, cap, slopes, width, causal, prefix, lengths, q_documents, k_documents):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("matchattn_b200::norm_rotary_op", mutates_args=())
+def norm_rotary_op(q: torch.Tensor, k: torch.Tensor, freqs: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+                   q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float) -> List[torch.Tensor]:
+    return list(norm_rotary(q, k, freqs, positions, q_weight=q_weight, k_weight=k_weight, eps=eps))
+
+
+@norm_rotary_op.register_fake
+def _(q, k, freqs, positions, q_weight, k_weight, eps):
+    return [q.new_empty(q.shape), k.new_empty(k.shape)]
