@@ -13,6 +13,8 @@ namespace matchattn {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+struct DocRange;
+
 struct GlobalParams {
     const void *q, *k, *v;
     void *out;               // [B, N, h, d]
@@ -27,6 +29,8 @@ struct GlobalParams {
     int vec;                            // rows of q, k and v can be read four elements at a time
     // forward with few queries: each split takes a share of the keys, a second kernel joins them
     int splits, tiles_per_split;
+    int block_rows;                     // matrix kernels: queries of a block
+    const DocRange *ranges;      // with documents: of the blocks of 128 queries, then of keys, item by item
     float *part_out, *part_lse;         // [splits, B, h, N, d], [splits, B, h, N]
     // backward
     const void *d_out;                  // [B, N, h, d]

@@ -1,5 +1,5 @@
 // Dense attention: entry points, the choice of kernels, and the small kernels around them.
-#include "matchattn_global.cuh"
+#include "matchattn_global_mma.cuh"
 
 namespace matchattn {
 namespace {
@@ -58,6 +58,28 @@ __global__ void __launch_bounds__(256) global_delta_kernel(const GlobalParams p)
     if (lane == 0) p.delta[(b * p.h + head) * p.N + n] = sum;
 }
 
+// What the ids of a block of 128 tokens span: blocks of queries of all items, then blocks of keys.
+__global__ void __launch_bounds__(kTile) global_ranges_kernel(const GlobalParams p, DocRange *ranges)
+{
+    chain_begin();
+    const int query_tiles = (p.N + kTile - 1) / kTile, key_tiles = (p.M + kTile - 1) / kTile;
+    const bool keys = blockIdx.x >= p.B * query_tiles;
+    const int i = keys ? blockIdx.x - p.B * query_tiles : blockIdx.x, tiles = keys ? key_tiles : query_tiles, rows = keys ? p.M : p.N;
+    const int b = i / tiles, row = (i - b * tiles) * kTile + threadIdx.x;
+    const bool in = row < rows;
+    const int id = in ? (keys ? p.k_docs : p.q_docs)[static_cast<long long>(b) * rows + row] : -1;
+    __shared__ int low, high, impure;
+    if (threadIdx.x == 0) low = 0x7fffffff, high = -1, impure = 0;
+    __syncthreads();
+    if (in && id < 0) impure = 1;
+    if (in && id >= 0) {
+        atomicMin(&low, id);
+        atomicMax(&high, id);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) ranges[blockIdx.x] = DocRange{low, high, !impure, 0};
+}
+
 template <typename F>
 cudaError_t by_type(int dtype, F f)
 {
@@ -103,18 +125,50 @@ int splits_of(long long blocks, int tiles, int B)
     return s < 2 ? 1 : static_cast<int>(s);
 }
 
+// Queries times sharing heads up to which a call counts as one of single tokens.
+constexpr int kTokenRows = 16;
+
+bool matrix_call(const matchattn_global_args *a)
+{
+    return a->dtype != MATCHATTN_F32 && a->d <= 128 && a->d % 8 == 0 && aligned(a->out, 16) && rows_fit(a->q, a->q_stride, a->B, a->N, a->h) &&
+           rows_fit(a->k, a->k_stride, a->B, a->M, a->hk) && rows_fit(a->v, a->v_stride, a->B, a->M, a->hk);
+}
+
 struct Plan {
-    int splits, tiles_per_split;
+    bool matrix;
+    int block_rows, splits, tiles_per_split;
     size_t part_out, part_lse;      // floats
+    size_t ranges;                  // DocRange
+    size_t bytes() const { return ranges * sizeof(DocRange) + sizeof(float) * (part_out + part_lse); }
 };
+
+size_t range_count(const matchattn_global_args *a)
+{
+    return a->q_docs ? static_cast<size_t>(a->B) * ((a->N + kTile - 1) / kTile + (a->M + kTile - 1) / kTile) : 0;
+}
 
 Plan plan_forward(const matchattn_global_args *a)
 {
     const int g = a->h / a->hk, rows = a->N * g;
-    const int bm = any_forward_rows(rows, a->d), bn = any_forward_keys(rows, a->d);
-    const long long blocks = 1LL * ((rows + bm - 1) / bm) * a->hk * a->B;
-    const int tiles = (a->M + bn - 1) / bn;
     Plan p{};
+    p.matrix = rows > kTokenRows && matrix_call(a);
+    int tiles;
+    long long blocks;
+    if (p.matrix) {
+        // two tiles of queries keep the matrix unit and the exponentials busy at once; one where two leave SMs idle
+        blocks = 1LL * ((a->N + 2 * kTile - 1) / (2 * kTile)) * a->h * a->B;
+        p.block_rows = 2 * kTile;
+        if (blocks < sm_count()) {
+            p.block_rows = kTile;
+            blocks = 1LL * ((a->N + kTile - 1) / kTile) * a->h * a->B;
+        }
+        tiles = (a->M + kTile - 1) / kTile;
+        p.ranges = range_count(a);
+    } else {
+        const int bm = any_forward_rows(rows, a->d), bn = any_forward_keys(rows, a->d);
+        blocks = 1LL * ((rows + bm - 1) / bm) * a->hk * a->B;
+        tiles = (a->M + bn - 1) / bn;
+    }
     p.splits = splits_of(blocks, tiles, a->B);
     p.tiles_per_split = p.splits > 1 ? (tiles + p.splits - 1) / p.splits : tiles;
     if (p.splits > 1) {
@@ -123,6 +177,53 @@ Plan plan_forward(const matchattn_global_args *a)
         p.part_out = p.part_lse * a->d;
     }
     return p;
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                              const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's tensor-map encoder, looked up through the runtime (the library does not link libcuda).
+EncodeFn encoder()
+{
+    static const EncodeFn fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        if (status_of(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q)) != MATCHATTN_OK || q != cudaDriverEntryPointSuccess)
+            return static_cast<EncodeFn>(nullptr);
+        return reinterpret_cast<EncodeFn>(f);
+    }();
+    return fn;
+}
+
+// Dimensions without a second element have a stride that nothing uses: one that the encoder accepts.
+cudaError_t tile_map(CUtensorMap *map, const void *base, const long long (&stride)[3], int B, int rows, int heads, int d, int dtype)
+{
+    const EncodeFn encode = encoder();
+    if (encode == nullptr) return cudaErrorNotSupported;
+    const auto bytes = [](long long s, int size) { return static_cast<cuuint64_t>(size > 1 ? 2 * s : 16); };
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(B)};
+    const cuuint64_t strides[3] = {bytes(stride[2], heads), bytes(stride[1], rows), bytes(stride[0], B)};
+    const cuuint32_t box[4] = {64, 1, kTile, 1}, each[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, dtype == MATCHATTN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base),
+                              dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t operand_maps(GlobalMaps &maps, const matchattn_global_args *a)
+{
+    cudaError_t err = tile_map(&maps.q, a->q, a->q_stride, a->B, a->N, a->h, a->d, a->dtype);
+    if (err == cudaSuccess) err = tile_map(&maps.k, a->k, a->k_stride, a->B, a->M, a->hk, a->d, a->dtype);
+    if (err == cudaSuccess) err = tile_map(&maps.v, a->v, a->v_stride, a->B, a->M, a->hk, a->d, a->dtype);
+    return err;
+}
+
+cudaError_t find_ranges(GlobalParams &p, DocRange *ranges, cudaStream_t stream)
+{
+    if (p.q_docs == nullptr) return cudaSuccess;
+    p.ranges = ranges;
+    const unsigned blocks = static_cast<unsigned>(p.B) * ((p.N + kTile - 1) / kTile + (p.M + kTile - 1) / kTile);
+    return launch_chained(global_ranges_kernel, dim3(blocks), kTile, 0, stream, p, ranges);
 }
 
 GlobalParams params_of(const matchattn_global_args *a)
@@ -153,7 +254,7 @@ extern "C" size_t matchattn_global_scratch_bytes(const matchattn_global_args *a,
     if (check_global(a) != MATCHATTN_OK || a->M == 0) return 0;
     if (backward) return sizeof(float) * backward_floats(a);
     const Plan plan = plan_forward(a);
-    return sizeof(float) * (plan.part_out + plan.part_lse);
+    return plan.bytes();
 }
 
 extern "C" int matchattn_global_forward(const matchattn_global_args *a, void *scratch, size_t scratch_bytes, void *cuda_stream)
@@ -167,15 +268,23 @@ extern "C" int matchattn_global_forward(const matchattn_global_args *a, void *sc
         return status_of(cudaMemsetAsync(a->out, 0, static_cast<size_t>(a->B) * a->N * a->h * a->d * size, stream));
     }
     const Plan plan = plan_forward(a);
-    p.splits = plan.splits, p.tiles_per_split = plan.tiles_per_split;
-    if (plan.splits > 1) {
+    p.splits = plan.splits, p.tiles_per_split = plan.tiles_per_split, p.block_rows = plan.block_rows;
+    if (plan.bytes() != 0) {
         if (scratch == nullptr) return MATCHATTN_ERR_NULL;
-        if (scratch_bytes < sizeof(float) * (plan.part_out + plan.part_lse)) return MATCHATTN_ERR_SCRATCH_LIMIT;
+        if (scratch_bytes < plan.bytes()) return MATCHATTN_ERR_SCRATCH_LIMIT;
         if (!aligned(scratch, 16)) return MATCHATTN_ERR_ALIGN;
-        p.part_out = static_cast<float *>(scratch);
+        p.part_out = reinterpret_cast<float *>(static_cast<DocRange *>(scratch) + plan.ranges);
         p.part_lse = p.part_out + plan.part_out;
     }
-    cudaError_t err = run_global_any_forward(p, a->dtype, stream);
+    cudaError_t err;
+    if (plan.matrix) {
+        GlobalMaps maps{};
+        err = operand_maps(maps, a);
+        if (err == cudaSuccess) err = find_ranges(p, static_cast<DocRange *>(scratch), stream);
+        if (err == cudaSuccess) err = run_global_forward(p, maps, a->dtype, stream);
+    } else {
+        err = run_global_any_forward(p, a->dtype, stream);
+    }
     if (err == cudaSuccess && plan.splits > 1) {
         const unsigned blocks = static_cast<unsigned>((plan.part_lse / plan.splits + 7) / 8);
         err = by_type(a->dtype, [&](auto t) { return launch_chained(global_join_kernel<decltype(t)>, dim3(blocks), 256, 0, stream, p); });

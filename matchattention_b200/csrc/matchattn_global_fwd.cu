@@ -1,0 +1,391 @@
+// Dense attention, forward, 16-bit types of up to 128 channels, on the matrix units.
+//
+// A block owns 256 queries of a head as two tiles of 128 (or one tile, when the call has too few for the chip), a thread a query.
+// Warps 0-3 and 4-7 take the softmax of one tile each, warp 8 copies tiles of K and V into a ring of buffers (tensor memory
+// accelerator), one thread of warp 9 issues the products: S = Q K^T into tensor memory, and O += P V with P from tensor memory, where it
+// overwrites the scores.  While one tile's threads take exponentials the matrix unit works on the other's.
+//
+// The softmax keeps a reference per row, not the running maximum itself: O and the sum are scaled down only when a score exceeds
+// the reference by 2^8, so probabilities stay below 2^8 and O in tensor memory is hardly ever touched between products.
+// P is rounded to the type of V (a half step of it, relative, as torch rounds a softmax's result); scores, reference, sum and O are float32.
+//
+// A probability that the mask makes zero meets V all the same in the product, and 0 * NaN is NaN: where a tile is partly
+// hidden, its V is looked through first, and one with infinite or NaN values is added term by term.
+#include "matchattn_global_mma.cuh"
+
+namespace matchattn {
+namespace {
+
+constexpr int kForwardThreads = 320;
+constexpr float kSlack = 8.0f;           // log2 of what a probability may exceed one by
+
+template <int DP>
+struct ForwardShared {
+    static constexpr int kStages = DP == 128 ? 4 : 6;
+    uint8_t q[2][kTileBytes<DP>];
+    uint8_t kv[kStages][kTileBytes<DP>];
+    float2 place[8][kTile];              // per softmax warp: columns and rows of the tile's keys
+    int docs[8][kTile];
+    uint64_t q_full, kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], o_full[2];
+    uint32_t tmem;
+    uint64_t looked[2];                  // a warpgroup has looked through a tile of V
+    int broken, by_hand[2], odd[2][3];
+};
+
+// GENERAL: scores capped or with a bias
+template <typename T, int DP, bool GENERAL>
+__global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(const GlobalParams p, const __grid_constant__ GlobalMaps maps)
+{
+    chain_begin();
+    constexpr int STAGES = ForwardShared<DP>::kStages;
+    extern __shared__ uint8_t raw_shared[];
+    ForwardShared<DP> &sh = *reinterpret_cast<ForwardShared<DP> *>(raw_shared + (1024 - (shared_address(raw_shared) & 1023)) % 1024);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int bh = blockIdx.x % (p.B * p.h), split = blockIdx.x / (p.B * p.h);
+    const int b = bh / p.h, head = bh - b * p.h, kh = head / p.g;
+    // the last queries of a causal call see most: their blocks begin first
+    const int n0 = (gridDim.y - 1 - blockIdx.y) * p.block_rows;
+    const GlobalMask mask = global_mask(p, b);
+    const int key_tiles = (p.M + kTile - 1) / kTile, query_tiles = (p.N + kTile - 1) / kTile;
+    const DocRange *kr = p.q_docs ? p.ranges + p.B * query_tiles + b * key_tiles : nullptr;
+    const DocRange *qr = p.q_docs ? p.ranges + b * query_tiles + n0 / kTile : nullptr;
+    const int tiles = p.block_rows / kTile;          // 1 or 2
+    const auto state = [&](int w, int t) {
+        if (w >= tiles) return static_cast<int>(kHidden);
+        return tile_state(mask, p.N, n0 + w * kTile, t * kTile, qr ? qr + w : nullptr, kr ? kr + t : nullptr);
+    };
+    const int end = (key_limit(mask, min(n0 + p.block_rows, p.N) - 1) + kTile - 1) / kTile;
+    const int t_begin = split * p.tiles_per_split, t_end = p.splits > 1 ? min(end, t_begin + p.tiles_per_split) : end;
+
+    if (tid == 0) {
+        barrier_init(&sh.q_full, 1);
+        for (int i = 0; i < STAGES; ++i) {
+            barrier_init(&sh.kv_full[i], 1);
+            barrier_init(&sh.kv_empty[i], 1);
+        }
+        for (int w = 0; w < 2; ++w) {
+            barrier_init(&sh.s_full[w], 1);
+            barrier_init(&sh.p_full[w], kTile);
+            barrier_init(&sh.o_full[w], 1);
+            barrier_init(&sh.looked[w], kTile);
+            for (int i = 0; i < 3; ++i) sh.odd[w][i] = 0;
+        }
+        sh.broken = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) tmem_take(&sh.tmem);
+    tmem_before();
+    __syncthreads();
+    tmem_after();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp == 8) {
+        // ---- copies: Q, then K and V of every tile that one of the two query tiles sees
+        if (elected()) {
+            barrier_expect(&sh.q_full, tiles * kTileBytes<DP>);
+            for (int w = 0; w < tiles; ++w) load_tile<DP>(sh.q[w], &maps.q, head, n0 + w * kTile, b, &sh.q_full);
+            int n = 0;           // tiles copied, K and V counted apart
+            bool good = true;
+            for (int t = t_begin; t < t_end && good; ++t) {
+                if (state(0, t) == kHidden && state(1, t) == kHidden) continue;
+                for (int i = 0; i < 2 && good; ++i, ++n) {
+                    const int s = n % STAGES;
+                    if (n >= STAGES) good = barrier_wait(&sh.kv_empty[s], (n / STAGES - 1) & 1, &sh.broken);
+                    if (!good) break;
+                    barrier_expect(&sh.kv_full[s], kTileBytes<DP>);
+                    load_tile<DP>(sh.kv[s], i == 0 ? &maps.k : &maps.v, kh, t * kTile, b, &sh.kv_full[s]);
+                }
+            }
+            if (!good) {
+                // copies under way write to this block's memory: it stays until they are done
+                barrier_drain(&sh.q_full, 0);
+                for (int i = n > STAGES ? n - STAGES : 0; i < n; ++i) barrier_drain(&sh.kv_full[i % STAGES], (i / STAGES) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // ---- products
+        if (elected()) {
+            const int steps = (p.d + 15) / 16;
+            const uint32_t score_kind = product_kind<T>(kTile, false), value_kind = product_kind<T>(steps * 16, true);
+            const uint32_t q_at[2] = {shared_address(sh.q[0]), shared_address(sh.q[1])}, kv_at = shared_address(sh.kv[0]);
+            int used[2] = {0, 0}, n = 0;            // tiles that each query tile has taken; buffers
+            int last_state[2] = {kHidden, kHidden}, last_v = 0;
+            bool good = barrier_wait(&sh.q_full, 0, &sh.broken);
+            // O += P V of the tile before, for query tile w
+            const auto values = [&](int w) {
+                if (last_state[w] == kHidden || !good) return;
+                good = barrier_wait(&sh.p_full[w], (used[w] - 1) & 1, &sh.broken);
+                if (!good) return;
+                tmem_after();
+                if (!*static_cast<volatile int *>(&sh.by_hand[w])) {
+                    const uint32_t v = kv_at + last_v * kTileBytes<DP>, out = tmem + 256 + w * kTile, prob = tmem + w * kTile;
+#pragma unroll
+                    for (int s = 0; s < kTile / 16; ++s) product_ts(out, prob + 8 * s, by_rows(v, s), value_kind, used[w] > 1 || s > 0);
+                }
+            };
+            for (int t = t_begin; t < t_end && good; ++t) {
+                const int now[2] = {state(0, t), state(1, t)};
+                if (now[0] == kHidden && now[1] == kHidden) continue;
+                const int k = n % STAGES, v = (n + 1) % STAGES;
+                good = barrier_wait(&sh.kv_full[k], (n / STAGES) & 1, &sh.broken);
+                bool waited = n == 0;
+                for (int w = 0; w < 2 && good; ++w) {
+                    if (!waited && last_state[w] != kHidden) {
+                        // the values of the tile before have landed
+                        good = barrier_wait(&sh.kv_full[last_v], ((n - 1) / STAGES) & 1, &sh.broken);
+                        waited = true;
+                    }
+                    if (good) values(w);
+                    if (now[w] == kHidden || !good) continue;
+                    const uint32_t scores = tmem + w * kTile, key = kv_at + k * kTileBytes<DP>;
+                    tmem_after();
+                    for (int s = 0; s < steps; ++s) product_ss(scores, by_channels(q_at[w], s), by_channels(key, s), score_kind, s > 0);
+                    products_done(&sh.s_full[w]);
+                    ++used[w];
+                }
+                if (!good) break;
+                if (n > 0) products_done(&sh.kv_empty[last_v]);
+                products_done(&sh.kv_empty[k]);
+                last_state[0] = now[0], last_state[1] = now[1];
+                last_v = v;
+                n += 2;
+            }
+            if (good && n > 0) good = barrier_wait(&sh.kv_full[last_v], ((n - 1) / STAGES) & 1, &sh.broken);
+            for (int w = 0; w < 2; ++w) {
+                if (good) values(w);
+                products_done(&sh.o_full[w]);
+            }
+            if (!good) {
+                barrier_drain(&sh.o_full[0], 0);
+                barrier_drain(&sh.o_full[1], 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 8) {
+        // ---- softmax
+        const int w = warp >> 2, row = tid & 127, n = n0 + w * kTile + row;
+        const uint32_t mine = tmem + (static_cast<uint32_t>(warp & 3) << 21);        // lanes 32 (warp mod 4) on
+        const uint32_t scores = mine + w * kTile, out = mine + 256 + w * kTile;
+        const float factor = p.scale * kLog2e;
+        const float inner = p.cap != 0.0f ? 2.0f * factor / p.cap : 0.0f, outer = p.cap * kLog2e;
+        const int doc = p.q_docs && n < p.N ? p.q_docs[static_cast<long long>(b) * p.N + n] : -1;
+        const int limit = p.q_docs && doc < 0 ? 0 : key_limit(mask, n);
+        const float slope = GENERAL && p.slopes ? p.slopes[head] * kLog2e : 0.0f;
+        const float2 here = GENERAL ? map_place(n + mask.shift, p.width) : make_float2(0.0f, 0.0f);
+        float ref = -INFINITY, sum = 0.0f;
+        int used = 0, buffers = 0, looks = 0;
+        bool good = true;
+        for (int t = t_begin; t < t_end; ++t) {
+            const int other = state(1 - w, t), now = state(w, t);
+            if (now == kHidden) {
+                if (other != kHidden) buffers += 2;
+                continue;
+            }
+            const int j0 = t * kTile;
+            if (GENERAL && p.slopes && p.width > 1) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sh.place[warp][lane + 32 * i] = map_place(j0 + lane + 32 * i, p.width);
+            }
+            if (p.q_docs && now == kPartial) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = j0 + lane + 32 * i;
+                    sh.docs[warp][lane + 32 * i] = j < p.M ? p.k_docs[static_cast<long long>(b) * p.M + j] : -1;
+                }
+            }
+            __syncwarp();
+            good = good && barrier_wait(&sh.s_full[w], used & 1, &sh.broken);
+            if (!good) break;
+            tmem_after();
+            // First pass: the final scores' maximum.  Scores that differ from the product's are put back in its place; both
+            // passes go by 32 columns, because 128 of them and the rest do not fit the 168 registers that ten warps have.
+            const bool changed = GENERAL || now == kPartial;
+            float high = -INFINITY;
+            uint32_t raw[2][32];
+            tmem_load32(scores, raw[0]);
+#pragma unroll
+            for (int c = 0; c < kTile; c += 32) {
+                float *x = reinterpret_cast<float *>(raw[c / 32 % 2]);
+                tmem_loaded32(raw[c / 32 % 2]);
+                if (c + 32 < kTile) tmem_load32(scores + c + 32, raw[(c / 32 + 1) % 2]);
+                if constexpr (GENERAL) {
+                    if (p.cap != 0.0f) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] = outer * tanh_of(x[i] * inner);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] *= factor;
+                    }
+                    if (p.slopes) {
+                        if (p.width > 1) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const float4 two = *reinterpret_cast<const float4 *>(&sh.place[warp][c + i]);
+                                x[i] = fmaf(-slope, fabsf(here.x - two.x) + fabsf(here.y - two.y), x[i]);
+                                x[i + 1] = fmaf(-slope, fabsf(here.x - two.z) + fabsf(here.y - two.w), x[i + 1]);
+                            }
+                        } else {
+                            const float from = here.y - static_cast<float>(j0 + c);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) x[i] = fmaf(-slope, fabsf(from - static_cast<float>(i)), x[i]);
+                        }
+                    }
+                }
+                if (now == kPartial) {
+                    if (p.q_docs) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const int4 id = *reinterpret_cast<const int4 *>(&sh.docs[warp][c + i]);
+                            if (j0 + c + i >= limit || id.x != doc) x[i] = -INFINITY;
+                            if (j0 + c + i + 1 >= limit || id.y != doc) x[i + 1] = -INFINITY;
+                            if (j0 + c + i + 2 >= limit || id.z != doc) x[i + 2] = -INFINITY;
+                            if (j0 + c + i + 3 >= limit || id.w != doc) x[i + 3] = -INFINITY;
+                        }
+                    } else {
+                        const int left = limit - j0 - c;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i >= left) x[i] = -INFINITY;
+                    }
+                }
+                if (changed) tmem_store32(scores + c, raw[c / 32 % 2]);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) high = fmaxf(high, x[i]);
+            }
+            if (changed) tmem_stored();
+            if constexpr (!GENERAL) high *= factor;
+            if (used == 0) {
+                ref = high;
+            } else {
+                // (a row that has seen nothing so far has zeros in O and sum: any factor does)
+                const bool grown = high > ref + kSlack;
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float shrink = grown ? (ref == -INFINITY ? 0.0f : exp2_fast(ref - high)) : 1.0f;
+                    ref = grown ? high : ref;
+                    sum *= shrink;
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        tmem_load32(out + c, raw[0]);
+                        tmem_loaded32(raw[0]);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) raw[0][i] = __float_as_uint(__uint_as_float(raw[0][i]) * shrink);
+                        tmem_store32(out + c, raw[0]);
+                    }
+                }
+            }
+            const float base = ref == -INFINITY ? 0.0f : ref;
+            float part[2] = {0.0f, 0.0f};
+            tmem_load32(scores, raw[0]);
+#pragma unroll
+            for (int c = 0; c < kTile; c += 32) {
+                const float *x = reinterpret_cast<const float *>(raw[c / 32 % 2]);
+                tmem_loaded32(raw[c / 32 % 2]);
+                if (c + 32 < kTile) tmem_load32(scores + c + 32, raw[(c / 32 + 1) % 2]);
+                uint32_t packed[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float e0 = exp2_fast(GENERAL ? x[i] - base : fmaf(x[i], factor, -base));
+                    const float e1 = exp2_fast(GENERAL ? x[i + 1] - base : fmaf(x[i + 1], factor, -base));
+                    part[0] += e0;
+                    part[1] += e1;
+                    packed[i / 2] = pack_two<T>(e0, e1);
+                }
+                tmem_store16(scores + c / 2, packed);
+            }
+            sum += part[0] + part[1];
+            tmem_stored();
+            bool hand = false;
+            if (now == kPartial) {
+                const int s = (buffers + 1) % STAGES;
+                good = barrier_wait(&sh.kv_full[s], ((buffers + 1) / STAGES) & 1, &sh.broken);
+                if (good && row_tainted<T, DP>(sh.kv[s], row)) *static_cast<volatile int *>(&sh.odd[w][looks % 3]) = 1;
+                // (the slot after this one was last read two looks ago)
+                if (row == 0) *static_cast<volatile int *>(&sh.odd[w][(looks + 1) % 3]) = 0;
+                barrier_arrive(&sh.looked[w]);
+                good = good && barrier_wait(&sh.looked[w], looks & 1, &sh.broken);
+                hand = __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[w][looks % 3]) != 0);
+                ++looks;
+                if (hand) add_rows<T, DP>(out, scores, sh.kv[s], used > 0);
+            }
+            if (row == 0) sh.by_hand[w] = hand;
+            tmem_before();
+            barrier_arrive(&sh.p_full[w]);
+            ++used;
+            buffers += 2;
+        }
+        if (good) good = barrier_wait(&sh.o_full[w], 0, &sh.broken);
+        tmem_after();
+        const bool empty = sum == 0.0f;
+        const float inv = !good ? NAN : empty ? 0.0f : 1.0f / sum;
+        if (n0 + w * kTile < p.N && w < tiles) {          // a whole warpgroup
+            const long long line = (static_cast<long long>(b) * p.h + head) * p.N + n;
+            const long long part = static_cast<long long>(split) * p.B * p.h * p.N + line;
+            const float lse = ref + log2f(sum);
+            if (n < p.N) {
+                if (p.splits > 1) p.part_lse[part] = empty ? -INFINITY : lse;
+                else if (p.lse) p.lse[line] = empty ? INFINITY : lse;
+            }
+#pragma unroll 1
+            for (int c = 0; c < DP && c < p.d; c += 32) {
+                uint32_t o[32];
+                if (used > 0) {
+                    tmem_load32(out + c, o);
+                    tmem_loaded32(o);
+                }
+                float y[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = empty && good ? 0.0f : __uint_as_float(o[i]) * inv;
+                if (n >= p.N) {
+                    // no such query
+                } else if (p.splits > 1) {
+                    float *to = p.part_out + part * p.d + c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        if (c + i < p.d) *reinterpret_cast<float4 *>(to + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                } else {
+                    T *to = static_cast<T *>(p.out) + ((static_cast<long long>(b) * p.N + n) * p.h + head) * p.d + c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        if (c + i < p.d)
+                            *reinterpret_cast<uint4 *>(to + i) = make_uint4(pack_two<T>(y[i], y[i + 1]), pack_two<T>(y[i + 2], y[i + 3]),
+                                                                            pack_two<T>(y[i + 4], y[i + 5]), pack_two<T>(y[i + 6], y[i + 7]));
+                }
+                __syncwarp();
+            }
+        }
+    }
+    tmem_before();
+    __syncthreads();
+    if (warp == 9) tmem_give(tmem);
+}
+
+template <typename T, int DP, bool GENERAL>
+cudaError_t forward_one(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
+{
+    constexpr size_t smem = sizeof(ForwardShared<DP>) + 1024;
+    static_assert(smem <= 227 * 1024 && smem > 114 * 1024, "one block per SM: it takes all of the tensor memory");
+    const auto kernel = global_forward_kernel<T, DP, GENERAL>;
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (err != cudaSuccess) return err;
+    const dim3 grid(p.B * p.h * p.splits, (p.N + p.block_rows - 1) / p.block_rows);
+    return launch_chained(kernel, grid, kForwardThreads, smem, stream, p, maps);
+}
+
+template <typename T>
+cudaError_t forward_type(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
+{
+    const bool general = p.cap != 0.0f || p.slopes != nullptr;
+    if (p.d <= 64) return general ? forward_one<T, 64, true>(p, maps, stream) : forward_one<T, 64, false>(p, maps, stream);
+    return general ? forward_one<T, 128, true>(p, maps, stream) : forward_one<T, 128, false>(p, maps, stream);
+}
+
+}  // namespace
+
+cudaError_t run_global_forward(const GlobalParams &p, const GlobalMaps &maps, int dtype, cudaStream_t stream)
+{
+    return dtype == MATCHATTN_F16 ? forward_type<__half>(p, maps, stream) : forward_type<__nv_bfloat16>(p, maps, stream);
+}
+
+}  // namespace matchattn

@@ -1,0 +1,362 @@
+// Dense attention on the matrix units: tiles, barriers, tensor maps and the instructions around tcgen05.mma, for the kernels of
+// matchattn_global_fwd.cu and matchattn_global_bwd.cu.
+//
+// Tiles.  128 rows (tokens) of a head, up to 128 channels, as one or two halves of 64 channels; a half is 128 rows of 128 bytes,
+// 16-byte pieces swizzled by the row (piece ^ (row & 7)), as the tensor memory accelerator writes it and the matrix unit reads it.
+// The same tile serves as an operand along its channels (scores) and along its rows (sums over the tokens).  Channels beyond d and
+// rows beyond the tensor arrive as zeros.
+#pragma once
+
+#include <cuda.h>
+
+#include "matchattn_global.cuh"
+
+namespace matchattn {
+
+constexpr int kTile = 128;                        // rows of a tile
+constexpr int kHalfBytes = kTile * 128;           // 128 rows x 64 channels of 16 bits
+
+struct GlobalMaps {
+    CUtensorMap q, k, v, o;       // o: d_out (backward)
+};
+
+// lowest and highest id of a block of 128 tokens (ids that are not negative), and whether the block has no negative one
+struct DocRange {
+    int low, high, pure, unused;
+};
+
+// ---- shared-memory barriers ------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void barrier_init(uint64_t *bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(bar)), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_expect(uint64_t *bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(bar)), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive(uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+
+__device__ __forceinline__ bool barrier_test(uint64_t *bar, uint32_t parity)
+{
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(shared_address(bar)), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+
+__device__ __forceinline__ unsigned long long nanoseconds()
+{
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+
+// No wait of these kernels lasts longer than a tile's copies and products, microseconds; one of this length means that
+// something is broken.  The block then raises its flag, every wait of it ends, and its results are NaN.
+constexpr unsigned long long kWaitLimit = 2000000000ULL;
+
+static __device__ __noinline__ bool barrier_wait_long(uint64_t *bar, uint32_t parity, volatile int *broken)
+{
+    const unsigned long long begin = nanoseconds();
+    for (;;) {
+        if (barrier_test(bar, parity)) return true;
+        if (*broken != 0) return false;
+        if (nanoseconds() - begin > kWaitLimit) {
+            *broken = 1;
+            return false;
+        }
+    }
+}
+
+__device__ __forceinline__ bool barrier_wait(uint64_t *bar, uint32_t parity, volatile int *broken)
+{
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i)
+        if (barrier_test(bar, parity)) return true;
+    return barrier_wait_long(bar, parity, broken);
+}
+
+// After something broke: waits, no longer than the limit either, for what still writes to the block's memory.
+static __device__ __noinline__ void barrier_drain(uint64_t *bar, uint32_t parity)
+{
+    const unsigned long long begin = nanoseconds();
+    while (!barrier_test(bar, parity) && nanoseconds() - begin < kWaitLimit) {}
+}
+
+__device__ __forceinline__ bool elected()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// ---- copies ------------------------------------------------------------------------------------------
+
+// 128 tokens of a head from `token` on, 64 channels per half, into `dst`; the bytes are counted on `bar`
+template <int DP>
+__device__ __forceinline__ void load_tile(void *dst, const CUtensorMap *map, int head, int token, int item, uint64_t *bar)
+{
+#pragma unroll
+    for (int half = 0; half < DP / 64; ++half)
+        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                     " [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                     ::"r"(shared_address(dst) + half * kHalfBytes), "l"(reinterpret_cast<uint64_t>(map)), "r"(half * 64), "r"(head), "r"(token),
+                       "r"(item), "r"(shared_address(bar))
+                     : "memory");
+}
+
+template <int DP>
+constexpr int kTileBytes = DP / 64 * kHalfBytes;
+
+// ---- matrix instructions -------------------------------------------------------------------------------
+
+// Where an operand lies: address, and the distances between its 8-row groups and (rows taken as the sum's axis) its halves.
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t half_distance)
+{
+    return static_cast<uint64_t>((address >> 4) & 0x3fff) | static_cast<uint64_t>((half_distance >> 4) & 0x3fff) << 16 |
+           static_cast<uint64_t>(1024 >> 4) << 32 | 1ULL << 46 | 2ULL << 61;
+}
+
+// channels [16 s, 16 s + 16) of a tile, summed over
+__device__ __forceinline__ uint64_t by_channels(uint32_t tile, int s) { return operand(tile + (s >> 2) * kHalfBytes + (s & 3) * 32, 16); }
+// rows [16 s, 16 s + 16) of a tile, summed over
+__device__ __forceinline__ uint64_t by_rows(uint32_t tile, int s) { return operand(tile + s * 2048, kHalfBytes); }
+
+// Shape and types of a product of 128 rows: float32 sums; b_rows: the second operand is summed over its rows.
+template <typename T>
+__device__ __forceinline__ uint32_t product_kind(int columns, bool b_rows)
+{
+    constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    return 1u << 4 | type << 7 | type << 10 | (b_rows ? 1u << 16 : 0u) | static_cast<uint32_t>(columns >> 3) << 17 | (128u >> 4) << 24;
+}
+
+__device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+                 : "memory");
+}
+
+// the first operand from tensor memory
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+                 : "memory");
+}
+
+// `bar` is arrived at when all products issued so far by this thread are done
+__device__ __forceinline__ void products_done(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// a whole warp: all 512 columns
+__device__ __forceinline__ void tmem_take(uint32_t *where)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_address(where)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_give(uint32_t base)
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
+}
+
+#define MA_R8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
+#define MA_W8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
+
+// 32 columns of the thread's row (a warp: its 32 rows)
+__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t *x)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+                 "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : MA_R8(x, 0), MA_R8(x, 8), MA_R8(x, 16), MA_R8(x, 24)
+                 : "r"(at));
+}
+__device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t *x)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : MA_R8(x, 0) : "r"(at));
+}
+__device__ __forceinline__ uint32_t tmem_load1(uint32_t at)
+{
+    uint32_t x;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(x) : "r"(at));
+    return x;
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *x)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+                 "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::MA_W8(x, 0), MA_W8(x, 8), MA_W8(x, 16), MA_W8(x, 24),
+                 "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t *x)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::MA_W8(x, 0),
+                 MA_W8(x, 8), "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t *x)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::MA_W8(x, 0), "r"(at) : "memory");
+}
+#undef MA_R8
+#undef MA_W8
+
+// Waits for the loads before it; the registers pass through it, so that nothing reads them earlier.
+#define MA_P8(x, i) "+r"(x[i]), "+r"(x[i + 1]), "+r"(x[i + 2]), "+r"(x[i + 3]), "+r"(x[i + 4]), "+r"(x[i + 5]), "+r"(x[i + 6]), "+r"(x[i + 7])
+__device__ __forceinline__ void tmem_loaded32(uint32_t *x)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : MA_P8(x, 0), MA_P8(x, 8), MA_P8(x, 16), MA_P8(x, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_loaded8(uint32_t *x) { asm volatile("tcgen05.wait::ld.sync.aligned;" : MA_P8(x, 0)::"memory"); }
+__device__ __forceinline__ void tmem_loaded1(uint32_t &x) { asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x)::"memory"); }
+#undef MA_P8
+
+// ---- arithmetic ---------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// tanh from one exponential, 1 - 2 / (e^2y + 1), given 2 y log2(e): off by a few 2^-24, absolutely
+__device__ __forceinline__ float tanh_of(float two_y_log2e) { return 1.0f - __fdividef(2.0f, exp2_fast(two_y_log2e) + 1.0f); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_two(float low, float high)
+{
+    const float x[2] = {low, high};
+    return DT<T>::pack(x);
+}
+
+// zero times every element of a word, added to acc: NaN as soon as one is infinite or NaN
+template <typename T>
+__device__ __forceinline__ uint32_t taint(uint32_t w, uint32_t acc)
+{
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&w), __float2half2_rn(0.0f), *reinterpret_cast<const __half2 *>(&acc));
+        return *reinterpret_cast<const uint32_t *>(&r);
+    } else {
+        const __nv_bfloat162 r =
+            __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&w), __float2bfloat162_rn(0.0f), *reinterpret_cast<const __nv_bfloat162 *>(&acc));
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ bool tainted(uint32_t acc)
+{
+    const float a = DT<T>::unpack(acc, 0), b = DT<T>::unpack(acc, 1);
+    return a != a || b != b;
+}
+
+// Whether row `row` of a tile holds an infinite or NaN value.
+template <typename T, int DP>
+__device__ __forceinline__ bool row_tainted(const uint8_t *tile, int row)
+{
+    uint32_t acc = 0;
+#pragma unroll
+    for (int half = 0; half < DP / 64; ++half)
+#pragma unroll
+        for (int piece = 0; piece < 8; ++piece) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(tile + half * kHalfBytes + row * 128 + ((piece ^ (row & 7)) << 4));
+            acc = taint<T>(x.x, taint<T>(x.y, taint<T>(x.z, taint<T>(x.w, acc))));
+        }
+    return tainted<T>(acc);
+}
+
+// The product of the weights in tensor memory (128 x 16 bits per row at `weights`) and a tile's rows, added to the thread's row
+// of sums at `sums` term by term, leaving out the terms of weight zero: in place of the matrix instruction where the tile holds
+// infinite or NaN values that some rows do not see.  A warp's 32 rows; rare, and slow.
+template <typename T, int DP>
+static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, const uint8_t *tile, bool add)
+{
+    for (int c = 0; c < DP; c += 8) {
+        uint32_t raw[8] = {};
+        if (add) {
+            tmem_load8(sums + c, raw);
+            tmem_loaded8(raw);
+        }
+        float acc[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = __uint_as_float(raw[i]);
+        for (int j = 0; j < kTile; j += 2) {
+            uint32_t w = tmem_load1(weights + j / 2);
+            tmem_loaded1(w);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float x = DT<T>::unpack(w, e);
+                const int row = j + e;
+                const uint4 y = *reinterpret_cast<const uint4 *>(tile + c / 64 * kHalfBytes + row * 128 + ((c % 64 / 8 ^ (row & 7)) << 4));
+                const uint32_t words[4] = {y.x, y.y, y.z, y.w};
+                if (x != 0.0f) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[i] = fmaf(x, DT<T>::unpack(words[i / 2], i % 2), acc[i]);
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = __float_as_uint(acc[i]);
+        tmem_store8(sums + c, raw);
+    }
+    tmem_stored();
+}
+
+// ---- masks by tiles ------------------------------------------------------------------------------------
+
+// Keys that query n sees are those below this (and, with documents, of its id).
+__device__ __forceinline__ int key_limit(const GlobalMask &m, int n)
+{
+    return m.causal ? min(m.len, max(max(n + m.shift + 1, m.prefix), 0)) : m.len;
+}
+
+enum TileState { kHidden, kPartial, kWhole };
+
+// What the queries [n0, n0 + 128) see of the keys [j0, j0 + 128).
+__device__ __forceinline__ int tile_state(const GlobalMask &m, int N, int n0, int j0, const DocRange *qr, const DocRange *kr)
+{
+    if (n0 >= N || j0 >= key_limit(m, min(n0 + kTile, N) - 1)) return kHidden;
+    const bool whole = j0 + kTile <= key_limit(m, n0);
+    if (kr == nullptr) return whole ? kWhole : kPartial;
+    const DocRange q = *qr, k = *kr;
+    if (k.high < q.low || k.low > q.high || q.high < 0 || k.high < 0) return kHidden;
+    return whole && q.pure && k.pure && q.low == q.high && k.low == k.high ? kWhole : kPartial;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------
+
+// Whether the matrix kernels take a tensor: 16-byte aligned rows, no dimension repeated by a stride of zero.
+inline bool rows_fit(const void *base, const long long (&stride)[3], int B, int rows, int heads)
+{
+    const int sizes[3] = {B, rows, heads};
+    if (reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
+    for (int i = 0; i < 3; ++i)
+        if (sizes[i] > 1 && (stride[i] <= 0 || stride[i] % 8 != 0 || stride[i] >= (1LL << 38))) return false;
+    return true;
+}
+cudaError_t tile_map(CUtensorMap *map, const void *base, const long long (&stride)[3], int B, int rows, int heads, int d, int dtype);
+
+cudaError_t run_global_forward(const GlobalParams &p, const GlobalMaps &maps, int dtype, cudaStream_t stream);
+
+
+}  // namespace matchattn
