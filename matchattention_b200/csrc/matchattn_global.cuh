@@ -36,6 +36,7 @@ struct GlobalParams {
     const void *d_out;                  // [B, N, h, d]
     void *d_q, *d_k, *d_v;              // [B, N, h, d], [B, M, hk, d]
     float *delta;                       // [B, h, N] sum of d_out * out of a row
+    float *norms;                       // float16: the largest row norms of d_out and of v (rows with infinite or NaN values left out)
 };
 
 // What an item's masks say.

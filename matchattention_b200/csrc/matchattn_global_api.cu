@@ -40,22 +40,46 @@ __global__ void __launch_bounds__(256) global_join_kernel(const GlobalParams p)
         if (lane + 32 * i < p.d) store_one<T>(out + lane + 32 * i, empty ? 0.0f : acc[i] / sum);
 }
 
-// delta = sum over the channels of d_out * out: a warp per row.  Bound by memory.
+// delta = sum over the channels of d_out * out: a warp per row.  With `norms` also the largest norm of a row of d_out, and, by the
+// rows after those, of v (maxima do not depend on their order).  Bound by memory.
 template <typename T>
 __global__ void __launch_bounds__(256) global_delta_kernel(const GlobalParams p)
 {
     chain_begin();
-    const long long rows = static_cast<long long>(p.B) * p.N * p.h;
+    const long long rows = static_cast<long long>(p.B) * p.N * p.h, more = p.norms ? static_cast<long long>(p.B) * p.M * p.hk : 0;
     const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
-    if (row >= rows) return;
     const int lane = threadIdx.x & 31;
-    const T *o = static_cast<const T *>(p.out) + row * p.d, *g = static_cast<const T *>(p.d_out) + row * p.d;
-    float sum = 0.0f;
-    for (int c = lane; c < p.d; c += 32) sum = fmaf(load_one<T>(o + c), load_one<T>(g + c), sum);
+    __shared__ int largest[2];
+    if (threadIdx.x < 2) largest[threadIdx.x] = 0;
+    __syncthreads();
+    float square = 0.0f;
+    const bool of_v = row >= rows;
+    if (row < rows) {
+        const T *o = static_cast<const T *>(p.out) + row * p.d, *g = static_cast<const T *>(p.d_out) + row * p.d;
+        float sum = 0.0f;
+        for (int c = lane; c < p.d; c += 32) {
+            const float y = load_one<T>(g + c);
+            sum = fmaf(load_one<T>(o + c), y, sum);
+            square = fmaf(y, y, square);
+        }
 #pragma unroll
-    for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-    const long long bn = row / p.h, head = row - bn * p.h, b = bn / p.N, n = bn - b * p.N;
-    if (lane == 0) p.delta[(b * p.h + head) * p.N + n] = sum;
+        for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+        const long long bn = row / p.h, head = row - bn * p.h, b = bn / p.N, n = bn - b * p.N;
+        if (lane == 0) p.delta[(b * p.h + head) * p.N + n] = sum;
+    } else if (row < rows + more) {
+        const long long bj = (row - rows) / p.hk, head = row - rows - bj * p.hk, b = bj / p.M, j = bj - b * p.M;
+        const T *v = static_cast<const T *>(p.v) + b * p.vs[0] + j * p.vs[1] + head * p.vs[2];
+        for (int c = lane; c < p.d; c += 32) square = fmaf(load_one<T>(v + c), load_one<T>(v + c), square);
+    }
+    if (p.norms) {
+#pragma unroll
+        for (int i = 16; i > 0; i >>= 1) square += __shfl_xor_sync(0xffffffffu, square, i);
+        const float norm = sqrtf(square);
+        // floats that are not negative are ordered as their bits
+        if (lane == 0 && norm <= 3.402823466e38f) atomicMax(largest + of_v, __float_as_int(norm));
+        __syncthreads();
+        if (threadIdx.x < 2 && largest[threadIdx.x] > 0) atomicMax(reinterpret_cast<int *>(p.norms) + threadIdx.x, largest[threadIdx.x]);
+    }
 }
 
 // What the ids of a block of 128 tokens span: blocks of queries of all items, then blocks of keys.
@@ -108,7 +132,8 @@ int check_global(const matchattn_global_args *a)
         !aligned(a->slopes, 4) || !aligned(a->prefix, 4) || !aligned(a->lengths, 4) || !aligned(a->q_docs, 4) || !aligned(a->k_docs, 4))
         return MATCHATTN_ERR_ALIGN;
     // positions are exact in float32; rows of a key head and grid dimensions are 32- and 16-bit
-    if (a->N > (1 << 24) || a->M > (1 << 24) || a->h > 65535 || a->B > 65535 || 1LL * a->N * (a->h / a->hk) > (1LL << 30))
+    if (a->N > (1 << 24) || a->M > (1 << 24) || a->h > 65535 || a->B > 65535 || 1LL * a->N * (a->h / a->hk) > (1LL << 30) ||
+        1LL * a->B * a->h * (a->N / kTile + 1) > (1LL << 26) || 1LL * a->B * a->hk * (a->M / kTile + 1) > (1LL << 26))
         return MATCHATTN_ERR_TOO_LARGE;
     return MATCHATTN_OK;
 }
@@ -242,7 +267,9 @@ GlobalParams params_of(const matchattn_global_args *a)
     return p;
 }
 
+// Scratch of the backward call: two norms, the documents of the tiles, delta.
 size_t backward_floats(const matchattn_global_args *a) { return static_cast<size_t>(a->B) * a->h * a->N; }
+size_t backward_bytes(const matchattn_global_args *a) { return 16 + range_count(a) * sizeof(DocRange) + sizeof(float) * backward_floats(a); }
 
 }  // namespace
 }  // namespace matchattn
@@ -252,7 +279,7 @@ using namespace matchattn;
 extern "C" size_t matchattn_global_scratch_bytes(const matchattn_global_args *a, int backward)
 {
     if (check_global(a) != MATCHATTN_OK || a->M == 0) return 0;
-    if (backward) return sizeof(float) * backward_floats(a);
+    if (backward) return backward_bytes(a);
     const Plan plan = plan_forward(a);
     return plan.bytes();
 }
@@ -302,14 +329,34 @@ extern "C" int matchattn_global_backward(const matchattn_global_args *a, const v
     const size_t size = a->dtype == MATCHATTN_F32 ? 4 : 2;
     if (!aligned(d_out, size) || !aligned(d_q, size) || !aligned(d_k, size) || !aligned(d_v, size)) return MATCHATTN_ERR_ALIGN;
     if (a->M == 0) return status_of(cudaMemsetAsync(d_q, 0, static_cast<size_t>(a->B) * a->N * a->h * a->d * size, stream));
-    if (scratch_bytes < sizeof(float) * backward_floats(a)) return MATCHATTN_ERR_SCRATCH_LIMIT;
+    if (scratch_bytes < backward_bytes(a)) return MATCHATTN_ERR_SCRATCH_LIMIT;
     if (!aligned(scratch, 16)) return MATCHATTN_ERR_ALIGN;
     GlobalParams p = params_of(a);
     p.vec = p.vec && aligned(d_out, 4 * size);
     p.d_out = d_out, p.d_q = d_q, p.d_k = d_k, p.d_v = d_v;
-    p.delta = static_cast<float *>(scratch);
-    const unsigned blocks = static_cast<unsigned>((backward_floats(a) + 7) / 8);
-    cudaError_t err = by_type(a->dtype, [&](auto t) { return launch_chained(global_delta_kernel<decltype(t)>, dim3(blocks), 256, 0, stream, p); });
-    if (err == cudaSuccess) err = run_global_any_backward(p, a->dtype, stream);
+    DocRange *ranges = reinterpret_cast<DocRange *>(static_cast<char *>(scratch) + 16);
+    p.delta = reinterpret_cast<float *>(ranges + range_count(a));
+    const bool matrix = matrix_call(a) && aligned(d_out, 16) && aligned(d_q, 16) && aligned(d_k, 16) && aligned(d_v, 16);
+    cudaError_t err = cudaSuccess;
+    long long rows = static_cast<long long>(backward_floats(a));
+    if (matrix && a->dtype == MATCHATTN_F16) {
+        p.norms = static_cast<float *>(scratch);
+        rows += 1LL * a->B * a->M * a->hk;
+        err = cudaMemsetAsync(scratch, 0, 16, stream);
+    }
+    if (err == cudaSuccess)
+        err = by_type(a->dtype, [&](auto t) {
+            return launch_chained(global_delta_kernel<decltype(t)>, dim3(static_cast<unsigned>((rows + 7) / 8)), 256, 0, stream, p);
+        });
+    if (err == cudaSuccess && matrix) {
+        GlobalMaps maps{};
+        const long long stride[3] = {1LL * a->N * a->h * a->d, 1LL * a->h * a->d, a->d};
+        err = operand_maps(maps, a);
+        if (err == cudaSuccess) err = tile_map(&maps.o, d_out, stride, a->B, a->N, a->h, a->d, a->dtype);
+        if (err == cudaSuccess) err = find_ranges(p, ranges, stream);
+        if (err == cudaSuccess) err = run_global_backward(p, maps, a->dtype, stream);
+    } else if (err == cudaSuccess) {
+        err = run_global_any_backward(p, a->dtype, stream);
+    }
     return status_of(err);
 }

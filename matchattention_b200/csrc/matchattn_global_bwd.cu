@@ -1,0 +1,391 @@
+// Dense attention, backward, 16-bit types of up to 128 channels, on the matrix units.
+//
+//   P = 2^(x - lse),  dP = dO V^T,  dS = P (1 - tanh^2) (dP - delta),  delta = rowsum(dO O)
+//   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K
+//
+// Two passes of one kernel, each recomputing S and P: for keys (a block owns 128 keys of a key head, walks the queries of all
+// heads that share it, and keeps dK and dV in tensor memory) and for queries (128 queries, walks the keys, keeps dQ).  That is seven
+// products where one pass with dQ added up in global memory has five, but the sums have one order and no atomics.
+//
+// A block has a fixed pair of tiles (keys: K, V; queries: Q, dO) and a moving pair (Q, dO; K, V).  The scores and dP of
+// fixed by moving rows come to tensor memory; a thread holds a fixed row and half of the 128 moving ones (warps 0-3 and 4-7), and puts P
+// over S and dS over dP, rounded to the type, as first operands of the products that add up the moving rows.  Order of the
+// matrix unit: dV(i-1), S(i), dK(i-1), dP(i): while threads take exponentials of tile i it forms dK(i-1) and dP(i), while
+// they form dS(i) it forms dV(i) and S(i+1).
+//
+// float16 has few exponents: P is held times 2^12 (P of a row of 10^5 tokens is not subnormal), dS times the power of two that
+// brings the largest value that row norms of dO and V allow, |dS| <= 2 |dO| |V|, to between 2^14 and 2^15; both leave the sums exactly.
+//
+// As in the forward pass, tiles that are partly hidden are looked through for infinite and NaN values, and added term by term
+// where they have some.
+#include "matchattn_global_mma.cuh"
+
+namespace matchattn {
+namespace {
+
+constexpr int kBackThreads = 320;
+
+template <int DP>
+struct BackShared {
+    static constexpr int kStages = DP == 128 ? 2 : 3;
+    uint8_t fixed[2][kTileBytes<DP>];
+    uint8_t moving[kStages][2][kTileBytes<DP>];
+    float2 row[8][64], place[8][64];       // per warp, for its 64 moving rows: lse and delta; column and row on the map
+    int docs[8][64];
+    uint64_t fixed_full, full[kStages], empty[kStages], s_full, p_full, dp_full, ds_full, done, looked, stored;
+    uint32_t tmem;
+    int broken, by_hand[2], odd[2][3];
+};
+
+// KEYS: the pass for dK and dV.  GENERAL: scores capped or with a bias
+template <typename T, int DP, bool GENERAL, bool KEYS>
+__global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const GlobalParams p, const __grid_constant__ GlobalMaps maps)
+{
+    chain_begin();
+    constexpr int STAGES = BackShared<DP>::kStages;
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    constexpr float kLift = HALF ? 12.0f : 0.0f;           // log2 of the factor that P is held by
+    extern __shared__ uint8_t raw_shared[];
+    BackShared<DP> &sh = *reinterpret_cast<BackShared<DP> *>(raw_shared + (1024 - (shared_address(raw_shared) & 1023)) % 1024);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int heads = KEYS ? p.hk : p.h;
+    const int lot = p.B * heads, turn = blockIdx.x / lot, b = blockIdx.x % lot / heads, own = blockIdx.x % lot % heads, kh = KEYS ? own : own / p.g;
+    // causal: the first keys are seen by most queries, the last queries see most keys: their blocks begin first
+    const int f0 = (KEYS ? turn : gridDim.x / lot - 1 - turn) * kTile;
+    const GlobalMask mask = global_mask(p, b);
+    const int key_tiles = (p.M + kTile - 1) / kTile, query_tiles = (p.N + kTile - 1) / kTile;
+    const DocRange *kr = p.q_docs ? p.ranges + p.B * query_tiles + b * key_tiles : nullptr;
+    const DocRange *qr = p.q_docs ? p.ranges + b * query_tiles : nullptr;
+    const auto state = [&](int t) {
+        const int n0 = KEYS ? t * kTile : f0, j0 = KEYS ? f0 : t * kTile;
+        return tile_state(mask, p.N, n0, j0, qr ? qr + n0 / kTile : nullptr, kr ? kr + j0 / kTile : nullptr);
+    };
+    const int rounds = KEYS ? p.g : 1;                     // heads that are walked
+    const int t_begin = KEYS ? min(query_begin(mask, f0), p.N) / kTile : 0;
+    const int t_end = KEYS ? query_tiles : (key_limit(mask, min(f0 + kTile, p.N) - 1) + kTile - 1) / kTile;
+
+    if (tid == 0) {
+        barrier_init(&sh.fixed_full, 1);
+        for (int i = 0; i < STAGES; ++i) {
+            barrier_init(&sh.full[i], 1);
+            barrier_init(&sh.empty[i], 1);
+        }
+        barrier_init(&sh.s_full, 1);
+        barrier_init(&sh.dp_full, 1);
+        barrier_init(&sh.done, 1);
+        barrier_init(&sh.p_full, 256);
+        barrier_init(&sh.ds_full, 256);
+        barrier_init(&sh.looked, 256);
+        barrier_init(&sh.stored, 256);
+        sh.broken = 0;
+        for (int i = 0; i < 3; ++i) sh.odd[0][i] = sh.odd[1][i] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) tmem_take(&sh.tmem);
+    tmem_before();
+    __syncthreads();
+    tmem_after();
+    const uint32_t tmem = sh.tmem;
+    const uint32_t scores = tmem, slopes = tmem + 128, sum_v = tmem + 256, sum_k = tmem + 384;       // sum_k: dK or dQ
+
+    if (warp == 8) {
+        // ---- copies
+        if (elected()) {
+            barrier_expect(&sh.fixed_full, 2 * kTileBytes<DP>);
+            load_tile<DP>(sh.fixed[0], KEYS ? &maps.k : &maps.q, own, f0, b, &sh.fixed_full);
+            load_tile<DP>(sh.fixed[1], KEYS ? &maps.v : &maps.o, own, f0, b, &sh.fixed_full);
+            int i = 0;
+            bool good = true;
+            for (int r = 0; r < rounds && good; ++r)
+                for (int t = t_begin; t < t_end; ++t) {
+                    if (state(t) == kHidden) continue;
+                    const int s = i % STAGES, head = KEYS ? kh * p.g + r : kh;
+                    if (i >= STAGES) good = barrier_wait(&sh.empty[s], (i / STAGES - 1) & 1, &sh.broken);
+                    if (!good) break;
+                    barrier_expect(&sh.full[s], 2 * kTileBytes<DP>);
+                    load_tile<DP>(sh.moving[s][0], KEYS ? &maps.q : &maps.k, head, t * kTile, b, &sh.full[s]);
+                    load_tile<DP>(sh.moving[s][1], KEYS ? &maps.o : &maps.v, head, t * kTile, b, &sh.full[s]);
+                    ++i;
+                }
+            if (!good) {
+                // copies under way write to this block's memory: it stays until they are done
+                barrier_drain(&sh.fixed_full, 0);
+                for (int n = i > STAGES ? i - STAGES : 0; n < i; ++n) barrier_drain(&sh.full[n % STAGES], (n / STAGES) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // ---- products
+        if (elected()) {
+            const int steps = (p.d + 15) / 16;
+            const uint32_t score_kind = product_kind<T>(kTile, false), sum_kind = product_kind<T>(steps * 16, true);
+            const uint32_t fixed[2] = {shared_address(sh.fixed[0]), shared_address(sh.fixed[1])};
+            bool good = barrier_wait(&sh.fixed_full, 0, &sh.broken);
+            int i = 0;
+            const auto moving = [&](int n, int which) { return shared_address(sh.moving[n % STAGES][which]); };
+            // columns of a first operand: 64 moving rows in 32 words, the other 64 behind the first half's place of scores
+            const auto add_up = [&](uint32_t sums, uint32_t weights, uint32_t tile, bool add) {
+#pragma unroll
+                for (int s = 0; s < kTile / 16; ++s) product_ts(sums, weights + 8 * s + (s >= 4 ? 32 : 0), by_rows(tile, s), sum_kind, add || s > 0);
+            };
+            const auto after_scores = [&](int n) {         // dV of tile n, when its P is there
+                good = good && barrier_wait(&sh.p_full, n & 1, &sh.broken);
+                if (!good) return;
+                tmem_after();
+                if (KEYS && !*static_cast<volatile int *>(&sh.by_hand[0])) add_up(sum_v, scores, moving(n, 1), n > 0);
+            };
+            const auto after_slopes = [&](int n) {         // dK or dQ of tile n, when its dS is there
+                good = good && barrier_wait(&sh.ds_full, n & 1, &sh.broken);
+                if (!good) return;
+                tmem_after();
+                if (!*static_cast<volatile int *>(&sh.by_hand[1])) add_up(sum_k, slopes, moving(n, 0), n > 0);
+                products_done(&sh.empty[n % STAGES]);
+            };
+            for (int r = 0; r < rounds && good; ++r)
+                for (int t = t_begin; t < t_end && good; ++t) {
+                    if (state(t) == kHidden) continue;
+                    good = barrier_wait(&sh.full[i % STAGES], (i / STAGES) & 1, &sh.broken);
+                    if (i > 0) after_scores(i - 1);
+                    if (!good) break;
+                    for (int s = 0; s < steps; ++s) product_ss(scores, by_channels(fixed[0], s), by_channels(moving(i, 0), s), score_kind, s > 0);
+                    products_done(&sh.s_full);
+                    if (i > 0) after_slopes(i - 1);
+                    if (!good) break;
+                    for (int s = 0; s < steps; ++s) product_ss(slopes, by_channels(fixed[1], s), by_channels(moving(i, 1), s), score_kind, s > 0);
+                    products_done(&sh.dp_full);
+                    ++i;
+                }
+            if (good && i > 0) {
+                after_scores(i - 1);
+                after_slopes(i - 1);
+            }
+            products_done(&sh.done);
+            if (!good) barrier_drain(&sh.done, 0);
+        }
+        __syncwarp();
+    } else {
+        // ---- probabilities and slopes
+        const int w = warp >> 2, f = f0 + (tid & 127);                          // half of the moving rows; the fixed row
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+        const uint32_t my_scores = scores + lanes + w * 64, my_slopes = slopes + lanes + w * 64;
+        const float factor = p.scale * kLog2e, inner = p.cap != 0.0f ? 2.0f * factor / p.cap : 0.0f, outer = p.cap * kLog2e;
+        // dS is held times 2^(lift - kLift), the sums of dS times 2^-lift
+        int lift = 0;
+        if (HALF) {
+            const float bound = 2.0f * p.norms[0] * p.norms[1];
+            if (bound > 0.0f && bound <= 3.402823466e38f) lift = min(max(14 - ilogbf(bound), -60), 60);
+        }
+        const float hold = ldexpf(1.0f, lift) * (HALF ? 1.0f / 4096.0f : 1.0f);
+        const int limit = KEYS ? 0 : key_limit(mask, f);                        // queries: keys below it are seen
+        const int first = KEYS ? query_begin(mask, f) : 0;                      // keys: queries from it on see it
+        int doc = -1;
+        if (p.q_docs) {
+            if (KEYS) doc = f < p.M ? p.k_docs[static_cast<long long>(b) * p.M + f] : -1;
+            else doc = f < p.N ? p.q_docs[static_cast<long long>(b) * p.N + f] : -1;
+        }
+        const float2 here = GENERAL ? map_place(KEYS ? f : f + mask.shift, p.width) : make_float2(0.0f, 0.0f);
+        float lse = INFINITY, delta = 0.0f;
+        if (!KEYS && f < p.N) {
+            const long long line = (static_cast<long long>(b) * p.h + own) * p.N + f;
+            lse = p.lse[line] - kLift;
+            delta = p.delta[line];
+        }
+        int i = 0, looks = 0, stores = 0;
+        bool good = true;
+        for (int r = 0; r < rounds && good; ++r) {
+            const int head = KEYS ? kh * p.g + r : own;
+            const float slope = GENERAL && p.slopes ? p.slopes[head] * kLog2e : 0.0f;
+            for (int t = t_begin; t < t_end; ++t) {
+                const int now = state(t);
+                if (now == kHidden) continue;
+                const int m0 = t * kTile + w * 64;                              // first of the warp's moving rows
+#pragma unroll
+                for (int e = lane; e < 64; e += 32) {
+                    const int m = m0 + e;
+                    if (KEYS) {
+                        const long long line = (static_cast<long long>(b) * p.h + head) * p.N + m;
+                        sh.row[warp][e] = m < p.N ? make_float2(p.lse[line] - kLift, p.delta[line]) : make_float2(INFINITY, 0.0f);
+                    }
+                    if (p.q_docs && now == kPartial) {
+                        const int rows = KEYS ? p.N : p.M;
+                        sh.docs[warp][e] = m < rows ? (KEYS ? p.q_docs : p.k_docs)[static_cast<long long>(b) * rows + m] : -1;
+                    }
+                    if (GENERAL && p.slopes && p.width > 1) sh.place[warp][e] = map_place(KEYS ? m + mask.shift : m, p.width);
+                }
+                __syncwarp();
+                good = good && barrier_wait(&sh.s_full, i & 1, &sh.broken);
+                if (!good) break;
+                tmem_after();
+                float prob[64];                                                 // P, then P (1 - tanh^2)
+                uint32_t *raw = reinterpret_cast<uint32_t *>(prob);
+                tmem_load32(my_scores, raw);
+                tmem_load32(my_scores + 32, raw + 32);
+                tmem_loaded32(raw);
+                tmem_loaded32(raw + 32);
+#pragma unroll
+                for (int c = 0; c < 64; c += 32) {
+                    uint32_t packed[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float pair[2], slant[2] = {1.0f, 1.0f};
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int at = c + e + u;
+                            const float level = KEYS ? sh.row[warp][at].x : lse;
+                            float x;
+                            if constexpr (GENERAL) {
+                                if (p.cap != 0.0f) {
+                                    const float tanh_x = tanh_of(prob[at] * inner);
+                                    slant[u] = fmaf(-tanh_x, tanh_x, 1.0f);
+                                    x = outer * tanh_x;
+                                } else {
+                                    x = prob[at] * factor;
+                                }
+                                if (p.slopes) {
+                                    float far;
+                                    if (p.width > 1) far = map_distance(here, sh.place[warp][at]);
+                                    else far = fabsf(here.y - static_cast<float>((KEYS ? m0 + mask.shift : m0) + at));
+                                    x = fmaf(-slope, far, x);
+                                }
+                                x -= level;
+                            } else {
+                                x = fmaf(prob[at], factor, -level);
+                            }
+                            if (now == kPartial) {
+                                bool seen = KEYS ? m0 + at >= first : m0 + at < limit;
+                                if (p.q_docs) seen = seen && doc >= 0 && sh.docs[warp][at] == doc;
+                                x = seen ? x : -INFINITY;
+                            }
+                            pair[u] = exp2_fast(x);
+                            prob[at] = GENERAL ? pair[u] * slant[u] : pair[u];
+                        }
+                        packed[e / 2] = pack_two<T>(pair[0], pair[1]);
+                    }
+                    if (KEYS) tmem_store16(my_scores + c / 2, packed);
+                }
+                if (KEYS) tmem_stored();
+                // a partly hidden tile's moving rows are looked through: warps 0-3 the first tile, 4-7 the second
+                bool hand_v = false, hand_k = false;
+                if (now == kPartial) {
+                    const int s = i % STAGES;
+                    good = barrier_wait(&sh.full[s], (i / STAGES) & 1, &sh.broken);
+                    if (good && (KEYS || w == 0) && row_tainted<T, DP>(sh.moving[s][w], tid & 127)) *static_cast<volatile int *>(&sh.odd[w][looks % 3]) = 1;
+                    // (the slot after this one was last read two looks ago)
+                    if ((tid & 127) == 0) *static_cast<volatile int *>(&sh.odd[w][(looks + 1) % 3]) = 0;
+                    tmem_before();
+                    barrier_arrive(&sh.looked);
+                    good = good && barrier_wait(&sh.looked, looks & 1, &sh.broken);
+                    tmem_after();
+                    hand_k = __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[0][looks % 3]) != 0);
+                    hand_v = KEYS && __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[1][looks % 3]) != 0);
+                    ++looks;
+                    if (hand_v && w == 0) add_rows<T, DP>(sum_v + lanes, scores + lanes, 32, sh.moving[s][1], i > 0);
+                }
+                if (tid == 0) sh.by_hand[0] = hand_v;
+                tmem_before();
+                barrier_arrive(&sh.p_full);
+                good = good && barrier_wait(&sh.dp_full, i & 1, &sh.broken);
+                if (!good) break;
+                tmem_after();
+#pragma unroll
+                for (int c = 0; c < 64; c += 32) {
+                    uint32_t dp[32], packed[16];
+                    tmem_load32(my_slopes + c, dp);
+                    tmem_loaded32(dp);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float pair[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int at = c + e + u;
+                            const float off = __uint_as_float(dp[e + u]) - (KEYS ? sh.row[warp][at].y : delta);
+                            pair[u] = prob[at] * (HALF ? off * hold : off);
+                            if (now == kPartial && prob[at] == 0.0f) pair[u] = 0.0f;
+                        }
+                        packed[e / 2] = pack_two<T>(pair[0], pair[1]);
+                    }
+                    tmem_store16(my_slopes + c / 2, packed);
+                }
+                tmem_stored();
+                if (hand_k) {
+                    tmem_before();
+                    barrier_arrive(&sh.stored);
+                    good = barrier_wait(&sh.stored, stores & 1, &sh.broken);
+                    tmem_after();
+                    ++stores;
+                    if (w == 1) add_rows<T, DP>(sum_k + lanes, slopes + lanes, 32, sh.moving[i % STAGES][0], i > 0);
+                }
+                if (tid == 0) sh.by_hand[1] = hand_k;
+                tmem_before();
+                barrier_arrive(&sh.ds_full);
+                ++i;
+            }
+        }
+        if (good) good = barrier_wait(&sh.done, 0, &sh.broken);
+        tmem_after();
+        // ---- results: dV by warps 0-3 and dK by 4-7, or dQ's channels in turn
+        const int rows = KEYS ? p.M : p.N;
+        const float times = KEYS && w == 0 ? (HALF ? 1.0f / 4096.0f : 1.0f) : p.scale * ldexpf(1.0f, -lift);
+        T *to = static_cast<T *>(KEYS ? (w == 0 ? p.d_v : p.d_k) : p.d_q) + ((static_cast<long long>(b) * rows + f) * heads + own) * p.d;
+        const uint32_t from = (KEYS && w == 0 ? sum_v : sum_k) + lanes;
+#pragma unroll 1
+        for (int c = KEYS ? 0 : w * 32; c < DP && c < p.d; c += KEYS ? 32 : 64) {
+            uint32_t raw[32] = {};
+            if (i > 0) {
+                tmem_load32(from + c, raw);
+                tmem_loaded32(raw);
+            }
+            if (f < rows) {
+                float y[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) y[e] = good ? __uint_as_float(raw[e]) * times : NAN;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+                    if (c + e < p.d)
+                        *reinterpret_cast<uint4 *>(to + c + e) = make_uint4(pack_two<T>(y[e], y[e + 1]), pack_two<T>(y[e + 2], y[e + 3]),
+                                                                            pack_two<T>(y[e + 4], y[e + 5]), pack_two<T>(y[e + 6], y[e + 7]));
+            }
+            __syncwarp();
+        }
+    }
+    tmem_before();
+    __syncthreads();
+    if (warp == 9) tmem_give(tmem);
+}
+
+template <typename T, int DP, bool GENERAL, bool KEYS>
+cudaError_t backward_pass(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
+{
+    constexpr size_t smem = sizeof(BackShared<DP>) + 1024;
+    static_assert(smem <= 227 * 1024 && smem > 114 * 1024, "one block per SM: it takes all of the tensor memory");
+    const auto kernel = global_backward_kernel<T, DP, GENERAL, KEYS>;
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (err != cudaSuccess) return err;
+    const dim3 grid(static_cast<unsigned>(p.B) * (KEYS ? p.hk : p.h) * (((KEYS ? p.M : p.N) + kTile - 1) / kTile));
+    return launch_chained(kernel, grid, kBackThreads, smem, stream, p, maps);
+}
+
+template <typename T, int DP, bool GENERAL>
+cudaError_t backward_one(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
+{
+    const cudaError_t err = backward_pass<T, DP, GENERAL, true>(p, maps, stream);
+    return err != cudaSuccess ? err : backward_pass<T, DP, GENERAL, false>(p, maps, stream);
+}
+
+template <typename T>
+cudaError_t backward_type(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
+{
+    const bool general = p.cap != 0.0f || p.slopes != nullptr;
+    if (p.d <= 64) return general ? backward_one<T, 64, true>(p, maps, stream) : backward_one<T, 64, false>(p, maps, stream);
+    return general ? backward_one<T, 128, true>(p, maps, stream) : backward_one<T, 128, false>(p, maps, stream);
+}
+
+}  // namespace
+
+cudaError_t run_global_backward(const GlobalParams &p, const GlobalMaps &maps, int dtype, cudaStream_t stream)
+{
+    return dtype == MATCHATTN_F16 ? backward_type<__half>(p, maps, stream) : backward_type<__nv_bfloat16>(p, maps, stream);
+}
+
+}  // namespace matchattn

@@ -41,10 +41,10 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
     extern __shared__ uint8_t raw_shared[];
     ForwardShared<DP> &sh = *reinterpret_cast<ForwardShared<DP> *>(raw_shared + (1024 - (shared_address(raw_shared) & 1023)) % 1024);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int bh = blockIdx.x % (p.B * p.h), split = blockIdx.x / (p.B * p.h);
+    const int lot = p.B * p.h * p.splits, turn = blockIdx.x / lot, bh = blockIdx.x % lot % (p.B * p.h), split = blockIdx.x % lot / (p.B * p.h);
     const int b = bh / p.h, head = bh - b * p.h, kh = head / p.g;
     // the last queries of a causal call see most: their blocks begin first
-    const int n0 = (gridDim.y - 1 - blockIdx.y) * p.block_rows;
+    const int n0 = (gridDim.x / lot - 1 - turn) * p.block_rows;
     const GlobalMask mask = global_mask(p, b);
     const int key_tiles = (p.M + kTile - 1) / kTile, query_tiles = (p.N + kTile - 1) / kTile;
     const DocRange *kr = p.q_docs ? p.ranges + p.B * query_tiles + b * key_tiles : nullptr;
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                 good = good && barrier_wait(&sh.looked[w], looks & 1, &sh.broken);
                 hand = __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[w][looks % 3]) != 0);
                 ++looks;
-                if (hand) add_rows<T, DP>(out, scores, sh.kv[s], used > 0);
+                if (hand) add_rows<T, DP>(out, scores, 0, sh.kv[s], used > 0);
             }
             if (row == 0) sh.by_hand[w] = hand;
             tmem_before();
@@ -369,7 +369,7 @@ cudaError_t forward_one(const GlobalParams &p, const GlobalMaps &maps, cudaStrea
     const auto kernel = global_forward_kernel<T, DP, GENERAL>;
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (err != cudaSuccess) return err;
-    const dim3 grid(p.B * p.h * p.splits, (p.N + p.block_rows - 1) / p.block_rows);
+    const dim3 grid(static_cast<unsigned>(p.B) * p.h * p.splits * ((p.N + p.block_rows - 1) / p.block_rows));
     return launch_chained(kernel, grid, kForwardThreads, smem, stream, p, maps);
 }
 

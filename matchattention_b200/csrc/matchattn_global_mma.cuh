@@ -284,11 +284,11 @@ __device__ __forceinline__ bool row_tainted(const uint8_t *tile, int row)
     return tainted<T>(acc);
 }
 
-// The product of the weights in tensor memory (128 x 16 bits per row at `weights`) and a tile's rows, added to the thread's row
+// The product of the weights in tensor memory (128 x 16 bits per row at `weights`, `gap` words between the halves) and a tile's rows, added to the thread's row
 // of sums at `sums` term by term, leaving out the terms of weight zero: in place of the matrix instruction where the tile holds
 // infinite or NaN values that some rows do not see.  A warp's 32 rows; rare, and slow.
 template <typename T, int DP>
-static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, const uint8_t *tile, bool add)
+static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, int gap, const uint8_t *tile, bool add)
 {
     for (int c = 0; c < DP; c += 8) {
         uint32_t raw[8] = {};
@@ -300,7 +300,7 @@ static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, co
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] = __uint_as_float(raw[i]);
         for (int j = 0; j < kTile; j += 2) {
-            uint32_t w = tmem_load1(weights + j / 2);
+            uint32_t w = tmem_load1(weights + j / 2 + (j >= kTile / 2 ? gap : 0));
             tmem_loaded1(w);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -354,9 +354,9 @@ inline bool rows_fit(const void *base, const long long (&stride)[3], int B, int 
         if (sizes[i] > 1 && (stride[i] <= 0 || stride[i] % 8 != 0 || stride[i] >= (1LL << 38))) return false;
     return true;
 }
-cudaError_t tile_map(CUtensorMap *map, const void *base, const long long (&stride)[3], int B, int rows, int heads, int d, int dtype);
 
 cudaError_t run_global_forward(const GlobalParams &p, const GlobalMaps &maps, int dtype, cudaStream_t stream);
+cudaError_t run_global_backward(const GlobalParams &p, const GlobalMaps &maps, int dtype, cudaStream_t stream);
 
 
 }  // namespace matchattn
