@@ -308,7 +308,7 @@ extern "C" int matchattn_global_forward(const matchattn_global_args *a, void *sc
         GlobalMaps maps{};
         err = operand_maps(maps, a);
         if (err == cudaSuccess) err = find_ranges(p, static_cast<DocRange *>(scratch), stream);
-        if (err == cudaSuccess) err = run_global_forward(p, maps, a->dtype, stream);
+        if (err == cudaSuccess) err = a->dtype == MATCHATTN_F16 ? run_global_forward<__half>(p, maps, stream) : run_global_forward<__nv_bfloat16>(p, maps, stream);
     } else {
         err = run_global_any_forward(p, a->dtype, stream);
     }
@@ -354,7 +354,7 @@ extern "C" int matchattn_global_backward(const matchattn_global_args *a, const v
         err = operand_maps(maps, a);
         if (err == cudaSuccess) err = tile_map(&maps.o, d_out, stride, a->B, a->N, a->h, a->d, a->dtype);
         if (err == cudaSuccess) err = find_ranges(p, ranges, stream);
-        if (err == cudaSuccess) err = run_global_backward(p, maps, a->dtype, stream);
+        if (err == cudaSuccess) err = a->dtype == MATCHATTN_F16 ? run_global_backward<__half>(p, maps, stream) : run_global_backward<__nv_bfloat16>(p, maps, stream);
     } else if (err == cudaSuccess) {
         err = run_global_any_backward(p, a->dtype, stream);
     }

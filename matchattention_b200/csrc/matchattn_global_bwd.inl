@@ -1,4 +1,5 @@
-// Dense attention, backward, 16-bit types of up to 128 channels, on the matrix units.
+// Dense attention, backward, 16-bit types of up to 128 channels, on the matrix units.  Included once per type with MATCHATTN_T
+// defined.
 //
 //   P = 2^(x - lse),  dP = dO V^T,  dS = P (1 - tanh^2) (dP - delta),  delta = rowsum(dO O)
 //   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K
@@ -30,15 +31,18 @@ struct BackShared {
     static constexpr int kStages = DP == 128 ? 2 : 3;
     uint8_t fixed[2][kTileBytes<DP>];
     uint8_t moving[kStages][2][kTileBytes<DP>];
-    float2 row[8][64], place[8][64];       // per warp, for its 64 moving rows: lse and delta; column and row on the map
-    int docs[8][64];
+    float4 lse[8][16], delta[8][16], across[8][16], down[8][16];      // per warp, for its 64 moving rows; column and row on the map
+    int4 docs[8][16];
     uint64_t fixed_full, full[kStages], empty[kStages], s_full, p_full, dp_full, ds_full, done, looked, stored;
     uint32_t tmem;
     int broken, by_hand[2], odd[2][3];
 };
 
-// KEYS: the pass for dK and dV.  GENERAL: scores capped or with a bias
-template <typename T, int DP, bool GENERAL, bool KEYS>
+__device__ __forceinline__ float element(const float4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+__device__ __forceinline__ int element(const int4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
+// KEYS: the pass for dK and dV
+template <typename T, int DP, bool CAP, GlobalBias BIAS, bool KEYS>
 __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const GlobalParams p, const __grid_constant__ GlobalMaps maps)
 {
     chain_begin();
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         const int w = warp >> 2, f = f0 + (tid & 127);                          // half of the moving rows; the fixed row
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
         const uint32_t my_scores = scores + lanes + w * 64, my_slopes = slopes + lanes + w * 64;
-        const float factor = p.scale * kLog2e, inner = p.cap != 0.0f ? 2.0f * factor / p.cap : 0.0f, outer = p.cap * kLog2e;
+        const float factor = p.scale * kLog2e, inner = CAP ? 2.0f * factor / p.cap : 0.0f, outer = p.cap * kLog2e;
         // dS is held times 2^(lift - kLift), the sums of dS times 2^-lift
         int lift = 0;
         if (HALF) {
@@ -177,14 +181,15 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
             if (bound > 0.0f && bound <= 3.402823466e38f) lift = min(max(14 - ilogbf(bound), -60), 60);
         }
         const float hold = ldexpf(1.0f, lift) * (HALF ? 1.0f / 4096.0f : 1.0f);
-        const int limit = KEYS ? 0 : key_limit(mask, f);                        // queries: keys below it are seen
-        const int first = KEYS ? query_begin(mask, f) : 0;                      // keys: queries from it on see it
         int doc = -1;
         if (p.q_docs) {
             if (KEYS) doc = f < p.M ? p.k_docs[static_cast<long long>(b) * p.M + f] : -1;
             else doc = f < p.N ? p.q_docs[static_cast<long long>(b) * p.N + f] : -1;
         }
-        const float2 here = GENERAL ? map_place(KEYS ? f : f + mask.shift, p.width) : make_float2(0.0f, 0.0f);
+        const bool apart = p.q_docs && doc < 0;                                 // of no document
+        const int limit = apart ? 0 : key_limit(mask, f);                       // queries: keys below it are seen
+        const int first = apart ? 1 << 30 : query_begin(mask, f);               // keys: queries from it on see it
+        const float2 here = BIAS != kNoBias ? map_place(KEYS ? f : f + mask.shift, p.width) : make_float2(0.0f, 0.0f);
         float lse = INFINITY, delta = 0.0f;
         if (!KEYS && f < p.N) {
             const long long line = (static_cast<long long>(b) * p.h + own) * p.N + f;
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         bool good = true;
         for (int r = 0; r < rounds && good; ++r) {
             const int head = KEYS ? kh * p.g + r : own;
-            const float slope = GENERAL && p.slopes ? p.slopes[head] * kLog2e : 0.0f;
+            const float slope = BIAS != kNoBias ? p.slopes[head] * kLog2e : 0.0f;
             for (int t = t_begin; t < t_end; ++t) {
                 const int now = state(t);
                 if (now == kHidden) continue;
@@ -205,13 +210,18 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     const int m = m0 + e;
                     if (KEYS) {
                         const long long line = (static_cast<long long>(b) * p.h + head) * p.N + m;
-                        sh.row[warp][e] = m < p.N ? make_float2(p.lse[line] - kLift, p.delta[line]) : make_float2(INFINITY, 0.0f);
+                        reinterpret_cast<float *>(sh.lse[warp])[e] = m < p.N ? p.lse[line] - kLift : INFINITY;
+                        reinterpret_cast<float *>(sh.delta[warp])[e] = m < p.N ? p.delta[line] : 0.0f;
                     }
                     if (p.q_docs && now == kPartial) {
                         const int rows = KEYS ? p.N : p.M;
-                        sh.docs[warp][e] = m < rows ? (KEYS ? p.q_docs : p.k_docs)[static_cast<long long>(b) * rows + m] : -1;
+                        reinterpret_cast<int *>(sh.docs[warp])[e] = m < rows ? (KEYS ? p.q_docs : p.k_docs)[static_cast<long long>(b) * rows + m] : -1;
                     }
-                    if (GENERAL && p.slopes && p.width > 1) sh.place[warp][e] = map_place(KEYS ? m + mask.shift : m, p.width);
+                    if (BIAS == kMapBias) {
+                        const float2 at = map_place(KEYS ? m + mask.shift : m, p.width);
+                        reinterpret_cast<float *>(sh.across[warp])[e] = at.x;
+                        reinterpret_cast<float *>(sh.down[warp])[e] = at.y;
+                    }
                 }
                 __syncwarp();
                 good = good && barrier_wait(&sh.s_full, i & 1, &sh.broken);
@@ -223,44 +233,44 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 tmem_load32(my_scores + 32, raw + 32);
                 tmem_loaded32(raw);
                 tmem_loaded32(raw + 32);
+                const float from = here.y - static_cast<float>(KEYS ? m0 + mask.shift : m0);
+                const int bar = (KEYS ? first : limit) - m0;                    // keys: the moving rows from it on are seen; queries: those below
 #pragma unroll
                 for (int c = 0; c < 64; c += 32) {
                     uint32_t packed[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float pair[2], slant[2] = {1.0f, 1.0f};
+                    for (int e = 0; e < 32; e += 4) {
+                        const int four = (c + e) / 4;
+                        float level[4], value[4];
+                        float4 row_lse, across, down;
+                        int4 docs;
+                        if (KEYS) row_lse = sh.lse[warp][four];
+                        if (BIAS == kMapBias) across = sh.across[warp][four], down = sh.down[warp][four];
+                        if (now == kPartial && p.q_docs) docs = sh.docs[warp][four];
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
+                        for (int u = 0; u < 4; ++u) {
                             const int at = c + e + u;
-                            const float level = KEYS ? sh.row[warp][at].x : lse;
-                            float x;
-                            if constexpr (GENERAL) {
-                                if (p.cap != 0.0f) {
-                                    const float tanh_x = tanh_of(prob[at] * inner);
-                                    slant[u] = fmaf(-tanh_x, tanh_x, 1.0f);
-                                    x = outer * tanh_x;
-                                } else {
-                                    x = prob[at] * factor;
-                                }
-                                if (p.slopes) {
-                                    float far;
-                                    if (p.width > 1) far = map_distance(here, sh.place[warp][at]);
-                                    else far = fabsf(here.y - static_cast<float>((KEYS ? m0 + mask.shift : m0) + at));
-                                    x = fmaf(-slope, far, x);
-                                }
-                                x -= level;
+                            level[u] = KEYS ? element(row_lse, u) : lse;
+                            if (BIAS == kMapBias) level[u] = fmaf(slope, fabsf(here.x - element(across, u)) + fabsf(here.y - element(down, u)), level[u]);
+                            if (BIAS == kSequenceBias) level[u] = fmaf(slope, fabsf(from - static_cast<float>(at)), level[u]);
+                            float slant = 1.0f;
+                            if (CAP) {
+                                const float tanh_x = tanh_of(prob[at] * inner);
+                                slant = fmaf(-tanh_x, tanh_x, 1.0f);
+                                value[u] = fmaf(outer, tanh_x, -level[u]);
                             } else {
-                                x = fmaf(prob[at], factor, -level);
+                                value[u] = fmaf(prob[at], factor, -level[u]);
                             }
                             if (now == kPartial) {
-                                bool seen = KEYS ? m0 + at >= first : m0 + at < limit;
-                                if (p.q_docs) seen = seen && doc >= 0 && sh.docs[warp][at] == doc;
-                                x = seen ? x : -INFINITY;
+                                bool seen = KEYS ? at >= bar : at < bar;
+                                if (p.q_docs) seen = seen && element(docs, u) == doc;
+                                value[u] = seen ? value[u] : -INFINITY;
                             }
-                            pair[u] = exp2_fast(x);
-                            prob[at] = GENERAL ? pair[u] * slant[u] : pair[u];
+                            value[u] = exp2_fast(value[u]);
+                            prob[at] = CAP ? value[u] * slant : value[u];
                         }
-                        packed[e / 2] = pack_two<T>(pair[0], pair[1]);
+                        packed[e / 2] = pack_two<T>(value[0], value[1]);
+                        packed[e / 2 + 1] = pack_two<T>(value[2], value[3]);
                     }
                     if (KEYS) tmem_store16(my_scores + c / 2, packed);
                 }
@@ -294,16 +304,19 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     tmem_load32(my_slopes + c, dp);
                     tmem_loaded32(dp);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float pair[2];
+                    for (int e = 0; e < 32; e += 4) {
+                        float4 row_delta;
+                        if (KEYS) row_delta = sh.delta[warp][(c + e) / 4];
+                        float value[4];
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
+                        for (int u = 0; u < 4; ++u) {
                             const int at = c + e + u;
-                            const float off = __uint_as_float(dp[e + u]) - (KEYS ? sh.row[warp][at].y : delta);
-                            pair[u] = prob[at] * (HALF ? off * hold : off);
-                            if (now == kPartial && prob[at] == 0.0f) pair[u] = 0.0f;
+                            const float off = __uint_as_float(dp[e + u]) - (KEYS ? element(row_delta, u) : delta);
+                            value[u] = prob[at] * (HALF ? off * hold : off);
+                            if (now == kPartial && prob[at] == 0.0f) value[u] = 0.0f;
                         }
-                        packed[e / 2] = pack_two<T>(pair[0], pair[1]);
+                        packed[e / 2] = pack_two<T>(value[0], value[1]);
+                        packed[e / 2 + 1] = pack_two<T>(value[2], value[3]);
                     }
                     tmem_store16(my_slopes + c / 2, packed);
                 }
@@ -354,38 +367,32 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
     if (warp == 9) tmem_give(tmem);
 }
 
-template <typename T, int DP, bool GENERAL, bool KEYS>
+template <typename T, int DP, bool CAP, GlobalBias BIAS, bool KEYS>
 cudaError_t backward_pass(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
 {
     constexpr size_t smem = sizeof(BackShared<DP>) + 1024;
     static_assert(smem <= 227 * 1024 && smem > 114 * 1024, "one block per SM: it takes all of the tensor memory");
-    const auto kernel = global_backward_kernel<T, DP, GENERAL, KEYS>;
+    const auto kernel = global_backward_kernel<T, DP, CAP, BIAS, KEYS>;
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (err != cudaSuccess) return err;
     const dim3 grid(static_cast<unsigned>(p.B) * (KEYS ? p.hk : p.h) * (((KEYS ? p.M : p.N) + kTile - 1) / kTile));
     return launch_chained(kernel, grid, kBackThreads, smem, stream, p, maps);
 }
 
-template <typename T, int DP, bool GENERAL>
-cudaError_t backward_one(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
-{
-    const cudaError_t err = backward_pass<T, DP, GENERAL, true>(p, maps, stream);
-    return err != cudaSuccess ? err : backward_pass<T, DP, GENERAL, false>(p, maps, stream);
-}
-
-template <typename T>
-cudaError_t backward_type(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
-{
-    const bool general = p.cap != 0.0f || p.slopes != nullptr;
-    if (p.d <= 64) return general ? backward_one<T, 64, true>(p, maps, stream) : backward_one<T, 64, false>(p, maps, stream);
-    return general ? backward_one<T, 128, true>(p, maps, stream) : backward_one<T, 128, false>(p, maps, stream);
-}
-
 }  // namespace
 
-cudaError_t run_global_backward(const GlobalParams &p, const GlobalMaps &maps, int dtype, cudaStream_t stream)
+template <typename T>
+cudaError_t run_global_backward(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
 {
-    return dtype == MATCHATTN_F16 ? backward_type<__half>(p, maps, stream) : backward_type<__nv_bfloat16>(p, maps, stream);
+    return by_scores(p, [&](auto width, auto cap, auto bias) {
+        constexpr int DP = decltype(width)::value;
+        constexpr bool CAP = decltype(cap)::value;
+        constexpr GlobalBias BIAS = decltype(bias)::value;
+        const cudaError_t err = backward_pass<T, DP, CAP, BIAS, true>(p, maps, stream);
+        return err != cudaSuccess ? err : backward_pass<T, DP, CAP, BIAS, false>(p, maps, stream);
+    });
 }
+
+template cudaError_t run_global_backward<MATCHATTN_T>(const GlobalParams &, const GlobalMaps &, cudaStream_t);
 
 }  // namespace matchattn

@@ -1,4 +1,5 @@
-// Dense attention, forward, 16-bit types of up to 128 channels, on the matrix units.
+// Dense attention, forward, 16-bit types of up to 128 channels, on the matrix units.  Included once per type with MATCHATTN_T
+// defined.
 //
 // A block owns 256 queries of a head as two tiles of 128 (or one tile, when the call has too few for the chip), a thread a query.
 // Warps 0-3 and 4-7 take the softmax of one tile each, warp 8 copies tiles of K and V into a ring of buffers (tensor memory
@@ -32,12 +33,12 @@ struct ForwardShared {
     int broken, by_hand[2], odd[2][3];
 };
 
-// GENERAL: scores capped or with a bias
-template <typename T, int DP, bool GENERAL>
+template <typename T, int DP, bool CAP, GlobalBias BIAS>
 __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(const GlobalParams p, const __grid_constant__ GlobalMaps maps)
 {
     chain_begin();
     constexpr int STAGES = ForwardShared<DP>::kStages;
+    constexpr bool GENERAL = CAP || BIAS != kNoBias;
     extern __shared__ uint8_t raw_shared[];
     ForwardShared<DP> &sh = *reinterpret_cast<ForwardShared<DP> *>(raw_shared + (1024 - (shared_address(raw_shared) & 1023)) % 1024);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -169,11 +170,11 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
         const uint32_t mine = tmem + (static_cast<uint32_t>(warp & 3) << 21);        // lanes 32 (warp mod 4) on
         const uint32_t scores = mine + w * kTile, out = mine + 256 + w * kTile;
         const float factor = p.scale * kLog2e;
-        const float inner = p.cap != 0.0f ? 2.0f * factor / p.cap : 0.0f, outer = p.cap * kLog2e;
+        const float inner = CAP ? 2.0f * factor / p.cap : 0.0f, outer = p.cap * kLog2e;
         const int doc = p.q_docs && n < p.N ? p.q_docs[static_cast<long long>(b) * p.N + n] : -1;
         const int limit = p.q_docs && doc < 0 ? 0 : key_limit(mask, n);
-        const float slope = GENERAL && p.slopes ? p.slopes[head] * kLog2e : 0.0f;
-        const float2 here = GENERAL ? map_place(n + mask.shift, p.width) : make_float2(0.0f, 0.0f);
+        const float slope = BIAS != kNoBias ? p.slopes[head] * kLog2e : 0.0f;
+        const float2 here = BIAS != kNoBias ? map_place(n + mask.shift, p.width) : make_float2(0.0f, 0.0f);
         float ref = -INFINITY, sum = 0.0f;
         int used = 0, buffers = 0, looks = 0;
         bool good = true;
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                 continue;
             }
             const int j0 = t * kTile;
-            if (GENERAL && p.slopes && p.width > 1) {
+            if (BIAS == kMapBias) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sh.place[warp][lane + 32 * i] = map_place(j0 + lane + 32 * i, p.width);
             }
@@ -211,26 +212,19 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                 tmem_loaded32(raw[c / 32 % 2]);
                 if (c + 32 < kTile) tmem_load32(scores + c + 32, raw[(c / 32 + 1) % 2]);
                 if constexpr (GENERAL) {
-                    if (p.cap != 0.0f) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = outer * tanh_of(x[i] * inner);
-                    } else {
+                    for (int i = 0; i < 32; ++i) x[i] = CAP ? outer * tanh_of(x[i] * inner) : x[i] * factor;
+                    if constexpr (BIAS == kMapBias) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] *= factor;
-                    }
-                    if (p.slopes) {
-                        if (p.width > 1) {
-#pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                const float4 two = *reinterpret_cast<const float4 *>(&sh.place[warp][c + i]);
-                                x[i] = fmaf(-slope, fabsf(here.x - two.x) + fabsf(here.y - two.y), x[i]);
-                                x[i + 1] = fmaf(-slope, fabsf(here.x - two.z) + fabsf(here.y - two.w), x[i + 1]);
-                            }
-                        } else {
-                            const float from = here.y - static_cast<float>(j0 + c);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) x[i] = fmaf(-slope, fabsf(from - static_cast<float>(i)), x[i]);
+                        for (int i = 0; i < 32; i += 2) {
+                            const float4 two = *reinterpret_cast<const float4 *>(&sh.place[warp][c + i]);
+                            x[i] = fmaf(-slope, fabsf(here.x - two.x) + fabsf(here.y - two.y), x[i]);
+                            x[i + 1] = fmaf(-slope, fabsf(here.x - two.z) + fabsf(here.y - two.w), x[i + 1]);
                         }
+                    } else if constexpr (BIAS == kSequenceBias) {
+                        const float from = here.y - static_cast<float>(j0 + c);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] = fmaf(-slope, fabsf(from - static_cast<float>(i)), x[i]);
                     }
                 }
                 if (now == kPartial) {
@@ -361,31 +355,28 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
     if (warp == 9) tmem_give(tmem);
 }
 
-template <typename T, int DP, bool GENERAL>
+template <typename T, int DP, bool CAP, GlobalBias BIAS>
 cudaError_t forward_one(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
 {
     constexpr size_t smem = sizeof(ForwardShared<DP>) + 1024;
     static_assert(smem <= 227 * 1024 && smem > 114 * 1024, "one block per SM: it takes all of the tensor memory");
-    const auto kernel = global_forward_kernel<T, DP, GENERAL>;
+    const auto kernel = global_forward_kernel<T, DP, CAP, BIAS>;
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (err != cudaSuccess) return err;
     const dim3 grid(static_cast<unsigned>(p.B) * p.h * p.splits * ((p.N + p.block_rows - 1) / p.block_rows));
     return launch_chained(kernel, grid, kForwardThreads, smem, stream, p, maps);
 }
 
-template <typename T>
-cudaError_t forward_type(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
-{
-    const bool general = p.cap != 0.0f || p.slopes != nullptr;
-    if (p.d <= 64) return general ? forward_one<T, 64, true>(p, maps, stream) : forward_one<T, 64, false>(p, maps, stream);
-    return general ? forward_one<T, 128, true>(p, maps, stream) : forward_one<T, 128, false>(p, maps, stream);
-}
-
 }  // namespace
 
-cudaError_t run_global_forward(const GlobalParams &p, const GlobalMaps &maps, int dtype, cudaStream_t stream)
+template <typename T>
+cudaError_t run_global_forward(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream)
 {
-    return dtype == MATCHATTN_F16 ? forward_type<__half>(p, maps, stream) : forward_type<__nv_bfloat16>(p, maps, stream);
+    return by_scores(p, [&](auto width, auto cap, auto bias) {
+        return forward_one<T, decltype(width)::value, decltype(cap)::value, decltype(bias)::value>(p, maps, stream);
+    });
 }
+
+template cudaError_t run_global_forward<MATCHATTN_T>(const GlobalParams &, const GlobalMaps &, cudaStream_t);
 
 }  // namespace matchattn

@@ -1,5 +1,5 @@
 // Dense attention on the matrix units: tiles, barriers, tensor maps and the instructions around tcgen05.mma, for the kernels of
-// matchattn_global_fwd.cu and matchattn_global_bwd.cu.
+// matchattn_global_fwd.inl and matchattn_global_bwd.inl.
 //
 // Tiles.  128 rows (tokens) of a head, up to 128 channels, as one or two halves of 64 channels; a half is 128 rows of 128 bytes,
 // 16-byte pieces swizzled by the row (piece ^ (row & 7)), as the tensor memory accelerator writes it and the matrix unit reads it.
@@ -8,6 +8,8 @@
 #pragma once
 
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "matchattn_global.cuh"
 
@@ -332,6 +334,9 @@ __device__ __forceinline__ int key_limit(const GlobalMask &m, int n)
 
 enum TileState { kHidden, kPartial, kWhole };
 
+// By the tokens' distance: none, in a sequence, on a map.
+enum GlobalBias { kNoBias, kSequenceBias, kMapBias };
+
 // What the queries [n0, n0 + 128) see of the keys [j0, j0 + 128).
 __device__ __forceinline__ int tile_state(const GlobalMask &m, int N, int n0, int j0, const DocRange *qr, const DocRange *kr)
 {
@@ -355,8 +360,23 @@ inline bool rows_fit(const void *base, const long long (&stride)[3], int B, int 
     return true;
 }
 
-cudaError_t run_global_forward(const GlobalParams &p, const GlobalMaps &maps, int dtype, cudaStream_t stream);
-cudaError_t run_global_backward(const GlobalParams &p, const GlobalMaps &maps, int dtype, cudaStream_t stream);
+// Builds by what a score goes through: calls f(channels of a tile, capped, bias) as types.
+template <typename F>
+cudaError_t by_scores(const GlobalParams &p, F f)
+{
+    const auto bias = [&](auto width, auto cap) {
+        if (p.slopes == nullptr) return f(width, cap, std::integral_constant<GlobalBias, kNoBias>());
+        if (p.width == 1) return f(width, cap, std::integral_constant<GlobalBias, kSequenceBias>());
+        return f(width, cap, std::integral_constant<GlobalBias, kMapBias>());
+    };
+    const auto cap = [&](auto width) { return p.cap != 0.0f ? bias(width, std::true_type()) : bias(width, std::false_type()); };
+    return p.d <= 64 ? cap(std::integral_constant<int, 64>()) : cap(std::integral_constant<int, 128>());
+}
+
+template <typename T>
+cudaError_t run_global_forward(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream);
+template <typename T>
+cudaError_t run_global_backward(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream);
 
 
 }  // namespace matchattn
