@@ -360,13 +360,15 @@ MATCHATTN_API int matchattn_flow_init(const void *correlation, void *prob, void 
  *   q [B, N, h, d], k and v [B, M, hk, d] with the strides given (elements; item, token, head; channels are contiguous)
  *   out [B, N, h, d], contiguous, written.  h is a multiple of hk: query heads [i*h/hk, (i+1)*h/hk) share key head i.
  *   lse [B, h, N] float32, written: log2 of the sum of 2^(x log2 e) of a row, for the backward pass; may be NULL without one
+ *   out_low [B, N, h, d], contiguous, written in 16-bit types: what the rounding of out left, for the backward pass, whose row sums
+ *     of d_out * out would lose half their digits without it; may be NULL (not used in float32)
  *   d <= MATCHATTN_MAX_DENSE_D; 0 <= M <= 2^24; 0 < N <= 2^24; scale > 0; cap >= 0 (0: none); prefix needs causal.
  * Scores, softmax and sums are float32.  The sums do not depend on timing: equal calls give equal bits.
  */
 #define MATCHATTN_MAX_DENSE_D 256
 typedef struct matchattn_global_args {
     const void *q, *k, *v;
-    void *out;
+    void *out, *out_low;
     float *lse;
     long long q_stride[3], k_stride[3], v_stride[3];
     const float *slopes;               /* [h] or NULL                          */
@@ -380,8 +382,8 @@ typedef struct matchattn_global_args {
 /* Scratch bytes that the forward (backward = 0) or the backward call needs for these arguments (possibly 0); 0 if they are refused. */
 MATCHATTN_API size_t matchattn_global_scratch_bytes(const matchattn_global_args *args, int backward);
 MATCHATTN_API int matchattn_global_forward(const matchattn_global_args *args, void *scratch, size_t scratch_bytes, void *cuda_stream);
-/* Gradients to q, k and v, contiguous as [B, N, h, d] and [B, M, hk, d], from that of out (contiguous); args->out and args->lse
- * are the forward call's.  The probabilities are recomputed; scratch is 16-byte aligned, as in the forward call. */
+/* Gradients to q, k and v, contiguous as [B, N, h, d] and [B, M, hk, d], from that of out (contiguous); args->out, args->out_low
+ * and args->lse are the forward call's.  The probabilities are recomputed; scratch is 16-byte aligned, as in the forward call. */
 MATCHATTN_API int matchattn_global_backward(const matchattn_global_args *args, const void *d_out, void *d_q, void *d_k, void *d_v,
                                             void *scratch, size_t scratch_bytes, void *cuda_stream);
 

@@ -37,7 +37,7 @@ _strides = ctypes.c_longlong * 3
 
 class GlobalArgs(ctypes.Structure):
     """matchattn_global_args"""
-    _fields_ = [(n, _vp) for n in ("q", "k", "v", "out", "lse")] + \
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "out", "out_low", "lse")] + \
         [(n, _strides) for n in ("q_stride", "k_stride", "v_stride")] + \
         [(n, _vp) for n in ("slopes", "prefix", "lengths", "q_docs", "k_docs")] + \
         [(n, _i) for n in ("B", "N", "M", "h", "hk", "d", "dtype", "causal", "width")] + [("scale", _f), ("cap", _f)]

@@ -254,10 +254,11 @@ struct GlobalCall {
     int64_t width;
     bool causal;
 
-    matchattn_global_args args(const Tensor &out, const Tensor &lse) const
+    matchattn_global_args args(const Tensor &out, const Tensor &low, const Tensor &lse) const
     {
         matchattn_global_args a{};
-        a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr(), a.out = out.data_ptr(), a.lse = data_as<float>(lse);
+        a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr(), a.out = out.data_ptr(), a.out_low = data_as<void>(low);
+        a.lse = data_as<float>(lse);
         for (int i = 0; i < 3; ++i) a.q_stride[i] = q.stride(i), a.k_stride[i] = k.stride(i), a.v_stride[i] = v.stride(i);
         a.slopes = data_as<float>(slopes), a.prefix = data_as<int>(prefix), a.lengths = data_as<int>(lengths);
         a.q_docs = data_as<int>(q_docs), a.k_docs = data_as<int>(k_docs);
@@ -267,14 +268,15 @@ struct GlobalCall {
         return a;
     }
 
-    // The output, and lse where it is wanted; the tensors' device is current.
-    Tensor forward(Tensor *lse) const
+    // The output, and where they are wanted lse and what the rounding left; the tensors' device is current.
+    Tensor forward(Tensor *lse, Tensor *low) const
     {
         const int64_t B = q.size(0), N = q.size(1), h = q.size(2);
         Tensor out = at::empty({B, N, h, q.size(3)}, q.options());
         if (lse != nullptr) *lse = at::empty({B, h, N}, q.options().dtype(at::kFloat));
+        if (low != nullptr && dtype_code(q) != MATCHATTN_F32) *low = at::empty(out.sizes(), out.options());
         if (out.numel() == 0) return out;
-        const matchattn_global_args a = args(out, lse != nullptr ? *lse : Tensor());
+        const matchattn_global_args a = args(out, low != nullptr ? *low : Tensor(), lse != nullptr ? *lse : Tensor());
         const size_t bytes = matchattn_global_scratch_bytes(&a, 0);
         Tensor scratch;
         if (bytes != 0) scratch = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
@@ -290,8 +292,8 @@ struct GlobalAttentionFn : torch::autograd::Function<GlobalAttentionFn> {
         c.q = with_rows(q), c.k = with_rows(k), c.v = with_rows(v);
         const c10::cuda::CUDAGuard device(q.device());
         RECORD_FUNCTION(kGlobalName, std::vector<c10::IValue>({q, k, v}));
-        Tensor lse, out = c.forward(&lse);
-        ctx->save_for_backward({q, k, v, out, lse, c.slopes, c.prefix, c.lengths, c.q_docs, c.k_docs});
+        Tensor lse, low, out = c.forward(&lse, &low);
+        ctx->save_for_backward({q, k, v, out, low, lse, c.slopes, c.prefix, c.lengths, c.q_docs, c.k_docs});
         ctx->saved_data["scale"] = c.scale;
         ctx->saved_data["cap"] = c.cap;
         ctx->saved_data["width"] = c.width;
@@ -302,9 +304,9 @@ struct GlobalAttentionFn : torch::autograd::Function<GlobalAttentionFn> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
     {
         const auto s = ctx->get_saved_variables();
-        GlobalCall c{with_rows(s[0]), with_rows(s[1]), with_rows(s[2]), s[5], s[6], s[7], s[8], s[9], ctx->saved_data["scale"].toDouble(),
+        GlobalCall c{with_rows(s[0]), with_rows(s[1]), with_rows(s[2]), s[6], s[7], s[8], s[9], s[10], ctx->saved_data["scale"].toDouble(),
                      ctx->saved_data["cap"].toDouble(), ctx->saved_data["width"].toInt(), ctx->saved_data["causal"].toBool()};
-        const Tensor &out = s[3], &lse = s[4];
+        const Tensor &out = s[3], &low = s[4], &lse = s[5];
         const c10::cuda::CUDAGuard device(out.device());
         const Tensor d_out = grads[0].contiguous().resolve_neg();
         const auto like = [](const Tensor &t) { return at::empty(t.sizes(), t.options()); };
@@ -313,7 +315,7 @@ struct GlobalAttentionFn : torch::autograd::Function<GlobalAttentionFn> {
             d_k.zero_();
             d_v.zero_();
         } else {
-            const matchattn_global_args a = c.args(out, lse);
+            const matchattn_global_args a = c.args(out, low, lse);
             const size_t bytes = matchattn_global_scratch_bytes(&a, 1);
             Tensor scratch;
             if (bytes != 0) scratch = at::empty({static_cast<int64_t>(bytes)}, out.options().dtype(at::kByte));
@@ -691,7 +693,7 @@ PyObject *global_attention(PyObject *const *a, Py_ssize_t n)
             const c10::cuda::CUDAGuard device(c.q.device());
             RECORD_FUNCTION(kGlobalName, std::vector<c10::IValue>({c.q, c.k, c.v}));
             c.q = with_rows(c.q), c.k = with_rows(c.k), c.v = with_rows(c.v);
-            out = c.forward(nullptr);
+            out = c.forward(nullptr, nullptr);
         }
     }
     return THPVariable_Wrap(out);

@@ -17,7 +17,7 @@ struct DocRange;
 
 struct GlobalParams {
     const void *q, *k, *v;
-    void *out;               // [B, N, h, d]
+    void *out, *low;         // [B, N, h, d]; low, 16-bit types: what the rounding of out left, or null
     float *lse;              // [B, h, N] log2 of the sum of 2^x of a row, +inf for a row that sees nothing; or null
     long long qs[3], ks[3], vs[3];      // strides in elements: item, token, head
     const float *slopes;                // [h] or null
@@ -87,6 +87,15 @@ __device__ __forceinline__ float2 map_place(int pos, int width)
 }
 
 __device__ __forceinline__ float map_distance(float2 a, float2 b) { return fabsf(a.x - b.x) + fabsf(a.y - b.y); }
+
+// A result, and what its rounding left.
+template <typename T>
+__device__ __forceinline__ void store_result(const GlobalParams &p, long long at, float x)
+{
+    T *out = static_cast<T *>(p.out) + at;
+    store_one<T>(out, x);
+    if (sizeof(T) == 2 && p.low != nullptr) store_one<T>(static_cast<T *>(p.low) + at, x - DT<T>::rnd(x));
+}
 
 cudaError_t run_global_any_forward(const GlobalParams &p, int dtype, cudaStream_t stream);
 cudaError_t run_global_any_backward(const GlobalParams &p, int dtype, cudaStream_t stream);

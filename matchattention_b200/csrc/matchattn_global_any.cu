@@ -280,10 +280,10 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_forward_kernel(const G
                 if (tx + 16 * c < p.d) p.part_out[part * p.d + tx + 16 * c] = empty ? 0.0f : acc[i][c] * inv;
         } else {
             if (p.lse && tx == 0) p.lse[row] = empty ? INFINITY : lse;
-            T *out = static_cast<T *>(p.out) + ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
+            const long long out = ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
-                if (tx + 16 * c < p.d) store_one<T>(out + tx + 16 * c, empty ? 0.0f : acc[i][c] * inv);
+                if (tx + 16 * c < p.d) store_result<T>(p, out + tx + 16 * c, empty ? 0.0f : acc[i][c] * inv);
         }
     }
 }

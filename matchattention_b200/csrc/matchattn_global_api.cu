@@ -34,52 +34,91 @@ __global__ void __launch_bounds__(256) global_join_kernel(const GlobalParams p)
     const long long bh = row / p.N, b = bh / p.h, head = bh - b * p.h;
     const bool empty = sum == 0.0f;
     if (p.lse && lane == 0) p.lse[row] = empty ? INFINITY : ref + log2f(sum);
-    T *out = static_cast<T *>(p.out) + ((b * p.N + n) * p.h + head) * p.d;
+    const long long out = ((b * p.N + n) * p.h + head) * p.d;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < p.d) store_one<T>(out + lane + 32 * i, empty ? 0.0f : acc[i] / sum);
+        if (lane + 32 * i < p.d) store_result<T>(p, out + lane + 32 * i, empty ? 0.0f : acc[i] / sum);
 }
 
-// delta = sum over the channels of d_out * out: a warp per row.  With `norms` also the largest norm of a row of d_out, and, by the
-// rows after those, of v (maxima do not depend on their order).  Bound by memory.
-template <typename T>
-__global__ void __launch_bounds__(256) global_delta_kernel(const GlobalParams p)
+// A sum over the channels of V per lane, `lanes` to a row.
+template <typename T, int V>
+__device__ __forceinline__ void read_channels(const T *p, float (&x)[V])
+{
+    if constexpr (V == 1) {
+        x[0] = load_one<T>(p);
+    } else {
+        const uint4 t = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = DT<T>::unpack(w[i / DT<T>::kElemsPerWord], i % DT<T>::kElemsPerWord);
+    }
+}
+
+// delta = sum over the channels of d_out * out (with what its rounding left): `lanes` lanes per row, V channels at a time (16 bytes, or
+// one element).  With `norms` also the largest norm of a row of d_out and, by the rows after those, of v (maxima do not depend on their
+// order).  Bound by memory; 2 x 4096 tokens, 16 heads x 128, bfloat16, by single elements and a warp per row 36 us.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) global_delta_kernel(const GlobalParams p, int lanes)
 {
     chain_begin();
     const long long rows = static_cast<long long>(p.B) * p.N * p.h, more = p.norms ? static_cast<long long>(p.B) * p.M * p.hk : 0;
-    const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
+    const long long row = static_cast<long long>(blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
+    const int lane = threadIdx.x & (lanes - 1);
     __shared__ int largest[2];
     if (threadIdx.x < 2) largest[threadIdx.x] = 0;
     __syncthreads();
-    float square = 0.0f;
-    const bool of_v = row >= rows;
+    float square = 0.0f, sum = 0.0f;
     if (row < rows) {
         const T *o = static_cast<const T *>(p.out) + row * p.d, *g = static_cast<const T *>(p.d_out) + row * p.d;
-        float sum = 0.0f;
-        for (int c = lane; c < p.d; c += 32) {
-            const float y = load_one<T>(g + c);
-            sum = fmaf(load_one<T>(o + c), y, sum);
-            square = fmaf(y, y, square);
-        }
+        const T *low = p.low ? static_cast<const T *>(p.low) + row * p.d : nullptr;
+        for (int c = lane * V; c < p.d; c += lanes * V) {
+            float x[V], y[V], z[V] = {};
+            read_channels<T, V>(o + c, x);
+            read_channels<T, V>(g + c, y);
+            if (low) read_channels<T, V>(low + c, z);
 #pragma unroll
-        for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-        const long long bn = row / p.h, head = row - bn * p.h, b = bn / p.N, n = bn - b * p.N;
-        if (lane == 0) p.delta[(b * p.h + head) * p.N + n] = sum;
+            for (int i = 0; i < V; ++i) {
+                sum = fmaf(x[i], y[i], fmaf(z[i], y[i], sum));
+                square = fmaf(y[i], y[i], square);
+            }
+        }
     } else if (row < rows + more) {
         const long long bj = (row - rows) / p.hk, head = row - rows - bj * p.hk, b = bj / p.M, j = bj - b * p.M;
         const T *v = static_cast<const T *>(p.v) + b * p.vs[0] + j * p.vs[1] + head * p.vs[2];
-        for (int c = lane; c < p.d; c += 32) square = fmaf(load_one<T>(v + c), load_one<T>(v + c), square);
+        for (int c = lane * V; c < p.d; c += lanes * V) {
+            float x[V];
+            read_channels<T, V>(v + c, x);
+#pragma unroll
+            for (int i = 0; i < V; ++i) square = fmaf(x[i], x[i], square);
+        }
+    }
+    for (int i = lanes / 2; i > 0; i >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, i);
+        square += __shfl_xor_sync(0xffffffffu, square, i);
+    }
+    if (row < rows && lane == 0) {
+        const long long bn = row / p.h, head = row - bn * p.h, b = bn / p.N, n = bn - b * p.N;
+        p.delta[(b * p.h + head) * p.N + n] = sum;
     }
     if (p.norms) {
-#pragma unroll
-        for (int i = 16; i > 0; i >>= 1) square += __shfl_xor_sync(0xffffffffu, square, i);
         const float norm = sqrtf(square);
         // floats that are not negative are ordered as their bits
-        if (lane == 0 && norm <= 3.402823466e38f) atomicMax(largest + of_v, __float_as_int(norm));
+        if (lane == 0 && norm <= 3.402823466e38f) atomicMax(largest + (row >= rows), __float_as_int(norm));
         __syncthreads();
         if (threadIdx.x < 2 && largest[threadIdx.x] > 0) atomicMax(reinterpret_cast<int *>(p.norms) + threadIdx.x, largest[threadIdx.x]);
     }
+}
+
+template <typename T>
+cudaError_t find_delta(const GlobalParams &p, bool wide, cudaStream_t stream)
+{
+    constexpr int V = 16 / sizeof(T);
+    int lanes = 32;
+    while (wide && lanes > 1 && lanes / 2 * V >= p.d) lanes /= 2;
+    const long long rows = 1LL * p.B * p.N * p.h + (p.norms ? 1LL * p.B * p.M * p.hk : 0);
+    const dim3 grid(static_cast<unsigned>((rows + 256 / lanes - 1) / (256 / lanes)));
+    return wide ? launch_chained(global_delta_kernel<T, V>, grid, 256, 0, stream, p, lanes)
+                : launch_chained(global_delta_kernel<T, 1>, grid, 256, 0, stream, p, lanes);
 }
 
 // What the ids of a block of 128 tokens span: blocks of queries of all items, then blocks of keys.
@@ -128,7 +167,7 @@ int check_global(const matchattn_global_args *a)
     if (a->prefix && !a->causal) return MATCHATTN_ERR_SHAPE;
     if (a->dtype < MATCHATTN_F32 || a->dtype > MATCHATTN_BF16) return MATCHATTN_ERR_DTYPE;
     const size_t size = a->dtype == MATCHATTN_F32 ? 4 : 2;
-    if (!aligned(a->q, size) || !aligned(a->k, size) || !aligned(a->v, size) || !aligned(a->out, size) || !aligned(a->lse, 4) ||
+    if (!aligned(a->q, size) || !aligned(a->k, size) || !aligned(a->v, size) || !aligned(a->out, size) || !aligned(a->out_low, size) || !aligned(a->lse, 4) ||
         !aligned(a->slopes, 4) || !aligned(a->prefix, 4) || !aligned(a->lengths, 4) || !aligned(a->q_docs, 4) || !aligned(a->k_docs, 4))
         return MATCHATTN_ERR_ALIGN;
     // positions are exact in float32; rows of a key head and grid dimensions are 32- and 16-bit
@@ -155,7 +194,7 @@ constexpr int kTokenRows = 16;
 
 bool matrix_call(const matchattn_global_args *a)
 {
-    return a->dtype != MATCHATTN_F32 && a->d <= 128 && a->d % 8 == 0 && aligned(a->out, 16) && rows_fit(a->q, a->q_stride, a->B, a->N, a->h) &&
+    return a->dtype != MATCHATTN_F32 && a->d <= 128 && a->d % 8 == 0 && aligned(a->out, 16) && aligned(a->out_low, 16) && rows_fit(a->q, a->q_stride, a->B, a->N, a->h) &&
            rows_fit(a->k, a->k_stride, a->B, a->M, a->hk) && rows_fit(a->v, a->v_stride, a->B, a->M, a->hk);
 }
 
@@ -255,6 +294,7 @@ GlobalParams params_of(const matchattn_global_args *a)
 {
     GlobalParams p{};
     p.q = a->q, p.k = a->k, p.v = a->v, p.out = a->out, p.lse = a->lse;
+    p.low = a->dtype == MATCHATTN_F32 ? nullptr : a->out_low;
     for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i], p.ks[i] = a->k_stride[i], p.vs[i] = a->v_stride[i];
     p.slopes = a->slopes, p.prefix = a->prefix, p.lengths = a->lengths, p.q_docs = a->q_docs, p.k_docs = a->k_docs;
     p.B = a->B, p.N = a->N, p.M = a->M, p.h = a->h, p.hk = a->hk, p.g = a->h / a->hk, p.d = a->d;
@@ -338,16 +378,13 @@ extern "C" int matchattn_global_backward(const matchattn_global_args *a, const v
     p.delta = reinterpret_cast<float *>(ranges + range_count(a));
     const bool matrix = matrix_call(a) && aligned(d_out, 16) && aligned(d_q, 16) && aligned(d_k, 16) && aligned(d_v, 16);
     cudaError_t err = cudaSuccess;
-    long long rows = static_cast<long long>(backward_floats(a));
     if (matrix && a->dtype == MATCHATTN_F16) {
         p.norms = static_cast<float *>(scratch);
-        rows += 1LL * a->B * a->M * a->hk;
         err = cudaMemsetAsync(scratch, 0, 16, stream);
     }
-    if (err == cudaSuccess)
-        err = by_type(a->dtype, [&](auto t) {
-            return launch_chained(global_delta_kernel<decltype(t)>, dim3(static_cast<unsigned>((rows + 7) / 8)), 256, 0, stream, p);
-        });
+    // (the rows of v are read for the matrix kernels alone, which have them aligned)
+    const bool wide = a->d % (16 / static_cast<int>(size)) == 0 && aligned(a->out, 16) && aligned(a->out_low, 16) && aligned(d_out, 16);
+    if (err == cudaSuccess) err = by_type(a->dtype, [&](auto t) { return find_delta<decltype(t)>(p, wide, stream); });
     if (err == cudaSuccess && matrix) {
         GlobalMaps maps{};
         const long long stride[3] = {1LL * a->N * a->h * a->d, 1LL * a->h * a->d, a->d};

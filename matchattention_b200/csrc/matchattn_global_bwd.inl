@@ -355,9 +355,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 for (int e = 0; e < 32; ++e) y[e] = good ? __uint_as_float(raw[e]) * times : NAN;
 #pragma unroll
                 for (int e = 0; e < 32; e += 8)
-                    if (c + e < p.d)
-                        *reinterpret_cast<uint4 *>(to + c + e) = make_uint4(pack_two<T>(y[e], y[e + 1]), pack_two<T>(y[e + 2], y[e + 3]),
-                                                                            pack_two<T>(y[e + 4], y[e + 5]), pack_two<T>(y[e + 6], y[e + 7]));
+                    if (c + e < p.d) store_eight<T>(to + c + e, y + e);
             }
             __syncwarp();
         }

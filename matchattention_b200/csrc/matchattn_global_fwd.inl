@@ -339,12 +339,19 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                     for (int i = 0; i < 32; i += 4)
                         if (c + i < p.d) *reinterpret_cast<float4 *>(to + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
                 } else {
-                    T *to = static_cast<T *>(p.out) + ((static_cast<long long>(b) * p.N + n) * p.h + head) * p.d + c;
+                    const long long to = ((static_cast<long long>(b) * p.N + n) * p.h + head) * p.d + c;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-                        if (c + i < p.d)
-                            *reinterpret_cast<uint4 *>(to + i) = make_uint4(pack_two<T>(y[i], y[i + 1]), pack_two<T>(y[i + 2], y[i + 3]),
-                                                                            pack_two<T>(y[i + 4], y[i + 5]), pack_two<T>(y[i + 6], y[i + 7]));
+                    for (int i = 0; i < 32; i += 8) {
+                        if (c + i < p.d) {
+                            store_eight<T>(static_cast<T *>(p.out) + to + i, y + i);
+                            if (p.low) {
+                                float rest[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) rest[e] = y[i + e] - DT<T>::rnd(y[i + e]);
+                                store_eight<T>(static_cast<T *>(p.low) + to + i, rest);
+                            }
+                        }
+                    }
                 }
                 __syncwarp();
             }

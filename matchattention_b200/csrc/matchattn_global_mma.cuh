@@ -250,6 +250,12 @@ __device__ __forceinline__ uint32_t pack_two(float low, float high)
     return DT<T>::pack(x);
 }
 
+template <typename T>
+__device__ __forceinline__ void store_eight(T *to, const float *x)
+{
+    *reinterpret_cast<uint4 *>(to) = make_uint4(pack_two<T>(x[0], x[1]), pack_two<T>(x[2], x[3]), pack_two<T>(x[4], x[5]), pack_two<T>(x[6], x[7]));
+}
+
 // zero times every element of a word, added to acc: NaN as soon as one is infinite or NaN
 template <typename T>
 __device__ __forceinline__ uint32_t taint(uint32_t w, uint32_t acc)

@@ -90,7 +90,7 @@ def test_norm_arguments_are_rejected_on_the_host():
 
 
 def test_structures_have_the_size_that_the_header_gives_them():
-    assert ctypes.sizeof(_lib.GlobalArgs) == 5 * 8 + 9 * 8 + 5 * 8 + 9 * 4 + 2 * 4 + 4
+    assert ctypes.sizeof(_lib.GlobalArgs) == 6 * 8 + 9 * 8 + 5 * 8 + 9 * 4 + 2 * 4 + 4
     assert ctypes.sizeof(_lib.NormArgs) == 2 * 8 + 6 * 8 + 4 * 8 + 8 + 10 * 4 + 4 + 4
 
 
