@@ -29,7 +29,7 @@ INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 SOURCES = ["matchattn_api.cu", "matchattn_f32.cu", "matchattn_f16.cu", "matchattn_bf16.cu",
            "matchattn_static_scratch.cu", "matchattn_upsample.cu", "matchattn_volume.cu", "matchattn_field_ops.cu", "matchattn_flow_init.cu", "matchattn_backward.cu",
-           "matchattn_norm_rotary.cu", "matchattn_global_api.cu", "matchattn_global_any.cu",
+           "matchattn_norm_rotary.cu", "matchattn_global_api.cu", "matchattn_global_any.cu", "matchattn_global_token.cu",
            "matchattn_global_fwd_f16.cu", "matchattn_global_fwd_bf16.cu", "matchattn_global_bwd_f16.cu", "matchattn_global_bwd_bf16.cu"]
 HEADERS = ["matchattn_kernels.cuh", "matchattn_lanes.cuh", "matchattn_launch.inl", "matchattn_mma.cuh", "matchattn_binned.cuh",
            "matchattn_staged.cuh", "matchattn_global.cuh", "matchattn_global_mma.cuh", "matchattn_global_fwd.inl", "matchattn_global_bwd.inl"]

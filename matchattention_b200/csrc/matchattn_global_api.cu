@@ -189,7 +189,7 @@ int splits_of(long long blocks, int tiles, int B)
     return s < 2 ? 1 : static_cast<int>(s);
 }
 
-// Queries times sharing heads up to which a call counts as one of single tokens.
+// Queries times sharing heads up to which a call counts as one of single tokens: the rows of a warp's matrix instruction.
 constexpr int kTokenRows = 16;
 
 bool matrix_call(const matchattn_global_args *a)
@@ -199,7 +199,7 @@ bool matrix_call(const matchattn_global_args *a)
 }
 
 struct Plan {
-    bool matrix;
+    bool matrix, token;
     int block_rows, splits, tiles_per_split;
     size_t part_out, part_lse;      // floats
     size_t ranges;                  // DocRange
@@ -216,9 +216,17 @@ Plan plan_forward(const matchattn_global_args *a)
     const int g = a->h / a->hk, rows = a->N * g;
     Plan p{};
     p.matrix = rows > kTokenRows && matrix_call(a);
+    p.token = rows <= kTokenRows && matrix_call(a);
     int tiles;
     long long blocks;
-    if (p.matrix) {
+    if (p.token) {
+        blocks = 1LL * a->hk * a->B;
+        tiles = (a->M + kTile - 1) / kTile;
+        // several blocks per SM one after another, because caches are filled unevenly, of four runs of keys per warp at least
+        const long long most = tiles / 4, wanted = (4LL * sm_count() + blocks - 1) / blocks;
+        p.splits = static_cast<int>(wanted < most ? wanted : most);
+        if (p.splits > 64) p.splits = 64;
+    } else if (p.matrix) {
         // two tiles of queries keep the matrix unit and the exponentials busy at once; one where two leave SMs idle
         blocks = 1LL * ((a->N + 2 * kTile - 1) / (2 * kTile)) * a->h * a->B;
         p.block_rows = 2 * kTile;
@@ -233,7 +241,8 @@ Plan plan_forward(const matchattn_global_args *a)
         blocks = 1LL * ((rows + bm - 1) / bm) * a->hk * a->B;
         tiles = (a->M + bn - 1) / bn;
     }
-    p.splits = splits_of(blocks, tiles, a->B);
+    if (!p.token) p.splits = splits_of(blocks, tiles, a->B);
+    if (p.splits < 1) p.splits = 1;
     p.tiles_per_split = p.splits > 1 ? (tiles + p.splits - 1) / p.splits : tiles;
     if (p.splits > 1) {
         p.splits = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
@@ -349,6 +358,8 @@ extern "C" int matchattn_global_forward(const matchattn_global_args *a, void *sc
         err = operand_maps(maps, a);
         if (err == cudaSuccess) err = find_ranges(p, static_cast<DocRange *>(scratch), stream);
         if (err == cudaSuccess) err = a->dtype == MATCHATTN_F16 ? run_global_forward<__half>(p, maps, stream) : run_global_forward<__nv_bfloat16>(p, maps, stream);
+    } else if (plan.token) {
+        err = run_global_token(p, a->dtype, stream);
     } else {
         err = run_global_any_forward(p, a->dtype, stream);
     }

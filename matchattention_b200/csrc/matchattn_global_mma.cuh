@@ -381,6 +381,7 @@ cudaError_t by_scores(const GlobalParams &p, F f)
 
 template <typename T>
 cudaError_t run_global_forward(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream);
+cudaError_t run_global_token(const GlobalParams &p, int dtype, cudaStream_t stream);
 template <typename T>
 cudaError_t run_global_backward(const GlobalParams &p, const GlobalMaps &maps, cudaStream_t stream);
 

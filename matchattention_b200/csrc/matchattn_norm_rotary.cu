@@ -44,25 +44,33 @@ struct NormParams {
     float eps, inv_d;
 };
 
+// V channels as they lie in memory
 template <typename T, int V>
-__device__ __forceinline__ void load_run(const T *p, float (&x)[V])
-{
-    constexpr int bytes = V * sizeof(T);
-    if constexpr (V == 1) {
-        x[0] = load_one<T>(p);
-    } else {
-        uint32_t w[bytes / 4];
-        if constexpr (bytes == 16) {
+struct Run {
+    static constexpr int kWords = V == 1 ? 1 : V * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void load(const T *p, bool there)
+    {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+        if (!there) return;
+        if constexpr (V == 1) {
+            w[0] = __float_as_uint(load_one<T>(p));
+        } else if constexpr (kWords == 4) {
             const uint4 t = *reinterpret_cast<const uint4 *>(p);
             w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
         } else {
             const uint2 t = *reinterpret_cast<const uint2 *>(p);
             w[0] = t.x, w[1] = t.y;
         }
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = DT<T>::unpack(w[i / DT<T>::kElemsPerWord], i % DT<T>::kElemsPerWord);
     }
-}
+    __device__ __forceinline__ float get(int i) const
+    {
+        if constexpr (V == 1) return __uint_as_float(w[0]);
+        else return DT<T>::unpack(w[i / DT<T>::kElemsPerWord], i % DT<T>::kElemsPerWord);
+    }
+};
 
 template <typename T, int V>
 __device__ __forceinline__ void store_run(T *p, const float (&x)[V])
@@ -140,7 +148,7 @@ __device__ __forceinline__ float group_sum(float v, int lanes)
 
 // T: element, V: channels per run, S: slots per lane, BACK: the backward pass
 template <typename T, int V, int S, bool BACK>
-__global__ void __launch_bounds__(kNormThreads) norm_rotary_kernel(const NormParams p, int lanes)
+__global__ void __launch_bounds__(kNormThreads, BACK || S > 1 ? 4 : 6) norm_rotary_kernel(const NormParams p, int lanes)
 {
     chain_begin();
     __shared__ float reduced[BACK ? kNormThreads * 2 * V : 1];
@@ -156,7 +164,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_kernel(const NormPar
 #pragma unroll
     for (int k = 0; k < S; ++k) {
         at[k] = slot_of<V>(lane + k * lanes, paired, p.rot);
-        has_a[k] = at[k].a + V <= p.d && (lane + k * lanes < paired || at[k].a >= p.rot);
+        has_a[k] = at[k].a + V <= p.d;
         has_b[k] = at[k].b + V <= p.d;
 #pragma unroll
         for (int i = 0; i < V; ++i) wa[k][i] = wb[k][i] = dwa[k][i] = dwb[k][i] = 0.0f;
@@ -171,27 +179,39 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_kernel(const NormPar
         const long long token = on ? item / s.chunks : 0;
         const int h0 = on ? static_cast<int>(item - token * s.chunks) * s.per : 0;
         const int b = static_cast<int>(token / p.N), n = static_cast<int>(token - static_cast<long long>(b) * p.N);
-        Turns<S, V> t;
-        load_turns<V, S>(p, b, n, lane, lanes, paired, t);
         const T *row = static_cast<const T *>(s.x) + b * s.stride[0] + n * s.stride[1];
         const long long flat = token * s.heads * p.d;
-#pragma unroll 2
+        // the next head's row is on its way while one is computed
+        Run<T, V> next_x[S][2], next_g[S][2];
+        const auto fetch = [&](int head) {
+            const bool there = on && head < s.heads && head < h0 + s.per;
+#pragma unroll
+            for (int k = 0; k < S; ++k) {
+                next_x[k][0].load(row + head * s.stride[2] + at[k].a, there && has_a[k]);
+                next_x[k][1].load(row + head * s.stride[2] + at[k].b, there && has_b[k]);
+                if constexpr (BACK) {
+                    const T *dy = static_cast<const T *>(s.dy) + flat + static_cast<long long>(head) * p.d;
+                    next_g[k][0].load(dy + at[k].a, there && has_a[k]);
+                    next_g[k][1].load(dy + at[k].b, there && has_b[k]);
+                }
+            }
+        };
+        fetch(h0);
+        Turns<S, V> t;
+        load_turns<V, S>(p, b, n, lane, lanes, paired, t);
+#pragma unroll 1
         for (int i0 = 0; i0 < s.per; ++i0) {
             const int head = h0 + i0;
             const bool live = on && head < s.heads;
             float xa[S][V], xb[S][V], ga[S][V], gb[S][V], square = 0.0f;
 #pragma unroll
-            for (int k = 0; k < S; ++k) {
+            for (int k = 0; k < S; ++k)
 #pragma unroll
-                for (int i = 0; i < V; ++i) xa[k][i] = xb[k][i] = ga[k][i] = gb[k][i] = 0.0f;
-                if (live && has_a[k]) load_run<T, V>(row + head * s.stride[2] + at[k].a, xa[k]);
-                if (live && has_b[k]) load_run<T, V>(row + head * s.stride[2] + at[k].b, xb[k]);
-                if constexpr (BACK) {
-                    const T *dy = static_cast<const T *>(s.dy) + flat + static_cast<long long>(head) * p.d;
-                    if (live && has_a[k]) load_run<T, V>(dy + at[k].a, ga[k]);
-                    if (live && has_b[k]) load_run<T, V>(dy + at[k].b, gb[k]);
+                for (int i = 0; i < V; ++i) {
+                    xa[k][i] = next_x[k][0].get(i), xb[k][i] = next_x[k][1].get(i);
+                    if constexpr (BACK) ga[k][i] = next_g[k][0].get(i), gb[k][i] = next_g[k][1].get(i);
                 }
-            }
+            fetch(head + 1);
 #pragma unroll
             for (int k = 0; k < S; ++k)
 #pragma unroll
