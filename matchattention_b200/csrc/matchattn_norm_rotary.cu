@@ -105,6 +105,13 @@ struct Turns {
     float cosine[S][V], sine[S][V];
 };
 
+// A group's token and first head.
+struct Place {
+    unsigned token;
+    int b, n, h0;
+    bool on;
+};
+
 // first channel of a slot's two runs; slots below `paired` are rotated
 struct Slot {
     int a, b;
@@ -115,28 +122,53 @@ __device__ __forceinline__ Slot slot_of(int s, int paired, int rot)
     return s < paired ? Slot{s * V, s * V + rot / 2} : Slot{rot + 2 * (s - paired) * V, rot + (2 * (s - paired) + 1) * V};
 }
 
-template <int V, int S>
-__device__ __forceinline__ void load_turns(const NormParams &p, int b, int n, int lane, int lanes, int paired, Turns<S, V> &t)
+__device__ __forceinline__ void turn_of(const NormParams &p, const long long (&pos)[2], int pair, float &cosine, float &sine)
 {
-    long long pos[2] = {0, 0};
-    for (int a = 0; a < p.axes && p.rot > 0; ++a) {
-        const long long i = b * p.pos_item + static_cast<long long>(n) * p.axes + a;
-        pos[a] = p.pos64 ? static_cast<const long long *>(p.positions)[i] : static_cast<const int *>(p.positions)[i];
+    const int per_axis = p.rot / 2 / p.axes;
+    const unsigned long long turn = p.freqs[pair] * static_cast<unsigned long long>(pair >= per_axis ? pos[1] : pos[0]);
+    sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077393e-10f, &sine, &cosine);
+}
+
+// Of the V pairs of a lane's slot each of V / SHARE groups of lanes, which have the same token, forms SHARE.
+template <int V, int SHARE>
+__device__ __forceinline__ void share_turns(const NormParams &p, const long long (&pos)[2], int slot, bool turned, int member, int lanes, Turns<1, V> &t)
+{
+    float cosine[SHARE], sine[SHARE];
+#pragma unroll
+    for (int m = 0; m < SHARE; ++m) {
+        cosine[m] = 1.0f;
+        sine[m] = 0.0f;
+        if (turned) turn_of(p, pos, slot * V + member * SHARE + m, cosine[m], sine[m]);
     }
-    const int per_axis = p.rot / 2 / max(p.axes, 1);
+    const int base = (threadIdx.x & 31) - member * lanes;
 #pragma unroll
-    for (int k = 0; k < S; ++k) {
-        const int s = lane + k * lanes;
+    for (int i = 0; i < V; ++i) {
+        t.cosine[0][i] = __shfl_sync(0xffffffffu, cosine[i % SHARE], base + i / SHARE * lanes);
+        t.sine[0][i] = __shfl_sync(0xffffffffu, sine[i % SHARE], base + i / SHARE * lanes);
+    }
+}
+
+// lane: of its group; member: the group's place among the `spread` groups that take the heads of a token together
+template <int V, int S>
+__device__ __forceinline__ void find_turns(const NormParams &p, const long long (&pos)[2], int lane, int lanes, int member, int spread, int paired,
+                                           Turns<S, V> &t)
+{
+    if (p.rot == 0) return;
+    if constexpr (S == 1 && V > 1) {
+        const bool turned = lane < paired;
+        if (spread >= V) share_turns<V, 1>(p, pos, lane, turned, member, lanes, t);
+        else if (spread * 2 == V) share_turns<V, 2>(p, pos, lane, turned, member, lanes, t);
+        else if (spread * 4 == V) share_turns<V, 4>(p, pos, lane, turned, member, lanes, t);
+        else share_turns<V, V>(p, pos, lane, turned, member, lanes, t);
+    } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            t.cosine[k][i] = 1.0f;
-            t.sine[k][i] = 0.0f;
-            if (s < paired) {
-                const int pair = s * V + i;
-                const unsigned long long turn = p.freqs[pair] * static_cast<unsigned long long>(pair >= per_axis ? pos[1] : pos[0]);
-                sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077393e-10f, &t.sine[k][i], &t.cosine[k][i]);
+        for (int k = 0; k < S; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                t.cosine[k][i] = 1.0f;
+                t.sine[k][i] = 0.0f;
+                if (lane + k * lanes < paired) turn_of(p, pos, (lane + k * lanes) * V + i, t.cosine[k][i], t.sine[k][i]);
             }
-        }
     }
 }
 
@@ -148,16 +180,17 @@ __device__ __forceinline__ float group_sum(float v, int lanes)
 
 // T: element, V: channels per run, S: slots per lane, BACK: the backward pass
 template <typename T, int V, int S, bool BACK>
-__global__ void __launch_bounds__(kNormThreads, BACK || S > 1 ? 4 : 6) norm_rotary_kernel(const NormParams p, int lanes)
+__global__ void __launch_bounds__(kNormThreads, BACK || S > 1 ? 4 : 6) norm_rotary_kernel(const NormParams p, int lanes, int spread)
 {
     chain_begin();
     __shared__ float reduced[BACK ? kNormThreads * 2 * V : 1];
     const int second = blockIdx.x >= p.side[0].blocks;
     const NormSide &s = p.side[second];
     const int block = blockIdx.x - (second ? p.side[0].blocks : 0);
-    const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = kNormThreads / lanes;
+    const int lane = threadIdx.x & (lanes - 1), member = threadIdx.x / lanes & (spread - 1);
+    const int group = threadIdx.x / (lanes * spread), groups = kNormThreads / (lanes * spread);
     const int paired = p.rot / (2 * V);
-    const long long items = static_cast<long long>(p.B) * p.N * s.chunks;
+    const unsigned items = static_cast<unsigned>(p.B) * p.N * s.chunks;
     float wa[S][V], wb[S][V], dwa[S][V], dwb[S][V];
     bool has_a[S], has_b[S];
     Slot at[S];
@@ -171,38 +204,55 @@ __global__ void __launch_bounds__(kNormThreads, BACK || S > 1 ? 4 : 6) norm_rota
         if (has_a[k]) load_weight<T, V>(p, s.w, at[k].a, wa[k]);
         if (has_b[k]) load_weight<T, V>(p, s.w, at[k].b, wb[k]);
     }
-    // every group of a warp makes the same number of rounds (their sums are taken by the whole warp)
-    const long long step = static_cast<long long>(s.blocks) * groups;
-    for (long long first = static_cast<long long>(block) * groups; first < items; first += step) {
-        const long long item = first + group;
-        const bool on = item < items;
-        const long long token = on ? item / s.chunks : 0;
-        const int h0 = on ? static_cast<int>(item - token * s.chunks) * s.per : 0;
-        const int b = static_cast<int>(token / p.N), n = static_cast<int>(token - static_cast<long long>(b) * p.N);
-        const T *row = static_cast<const T *>(s.x) + b * s.stride[0] + n * s.stride[1];
-        const long long flat = token * s.heads * p.d;
-        // the next head's row is on its way while one is computed
-        Run<T, V> next_x[S][2], next_g[S][2];
-        const auto fetch = [&](int head) {
-            const bool there = on && head < s.heads && head < h0 + s.per;
+    // the next row, and the next token's position, are on their way while a row is computed
+    Run<T, V> next_x[S][2], next_g[S][2];
+    long long next_pos[2] = {0, 0};
+    const auto place_of = [&](unsigned item) {
+        Place at;
+        at.on = item < items;
+        at.token = at.on ? item / s.chunks : 0;
+        at.h0 = (at.on ? static_cast<int>(item - at.token * s.chunks) * s.per * spread : 0) + member;
+        at.b = static_cast<int>(at.token / p.N);
+        at.n = static_cast<int>(at.token) - at.b * p.N;
+        return at;
+    };
+    const auto fetch = [&](const Place &to, int i0) {
+        const int head = to.h0 + i0 * spread;
+        const bool there = to.on && head < s.heads;
+        const T *x = static_cast<const T *>(s.x) + to.b * s.stride[0] + to.n * s.stride[1] + head * s.stride[2];
+        const T *dy = static_cast<const T *>(s.dy) + (static_cast<long long>(to.token) * s.heads + head) * p.d;
 #pragma unroll
-            for (int k = 0; k < S; ++k) {
-                next_x[k][0].load(row + head * s.stride[2] + at[k].a, there && has_a[k]);
-                next_x[k][1].load(row + head * s.stride[2] + at[k].b, there && has_b[k]);
-                if constexpr (BACK) {
-                    const T *dy = static_cast<const T *>(s.dy) + flat + static_cast<long long>(head) * p.d;
-                    next_g[k][0].load(dy + at[k].a, there && has_a[k]);
-                    next_g[k][1].load(dy + at[k].b, there && has_b[k]);
-                }
+        for (int k = 0; k < S; ++k) {
+            next_x[k][0].load(x + at[k].a, there && has_a[k]);
+            next_x[k][1].load(x + at[k].b, there && has_b[k]);
+            if constexpr (BACK) {
+                next_g[k][0].load(dy + at[k].a, there && has_a[k]);
+                next_g[k][1].load(dy + at[k].b, there && has_b[k]);
             }
-        };
-        fetch(h0);
+        }
+        if (i0 == 0 && p.rot > 0) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+                if (a < p.axes) {
+                    const long long i = to.b * p.pos_item + static_cast<long long>(to.n) * p.axes + a;
+                    next_pos[a] = p.pos64 ? static_cast<const long long *>(p.positions)[i] : static_cast<const int *>(p.positions)[i];
+                }
+        }
+    };
+    // every group of a warp makes the same number of rounds (their sums are taken by the whole warp)
+    const unsigned step = static_cast<unsigned>(s.blocks) * groups;
+    Place next = place_of(static_cast<unsigned>(block) * groups + group);
+    fetch(next, 0);
+    for (unsigned first = static_cast<unsigned>(block) * groups; first < items; first += step) {
+        const Place now = next;
+        const long long flat = static_cast<long long>(now.token) * s.heads * p.d;
         Turns<S, V> t;
-        load_turns<V, S>(p, b, n, lane, lanes, paired, t);
+        find_turns<V, S>(p, next_pos, lane, lanes, member, spread, paired, t);
+        next = place_of(first + step + group);
 #pragma unroll 1
         for (int i0 = 0; i0 < s.per; ++i0) {
-            const int head = h0 + i0;
-            const bool live = on && head < s.heads;
+            const int head = now.h0 + i0 * spread;
+            const bool live = now.on && head < s.heads;
             float xa[S][V], xb[S][V], ga[S][V], gb[S][V], square = 0.0f;
 #pragma unroll
             for (int k = 0; k < S; ++k)
@@ -211,7 +261,8 @@ __global__ void __launch_bounds__(kNormThreads, BACK || S > 1 ? 4 : 6) norm_rota
                     xa[k][i] = next_x[k][0].get(i), xb[k][i] = next_x[k][1].get(i);
                     if constexpr (BACK) ga[k][i] = next_g[k][0].get(i), gb[k][i] = next_g[k][1].get(i);
                 }
-            fetch(head + 1);
+            if (i0 + 1 < s.per) fetch(now, i0 + 1);
+            else fetch(next, 0);
 #pragma unroll
             for (int k = 0; k < S; ++k)
 #pragma unroll
@@ -280,7 +331,7 @@ __global__ void __launch_bounds__(kNormThreads, BACK || S > 1 ? 4 : 6) norm_rota
                 const Slot c = slot_of<V>(l + k * lanes, paired, p.rot);
                 const int channel = i < V ? c.a + i : c.b + i - V;
                 float sum = 0.0f;
-                for (int g = 0; g < groups; ++g) sum += reduced[i * kNormThreads + g * lanes + l];
+                for (int g = 0; g < kNormThreads / lanes; ++g) sum += reduced[i * kNormThreads + g * lanes + l];
                 if (channel < p.d) s.partial[static_cast<long long>(block) * p.d + channel] = sum;
             }
         }
@@ -311,19 +362,19 @@ __global__ void __launch_bounds__(1024) norm_weight_kernel(const NormParams p)
     }
 }
 
-// The blocks of one side, and how its heads are cut.  Heads in turn share the angles; a small call spreads them instead, so
-// that the chip fills.  Backward blocks are few enough to keep the sums over them short.
-void lay_out(NormSide &s, long long tokens, int groups, bool back, long long wanted)
+// The blocks of one side, and how its heads are cut: `spread` at a time, `per` times in turn.  Heads in turn share the angles; a
+// small call spreads them instead, so that the chip fills.  No more than `most` blocks, each of which takes items in turn.
+void lay_out(NormSide &s, long long tokens, int groups, int spread, long long wanted, long long most)
 {
-    s.per = s.heads < kNormHeads ? s.heads : kNormHeads;
-    while (s.per > 1 && tokens * ((s.heads + s.per - 1) / s.per) < wanted * groups) s.per = (s.per + 1) / 2;
-    s.chunks = (s.heads + s.per - 1) / s.per;
+    const int turns = (s.heads + spread - 1) / spread;
+    s.per = turns < kNormHeads ? turns : kNormHeads;
+    while (s.per > 1 && tokens * ((turns + s.per - 1) / s.per) < wanted * groups) s.per = (s.per + 1) / 2;
+    s.chunks = (turns + s.per - 1) / s.per;
     const long long items = tokens * s.chunks, blocks = (items + groups - 1) / groups;
-    const long long most = back ? wanted : 1LL << 30;
     s.blocks = static_cast<int>(blocks < most ? blocks : most);
 }
 
-constexpr int kNormBackBlocks = 4;       // blocks per SM and side of the backward kernel at most
+constexpr int kNormBackBlocks = 4, kNormForwardBlocks = 6;       // blocks per SM and side at most
 
 template <typename T, int V, int S>
 cudaError_t run_norm_slots(NormParams &p, bool back, cudaStream_t stream)
@@ -331,14 +382,19 @@ cudaError_t run_norm_slots(NormParams &p, bool back, cudaStream_t stream)
     const int slots = ((p.d + V - 1) / V + 1) / 2;
     int lanes = 1;
     while (lanes < 32 && lanes * S < slots) lanes *= 2;
-    const int groups = kNormThreads / lanes;
+    // as many heads side by side as share a warp, up to one per pair of a lane: they read and write one run of memory, and each
+    // forms its share of the token's angles
+    int spread = 1;
+    while (S == 1 && V > 1 && spread < V && spread * lanes < 32 && spread < p.side[0].heads) spread *= 2;
+    const int groups = kNormThreads / (lanes * spread);
     int blocks = 0;
     for (NormSide &s : p.side) {
-        if (s.heads > 0) lay_out(s, static_cast<long long>(p.B) * p.N, groups, back, 1LL * sm_count() * kNormBackBlocks);
+        if (s.heads > 0) lay_out(s, static_cast<long long>(p.B) * p.N, groups, spread, 1LL * sm_count() * kNormBackBlocks,
+                                  1LL * sm_count() * (back ? kNormBackBlocks : kNormForwardBlocks));
         blocks += s.blocks;
     }
-    const cudaError_t err = back ? launch_chained(norm_rotary_kernel<T, V, S, true>, dim3(blocks), kNormThreads, 0, stream, p, lanes)
-                                 : launch_chained(norm_rotary_kernel<T, V, S, false>, dim3(blocks), kNormThreads, 0, stream, p, lanes);
+    const cudaError_t err = back ? launch_chained(norm_rotary_kernel<T, V, S, true>, dim3(blocks), kNormThreads, 0, stream, p, lanes, spread)
+                                 : launch_chained(norm_rotary_kernel<T, V, S, false>, dim3(blocks), kNormThreads, 0, stream, p, lanes, spread);
     if (err != cudaSuccess || (p.side[0].partial == nullptr && p.side[1].partial == nullptr)) return err;
     return launch_chained(norm_weight_kernel<T>, dim3((p.d + 31) / 32, 2), dim3(32, 32), 0, stream, p);
 }
