@@ -38,9 +38,6 @@ struct BackShared {
     int broken, by_hand[2], odd[2][3];
 };
 
-__device__ __forceinline__ float element(const float4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
-__device__ __forceinline__ int element(const int4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
-
 // KEYS: the pass for dK and dV
 template <typename T, int DP, bool CAP, GlobalBias BIAS, bool KEYS>
 __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const GlobalParams p, const __grid_constant__ GlobalMaps maps)
@@ -173,7 +170,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         const int w = warp >> 2, f = f0 + (tid & 127);                          // half of the moving rows; the fixed row
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
         const uint32_t my_scores = scores + lanes + w * 64, my_slopes = slopes + lanes + w * 64;
-        const float factor = p.scale * kLog2e, inner = CAP ? 2.0f * factor / p.cap : 0.0f, outer = p.cap * kLog2e;
+        const float factor = p.scale * kLog2e, inverse_cap = CAP ? p.scale / p.cap : 0.0f, outer = p.cap * kLog2e;
         // dS is held times 2^(lift - kLift), the sums of dS times 2^-lift
         int lift = 0;
         if (HALF) {
@@ -238,6 +235,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
 #pragma unroll
                 for (int c = 0; c < 64; c += 32) {
                     uint32_t packed[16];
+                    if (CAP) tanh_all<32>(prob + c, inverse_cap);
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         const int four = (c + e) / 4;
@@ -255,9 +253,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                             if (BIAS == kSequenceBias) level[u] = fmaf(slope, fabsf(from - static_cast<float>(at)), level[u]);
                             float slant = 1.0f;
                             if (CAP) {
-                                const float tanh_x = tanh_of(prob[at] * inner);
-                                slant = fmaf(-tanh_x, tanh_x, 1.0f);
-                                value[u] = fmaf(outer, tanh_x, -level[u]);
+                                slant = fmaf(-prob[at], prob[at], 1.0f);
+                                value[u] = fmaf(outer, prob[at], -level[u]);
                             } else {
                                 value[u] = fmaf(prob[at], factor, -level[u]);
                             }
@@ -280,7 +277,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 if (now == kPartial) {
                     const int s = i % STAGES;
                     good = barrier_wait(&sh.full[s], (i / STAGES) & 1, &sh.broken);
-                    if (good && (KEYS || w == 0) && row_tainted<T, DP>(sh.moving[s][w], tid & 127)) *static_cast<volatile int *>(&sh.odd[w][looks % 3]) = 1;
+                    if (good && (KEYS || w == 0) && (row_tainted<T, DP>(sh.moving[s][w], tid & 127, 0) || row_tainted<T, DP>(sh.moving[s][w], tid & 127, 1))) *static_cast<volatile int *>(&sh.odd[w][looks % 3]) = 1;
                     // (the slot after this one was last read two looks ago)
                     if ((tid & 127) == 0) *static_cast<volatile int *>(&sh.odd[w][(looks + 1) % 3]) = 0;
                     tmem_before();

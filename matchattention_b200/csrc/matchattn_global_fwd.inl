@@ -1,13 +1,14 @@
 // Dense attention, forward, 16-bit types of up to 128 channels, on the matrix units.  Included once per type with MATCHATTN_T
 // defined.
 //
-// A block owns 256 queries of a head as two tiles of 128 (or one tile, when the call has too few for the chip), a thread a query.
-// Warps 0-3 and 4-7 take the softmax of one tile each, warp 8 copies tiles of K and V into a ring of buffers (tensor memory
-// accelerator), one thread of warp 9 issues the products: S = Q K^T into tensor memory, and O += P V with P from tensor memory, where it
-// overwrites the scores.  While one tile's threads take exponentials the matrix unit works on the other's.
+// A block owns 256 queries of a head as two tiles of 128 (or one tile, when the call has too few for the chip).  Warps 0-7 and 8-15
+// take the softmax of one tile each, a thread 64 of the 128 scores of a query; warp 16 copies tiles of K and V into a ring of
+// buffers (tensor memory accelerator); one thread of warp 17 issues the products: S = Q K^T into tensor memory, and O += P V with P from
+// tensor memory, where it overwrites the scores.  While one tile's threads take exponentials the matrix unit works on the other's.
 //
-// The softmax keeps a reference per row, not the running maximum itself: O and the sum are scaled down only when a score exceeds
-// the reference by 2^8, so probabilities stay below 2^8 and O in tensor memory is hardly ever touched between products.
+// The softmax keeps a reference per row, not the running maximum itself: probabilities are taken with the reference as it stands,
+// and O, the sum and the probabilities only change to a new one when a score exceeds it by 2^8.  They stay below 2^8, O in
+// tensor memory is hardly ever touched between products, and nothing waits for a maximum.
 // P is rounded to the type of V (a half step of it, relative, as torch rounds a softmax's result); scores, reference, sum and O are float32.
 //
 // A probability that the mask makes zero meets V all the same in the product, and 0 * NaN is NaN: where a tile is partly
@@ -17,7 +18,7 @@
 namespace matchattn {
 namespace {
 
-constexpr int kForwardThreads = 320;
+constexpr int kForwardThreads = 576;
 constexpr float kSlack = 8.0f;           // log2 of what a probability may exceed one by
 
 template <int DP>
@@ -25,9 +26,10 @@ struct ForwardShared {
     static constexpr int kStages = DP == 128 ? 4 : 6;
     uint8_t q[2][kTileBytes<DP>];
     uint8_t kv[kStages][kTileBytes<DP>];
-    float2 place[8][kTile];              // per softmax warp: columns and rows of the tile's keys
-    int docs[8][kTile];
-    uint64_t q_full, kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], o_full[2];
+    float4 across[16][16], down[16][16];           // per softmax warp, its 64 keys: columns and rows on the map
+    int4 docs[16][16];
+    float high[2][2][2][kTile];                    // by turns: tile, half, row
+    uint64_t agreed[2][4], q_full, kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], o_full[2];
     uint32_t tmem;
     uint64_t looked[2];                  // a warpgroup has looked through a tile of V
     int broken, by_hand[2], odd[2][3];
@@ -66,22 +68,23 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
         }
         for (int w = 0; w < 2; ++w) {
             barrier_init(&sh.s_full[w], 1);
-            barrier_init(&sh.p_full[w], kTile);
+            barrier_init(&sh.p_full[w], 2 * kTile);
+            for (int i = 0; i < 4; ++i) barrier_init(&sh.agreed[w][i], 2);
             barrier_init(&sh.o_full[w], 1);
-            barrier_init(&sh.looked[w], kTile);
+            barrier_init(&sh.looked[w], 2 * kTile);
             for (int i = 0; i < 3; ++i) sh.odd[w][i] = 0;
         }
         sh.broken = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 9) tmem_take(&sh.tmem);
+    if (warp == 17) tmem_take(&sh.tmem);
     tmem_before();
     __syncthreads();
     tmem_after();
     const uint32_t tmem = sh.tmem;
 
-    if (warp == 8) {
+    if (warp == 16) {
         // ---- copies: Q, then K and V of every tile that one of the two query tiles sees
         if (elected()) {
             barrier_expect(&sh.q_full, tiles * kTileBytes<DP>);
@@ -105,7 +108,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         // ---- products
         if (elected()) {
             const int steps = (p.d + 15) / 16;
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                 if (!*static_cast<volatile int *>(&sh.by_hand[w])) {
                     const uint32_t v = kv_at + last_v * kTileBytes<DP>, out = tmem + 256 + w * kTile, prob = tmem + w * kTile;
 #pragma unroll
-                    for (int s = 0; s < kTile / 16; ++s) product_ts(out, prob + 8 * s, by_rows(v, s), value_kind, used[w] > 1 || s > 0);
+                    for (int s = 0; s < kTile / 16; ++s) product_ts(out, prob + 8 * s + (s >= 4 ? 32 : 0), by_rows(v, s), value_kind, used[w] > 1 || s > 0);
                 }
             };
             for (int t = t_begin; t < t_end && good; ++t) {
@@ -164,13 +167,13 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
             }
         }
         __syncwarp();
-    } else if (warp < 8) {
+    } else {
         // ---- softmax
-        const int w = warp >> 2, row = tid & 127, n = n0 + w * kTile + row;
+        const int w = warp >> 3, half = warp >> 2 & 1, row = tid & 127, n = n0 + w * kTile + row;
         const uint32_t mine = tmem + (static_cast<uint32_t>(warp & 3) << 21);        // lanes 32 (warp mod 4) on
-        const uint32_t scores = mine + w * kTile, out = mine + 256 + w * kTile;
+        const uint32_t scores = mine + w * kTile + half * 64, out = mine + 256 + w * kTile;
         const float factor = p.scale * kLog2e;
-        const float inner = CAP ? 2.0f * factor / p.cap : 0.0f, outer = p.cap * kLog2e;
+        const float inverse_cap = CAP ? p.scale / p.cap : 0.0f, outer = p.cap * kLog2e;
         const int doc = p.q_docs && n < p.N ? p.q_docs[static_cast<long long>(b) * p.N + n] : -1;
         const int limit = p.q_docs && doc < 0 ? 0 : key_limit(mask, n);
         const float slope = BIAS != kNoBias ? p.slopes[head] * kLog2e : 0.0f;
@@ -184,145 +187,151 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                 if (other != kHidden) buffers += 2;
                 continue;
             }
-            const int j0 = t * kTile;
-            if (BIAS == kMapBias) {
+            const int j0 = t * kTile + half * 64;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sh.place[warp][lane + 32 * i] = map_place(j0 + lane + 32 * i, p.width);
-            }
-            if (p.q_docs && now == kPartial) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int j = j0 + lane + 32 * i;
-                    sh.docs[warp][lane + 32 * i] = j < p.M ? p.k_docs[static_cast<long long>(b) * p.M + j] : -1;
+            for (int e = lane; e < 64; e += 32) {
+                if (BIAS == kMapBias) {
+                    const float2 at = map_place(j0 + e, p.width);
+                    reinterpret_cast<float *>(sh.across[warp])[e] = at.x;
+                    reinterpret_cast<float *>(sh.down[warp])[e] = at.y;
                 }
+                if (p.q_docs && now == kPartial)
+                    reinterpret_cast<int *>(sh.docs[warp])[e] = j0 + e < p.M ? p.k_docs[static_cast<long long>(b) * p.M + j0 + e] : -1;
             }
             __syncwarp();
             good = good && barrier_wait(&sh.s_full[w], used & 1, &sh.broken);
             if (!good) break;
             tmem_after();
-            // First pass: the final scores' maximum.  Scores that differ from the product's are put back in its place; both
-            // passes go by 32 columns, because 128 of them and the rest do not fit the 168 registers that ten warps have.
-            const bool changed = GENERAL || now == kPartial;
-            float high = -INFINITY;
-            uint32_t raw[2][32];
-            tmem_load32(scores, raw[0]);
+            // Probabilities of the thread's 64 scores for a reference, in registers; the largest score in units of log2.
+            uint32_t packed[32];
+            float part[2];
+            const auto probabilities = [&](float base) {
+                float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                part[0] = part[1] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < kTile; c += 32) {
-                float *x = reinterpret_cast<float *>(raw[c / 32 % 2]);
-                tmem_loaded32(raw[c / 32 % 2]);
-                if (c + 32 < kTile) tmem_load32(scores + c + 32, raw[(c / 32 + 1) % 2]);
-                if constexpr (GENERAL) {
+                for (int c = 0; c < 64; c += 32) {
+                    uint32_t raw[32];
+                    float *x = reinterpret_cast<float *>(raw);
+                    tmem_load32(scores + c, raw);
+                    tmem_loaded32(raw);
+                    if constexpr (CAP) tanh_all<32>(x, inverse_cap);
+                    if constexpr (GENERAL) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = CAP ? outer * tanh_of(x[i] * inner) : x[i] * factor;
+                        for (int i = 0; i < 32; ++i) x[i] *= CAP ? outer : factor;
+                    }
                     if constexpr (BIAS == kMapBias) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float4 two = *reinterpret_cast<const float4 *>(&sh.place[warp][c + i]);
-                            x[i] = fmaf(-slope, fabsf(here.x - two.x) + fabsf(here.y - two.y), x[i]);
-                            x[i + 1] = fmaf(-slope, fabsf(here.x - two.z) + fabsf(here.y - two.w), x[i + 1]);
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 across = sh.across[warp][(c + i) / 4], down = sh.down[warp][(c + i) / 4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u)
+                                x[i + u] = fmaf(-slope, fabsf(here.x - element(across, u)) + fabsf(here.y - element(down, u)), x[i + u]);
                         }
                     } else if constexpr (BIAS == kSequenceBias) {
                         const float from = here.y - static_cast<float>(j0 + c);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) x[i] = fmaf(-slope, fabsf(from - static_cast<float>(i)), x[i]);
                     }
-                }
-                if (now == kPartial) {
-                    if (p.q_docs) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const int4 id = *reinterpret_cast<const int4 *>(&sh.docs[warp][c + i]);
-                            if (j0 + c + i >= limit || id.x != doc) x[i] = -INFINITY;
-                            if (j0 + c + i + 1 >= limit || id.y != doc) x[i + 1] = -INFINITY;
-                            if (j0 + c + i + 2 >= limit || id.z != doc) x[i + 2] = -INFINITY;
-                            if (j0 + c + i + 3 >= limit || id.w != doc) x[i + 3] = -INFINITY;
-                        }
-                    } else {
+                    if (now == kPartial) {
                         const int left = limit - j0 - c;
+                        if (p.q_docs) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i >= left) x[i] = -INFINITY;
+                            for (int i = 0; i < 32; i += 4) {
+                                const int4 id = sh.docs[warp][(c + i) / 4];
+#pragma unroll
+                                for (int u = 0; u < 4; ++u)
+                                    if (i + u >= left || element(id, u) != doc) x[i + u] = -INFINITY;
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (i >= left) x[i] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        high[i % 4] = fmaxf(high[i % 4], x[i]);
+                        high[i % 4 + 1] = fmaxf(high[i % 4 + 1], x[i + 1]);
+                        const float e0 = exp2_fast(GENERAL ? x[i] - base : fmaf(x[i], factor, -base));
+                        const float e1 = exp2_fast(GENERAL ? x[i + 1] - base : fmaf(x[i + 1], factor, -base));
+                        part[0] += e0;
+                        part[1] += e1;
+                        packed[(c + i) / 2] = pack_two<T>(e0, e1);
                     }
                 }
-                if (changed) tmem_store32(scores + c, raw[c / 32 % 2]);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) high = fmaxf(high, x[i]);
-            }
-            if (changed) tmem_stored();
-            if constexpr (!GENERAL) high *= factor;
-            if (used == 0) {
-                ref = high;
-            } else {
+                const float most = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+                return GENERAL ? most : most * factor;
+            };
+            float high = probabilities(ref == -INFINITY ? 0.0f : ref);
+            // the two halves of a row agree on its largest score
+            sh.high[used & 1][w][half][row] = high;
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&sh.agreed[w][warp & 3]);
+            good = barrier_wait(&sh.agreed[w][warp & 3], used & 1, &sh.broken);
+            high = fmaxf(high, sh.high[used & 1][w][half ^ 1][row]);
+            const bool grown = high > ref + kSlack;
+            if (__any_sync(0xffffffffu, grown)) {
                 // (a row that has seen nothing so far has zeros in O and sum: any factor does)
-                const bool grown = high > ref + kSlack;
-                if (__any_sync(0xffffffffu, grown)) {
-                    const float shrink = grown ? (ref == -INFINITY ? 0.0f : exp2_fast(ref - high)) : 1.0f;
-                    ref = grown ? high : ref;
-                    sum *= shrink;
+                const float shrink = grown ? (ref == -INFINITY ? 0.0f : exp2_fast(ref - high)) : 1.0f;
+                ref = grown ? high : ref;
+                sum *= shrink;
+                if (used > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < DP; c += 32) {
-                        tmem_load32(out + c, raw[0]);
-                        tmem_loaded32(raw[0]);
+                    for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+                        uint32_t o[32];
+                        tmem_load32(out + c, o);
+                        tmem_loaded32(o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) raw[0][i] = __float_as_uint(__uint_as_float(raw[0][i]) * shrink);
-                        tmem_store32(out + c, raw[0]);
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+                        tmem_store32(out + c, o);
                     }
                 }
+                probabilities(ref == -INFINITY ? 0.0f : ref);
             }
-            const float base = ref == -INFINITY ? 0.0f : ref;
-            float part[2] = {0.0f, 0.0f};
-            tmem_load32(scores, raw[0]);
-#pragma unroll
-            for (int c = 0; c < kTile; c += 32) {
-                const float *x = reinterpret_cast<const float *>(raw[c / 32 % 2]);
-                tmem_loaded32(raw[c / 32 % 2]);
-                if (c + 32 < kTile) tmem_load32(scores + c + 32, raw[(c / 32 + 1) % 2]);
-                uint32_t packed[16];
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float e0 = exp2_fast(GENERAL ? x[i] - base : fmaf(x[i], factor, -base));
-                    const float e1 = exp2_fast(GENERAL ? x[i + 1] - base : fmaf(x[i + 1], factor, -base));
-                    part[0] += e0;
-                    part[1] += e1;
-                    packed[i / 2] = pack_two<T>(e0, e1);
-                }
-                tmem_store16(scores + c / 2, packed);
-            }
+            tmem_store32(scores, packed);
             sum += part[0] + part[1];
             tmem_stored();
             bool hand = false;
             if (now == kPartial) {
                 const int s = (buffers + 1) % STAGES;
                 good = barrier_wait(&sh.kv_full[s], ((buffers + 1) / STAGES) & 1, &sh.broken);
-                if (good && row_tainted<T, DP>(sh.kv[s], row)) *static_cast<volatile int *>(&sh.odd[w][looks % 3]) = 1;
+                if (good && row_tainted<T, DP>(sh.kv[s], row, half)) *static_cast<volatile int *>(&sh.odd[w][looks % 3]) = 1;
                 // (the slot after this one was last read two looks ago)
-                if (row == 0) *static_cast<volatile int *>(&sh.odd[w][(looks + 1) % 3]) = 0;
+                if (row == 0 && half == 0) *static_cast<volatile int *>(&sh.odd[w][(looks + 1) % 3]) = 0;
+                tmem_before();
                 barrier_arrive(&sh.looked[w]);
                 good = good && barrier_wait(&sh.looked[w], looks & 1, &sh.broken);
+                tmem_after();
                 hand = __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[w][looks % 3]) != 0);
                 ++looks;
-                if (hand) add_rows<T, DP>(out, scores, 0, sh.kv[s], used > 0);
+                if (hand && half == 0) add_rows<T, DP>(out, scores, 32, sh.kv[s], used > 0);
             }
-            if (row == 0) sh.by_hand[w] = hand;
+            if (row == 0 && half == 0) sh.by_hand[w] = hand;
             tmem_before();
             barrier_arrive(&sh.p_full[w]);
             ++used;
             buffers += 2;
         }
+        // the sum of the row's halves
+        sh.high[used & 1][w][half][row] = sum;
+        __syncwarp();
+        if (lane == 0) barrier_arrive(&sh.agreed[w][warp & 3]);
+        good = good && barrier_wait(&sh.agreed[w][warp & 3], used & 1, &sh.broken);
+        sum += sh.high[used & 1][w][half ^ 1][row];
         if (good) good = barrier_wait(&sh.o_full[w], 0, &sh.broken);
         tmem_after();
         const bool empty = sum == 0.0f;
         const float inv = !good ? NAN : empty ? 0.0f : 1.0f / sum;
-        if (n0 + w * kTile < p.N && w < tiles) {          // a whole warpgroup
+        if (n0 + w * kTile < p.N && w < tiles) {          // whole warps
             const long long line = (static_cast<long long>(b) * p.h + head) * p.N + n;
             const long long part = static_cast<long long>(split) * p.B * p.h * p.N + line;
             const float lse = ref + log2f(sum);
-            if (n < p.N) {
+            if (n < p.N && half == 0) {
                 if (p.splits > 1) p.part_lse[part] = empty ? -INFINITY : lse;
                 else if (p.lse) p.lse[line] = empty ? INFINITY : lse;
             }
 #pragma unroll 1
-            for (int c = 0; c < DP && c < p.d; c += 32) {
+            for (int c = half * 32; c < DP && c < p.d; c += 64) {
                 uint32_t o[32];
                 if (used > 0) {
                     tmem_load32(out + c, o);
@@ -359,7 +368,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
     }
     tmem_before();
     __syncthreads();
-    if (warp == 9) tmem_give(tmem);
+    if (warp == 17) tmem_give(tmem);
 }
 
 template <typename T, int DP, bool CAP, GlobalBias BIAS>

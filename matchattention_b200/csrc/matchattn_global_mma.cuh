@@ -191,6 +191,12 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t *x)
                  : MA_R8(x, 0), MA_R8(x, 8), MA_R8(x, 16), MA_R8(x, 24)
                  : "r"(at));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t *x)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : MA_R8(x, 0), MA_R8(x, 8)
+                 : "r"(at));
+}
 __device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t *x)
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : MA_R8(x, 0) : "r"(at));
@@ -227,6 +233,7 @@ __device__ __forceinline__ void tmem_loaded32(uint32_t *x)
 {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : MA_P8(x, 0), MA_P8(x, 8), MA_P8(x, 16), MA_P8(x, 24)::"memory");
 }
+__device__ __forceinline__ void tmem_loaded16(uint32_t *x) { asm volatile("tcgen05.wait::ld.sync.aligned;" : MA_P8(x, 0), MA_P8(x, 8)::"memory"); }
 __device__ __forceinline__ void tmem_loaded8(uint32_t *x) { asm volatile("tcgen05.wait::ld.sync.aligned;" : MA_P8(x, 0)::"memory"); }
 __device__ __forceinline__ void tmem_loaded1(uint32_t &x) { asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x)::"memory"); }
 #undef MA_P8
@@ -242,6 +249,38 @@ __device__ __forceinline__ float exp2_fast(float x)
 
 // tanh from one exponential, 1 - 2 / (e^2y + 1), given 2 y log2(e): off by a few 2^-24, absolutely
 __device__ __forceinline__ float tanh_of(float two_y_log2e) { return 1.0f - __fdividef(2.0f, exp2_fast(two_y_log2e) + 1.0f); }
+
+// tanh(y) = y P(y^2) for |y| <= 0.625: P of degree 5 with the smallest relative error there, 4e-9 (fitted by reweighted least squares);
+// evaluated in float32 it is off by 1.8 * 2^-24, relatively
+constexpr float kSmallTanh = 0.625f;
+__device__ __forceinline__ float tanh_small(float y)
+{
+    const float u = y * y;
+    float r = fmaf(u, -5.659989081e-3f, 2.059098892e-2f);
+    r = fmaf(u, r, -5.372106656e-2f);
+    r = fmaf(u, r, 1.333112717e-1f);
+    r = fmaf(u, r, -3.333325982e-1f);
+    return y * fmaf(u, r, 1.0f);
+}
+
+// x[i] = tanh(x[i] * inverse_cap).  Scores are mostly well below their cap: where all of a warp's are, the polynomial leaves the two
+// special-function instructions of the other form out, which bound the kernels (16 a clock on an SM).
+template <int N>
+__device__ __forceinline__ void tanh_all(float *x, float inverse_cap)
+{
+    float big[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) big[i % 4] = fmaxf(big[i % 4], fabsf(x[i]));
+    const float most = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+    if (__all_sync(0xffffffffu, most * inverse_cap <= kSmallTanh)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = tanh_small(x[i] * inverse_cap);
+    } else {
+        const float inner = 2.0f * kLog2e * inverse_cap;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = tanh_of(x[i] * inner);
+    }
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack_two(float low, float high)
@@ -277,15 +316,19 @@ __device__ __forceinline__ bool tainted(uint32_t acc)
     return a != a || b != b;
 }
 
-// Whether row `row` of a tile holds an infinite or NaN value.
+__device__ __forceinline__ float element(const float4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+__device__ __forceinline__ int element(const int4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
+// Whether a half (of the 16-byte pieces of each 64 channels) of row `row` of a tile holds an infinite or NaN value.
 template <typename T, int DP>
-__device__ __forceinline__ bool row_tainted(const uint8_t *tile, int row)
+__device__ __forceinline__ bool row_tainted(const uint8_t *tile, int row, int part)
 {
     uint32_t acc = 0;
 #pragma unroll
     for (int half = 0; half < DP / 64; ++half)
 #pragma unroll
-        for (int piece = 0; piece < 8; ++piece) {
+        for (int i = 0; i < 4; ++i) {
+            const int piece = 4 * part + i;
             const uint4 x = *reinterpret_cast<const uint4 *>(tile + half * kHalfBytes + row * 128 + ((piece ^ (row & 7)) << 4));
             acc = taint<T>(x.x, taint<T>(x.y, taint<T>(x.z, taint<T>(x.w, acc))));
         }
