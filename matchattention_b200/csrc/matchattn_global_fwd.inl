@@ -207,7 +207,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
             float part[2];
             const auto probabilities = [&](float base) {
                 float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                part[0] = part[1] = 0.0f;
+                Pair total(0.0f, 0.0f);
+                const Pair by(GENERAL ? 1.0f : factor, GENERAL ? 1.0f : factor), less(-base, -base);
 #pragma unroll
                 for (int c = 0; c < 64; c += 32) {
                     uint32_t raw[32];
@@ -252,13 +253,16 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                     for (int i = 0; i < 32; i += 2) {
                         high[i % 4] = fmaxf(high[i % 4], x[i]);
                         high[i % 4 + 1] = fmaxf(high[i % 4 + 1], x[i + 1]);
-                        const float e0 = exp2_fast(GENERAL ? x[i] - base : fmaf(x[i], factor, -base));
-                        const float e1 = exp2_fast(GENERAL ? x[i + 1] - base : fmaf(x[i + 1], factor, -base));
-                        part[0] += e0;
-                        part[1] += e1;
+                        const Pair at(x[i], x[i + 1]);
+                        float e0, e1;
+                        (GENERAL ? pair_add(at, less) : pair_fma(at, by, less)).get(e0, e1);
+                        e0 = exp2_fast(e0);
+                        e1 = exp2_fast(e1);
+                        total = pair_add(total, Pair(e0, e1));
                         packed[(c + i) / 2] = pack_two<T>(e0, e1);
                     }
                 }
+                total.get(part[0], part[1]);
                 const float most = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
                 return GENERAL ? most : most * factor;
             };

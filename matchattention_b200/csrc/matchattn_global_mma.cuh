@@ -247,6 +247,23 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
+// Two float32 at a time.
+struct Pair {
+    unsigned long long v;
+    __device__ __forceinline__ Pair(float low, float high) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(low), "f"(high)); }
+    __device__ __forceinline__ void get(float &low, float &high) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(low), "=f"(high) : "l"(v)); }
+};
+__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c)
+{
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(a.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return a;
+}
+__device__ __forceinline__ Pair pair_add(Pair a, Pair b)
+{
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(a.v) : "l"(a.v), "l"(b.v));
+    return a;
+}
+
 // tanh from one exponential, 1 - 2 / (e^2y + 1), given 2 y log2(e): off by a few 2^-24, absolutely
 __device__ __forceinline__ float tanh_of(float two_y_log2e) { return 1.0f - __fdividef(2.0f, exp2_fast(two_y_log2e) + 1.0f); }
 
