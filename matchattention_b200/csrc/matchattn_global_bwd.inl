@@ -74,10 +74,10 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         barrier_init(&sh.s_full, 1);
         barrier_init(&sh.dp_full, 1);
         barrier_init(&sh.done, 1);
-        barrier_init(&sh.p_full, 256);
-        barrier_init(&sh.ds_full, 256);
-        barrier_init(&sh.looked, 256);
-        barrier_init(&sh.stored, 256);
+        barrier_init(&sh.p_full, 8);
+        barrier_init(&sh.ds_full, 8);
+        barrier_init(&sh.looked, 8);
+        barrier_init(&sh.stored, 8);
         sh.broken = 0;
         for (int i = 0; i < 3; ++i) sh.odd[0][i] = sh.odd[1][i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -121,26 +121,34 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         if (elected()) {
             const int steps = (p.d + 15) / 16;
             const uint32_t score_kind = product_kind<T>(kTile, false), sum_kind = product_kind<T>(steps * 16, true);
-            const uint32_t fixed[2] = {shared_address(sh.fixed[0]), shared_address(sh.fixed[1])};
+            const uint64_t fixed[2] = {channel_operand(shared_address(sh.fixed[0])), channel_operand(shared_address(sh.fixed[1]))};
+            const uint64_t by_channel = channel_operand(shared_address(sh.moving[0][0])), by_row = row_operand(shared_address(sh.moving[0][0]));
             bool good = barrier_wait(&sh.fixed_full, 0, &sh.broken);
             int i = 0;
-            const auto moving = [&](int n, int which) { return shared_address(sh.moving[n % STAGES][which]); };
+            const auto moving = [&](uint64_t first, int n, int which) {
+                return first + static_cast<uint32_t>((n % STAGES * 2 + which) * (kTileBytes<DP> >> 4));
+            };
             // columns of a first operand: 64 moving rows in 32 words, the other 64 behind the first half's place of scores
-            const auto add_up = [&](uint32_t sums, uint32_t weights, uint32_t tile, bool add) {
+            const auto add_up = [&](uint32_t sums, uint32_t weights, uint64_t tile, bool add) {
 #pragma unroll
-                for (int s = 0; s < kTile / 16; ++s) product_ts(sums, weights + 8 * s + (s >= 4 ? 32 : 0), by_rows(tile, s), sum_kind, add || s > 0);
+                for (int s = 0; s < kTile / 16; ++s) product_ts(sums, weights + 8 * s + (s >= 4 ? 32 : 0), tile_rows(tile, s), sum_kind, add || s > 0);
+            };
+            const auto scores_of = [&](uint32_t to, uint64_t a, uint64_t b) {
+#pragma unroll
+                for (int s = 0; s < DP / 16; ++s)
+                    if (s < steps) product_ss(to, tile_channels(a, s), tile_channels(b, s), score_kind, s > 0);
             };
             const auto after_scores = [&](int n) {         // dV of tile n, when its P is there
                 good = good && barrier_wait(&sh.p_full, n & 1, &sh.broken);
                 if (!good) return;
                 tmem_after();
-                if (KEYS && !*static_cast<volatile int *>(&sh.by_hand[0])) add_up(sum_v, scores, moving(n, 1), n > 0);
+                if (KEYS && !*static_cast<volatile int *>(&sh.by_hand[0])) add_up(sum_v, scores, moving(by_row, n, 1), n > 0);
             };
             const auto after_slopes = [&](int n) {         // dK or dQ of tile n, when its dS is there
                 good = good && barrier_wait(&sh.ds_full, n & 1, &sh.broken);
                 if (!good) return;
                 tmem_after();
-                if (!*static_cast<volatile int *>(&sh.by_hand[1])) add_up(sum_k, slopes, moving(n, 0), n > 0);
+                if (!*static_cast<volatile int *>(&sh.by_hand[1])) add_up(sum_k, slopes, moving(by_row, n, 0), n > 0);
                 products_done(&sh.empty[n % STAGES]);
             };
             for (int r = 0; r < rounds && good; ++r)
@@ -149,11 +157,11 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     good = barrier_wait(&sh.full[i % STAGES], (i / STAGES) & 1, &sh.broken);
                     if (i > 0) after_scores(i - 1);
                     if (!good) break;
-                    for (int s = 0; s < steps; ++s) product_ss(scores, by_channels(fixed[0], s), by_channels(moving(i, 0), s), score_kind, s > 0);
+                    scores_of(scores, fixed[0], moving(by_channel, i, 0));
                     products_done(&sh.s_full);
                     if (i > 0) after_slopes(i - 1);
                     if (!good) break;
-                    for (int s = 0; s < steps; ++s) product_ss(slopes, by_channels(fixed[1], s), by_channels(moving(i, 1), s), score_kind, s > 0);
+                    scores_of(slopes, fixed[1], moving(by_channel, i, 1));
                     products_done(&sh.dp_full);
                     ++i;
                 }
@@ -281,7 +289,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     // (the slot after this one was last read two looks ago)
                     if ((tid & 127) == 0) *static_cast<volatile int *>(&sh.odd[w][(looks + 1) % 3]) = 0;
                     tmem_before();
-                    barrier_arrive(&sh.looked);
+                    warp_arrive(&sh.looked);
                     good = good && barrier_wait(&sh.looked, looks & 1, &sh.broken);
                     tmem_after();
                     hand_k = __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[0][looks % 3]) != 0);
@@ -291,7 +299,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 }
                 if (tid == 0) sh.by_hand[0] = hand_v;
                 tmem_before();
-                barrier_arrive(&sh.p_full);
+                warp_arrive(&sh.p_full);
                 good = good && barrier_wait(&sh.dp_full, i & 1, &sh.broken);
                 if (!good) break;
                 tmem_after();
@@ -320,7 +328,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 tmem_stored();
                 if (hand_k) {
                     tmem_before();
-                    barrier_arrive(&sh.stored);
+                    warp_arrive(&sh.stored);
                     good = barrier_wait(&sh.stored, stores & 1, &sh.broken);
                     tmem_after();
                     ++stores;
@@ -328,7 +336,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 }
                 if (tid == 0) sh.by_hand[1] = hand_k;
                 tmem_before();
-                barrier_arrive(&sh.ds_full);
+                warp_arrive(&sh.ds_full);
                 ++i;
             }
         }

@@ -58,6 +58,9 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
         return tile_state(mask, p.N, n0 + w * kTile, t * kTile, qr ? qr + w : nullptr, kr ? kr + t : nullptr);
     };
     const int end = (key_limit(mask, min(n0 + p.block_rows, p.N) - 1) + kTile - 1) / kTile;
+    // the same in short, for the two threads that copy and multiply: key tiles that a query tile sees any of
+    const int ends[2] = {(key_limit(mask, min(n0 + kTile, p.N) - 1) + kTile - 1) / kTile, tiles > 1 && n0 + kTile < p.N ? end : 0};
+    const auto seen = [&](int w, int t) { return tile_seen(t, ends[w], qr ? qr + w : nullptr, kr); };
     const int t_begin = split * p.tiles_per_split, t_end = p.splits > 1 ? min(end, t_begin + p.tiles_per_split) : end;
 
     if (tid == 0) {
@@ -68,10 +71,10 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
         }
         for (int w = 0; w < 2; ++w) {
             barrier_init(&sh.s_full[w], 1);
-            barrier_init(&sh.p_full[w], 2 * kTile);
+            barrier_init(&sh.p_full[w], 8);
             for (int i = 0; i < 4; ++i) barrier_init(&sh.agreed[w][i], 2);
             barrier_init(&sh.o_full[w], 1);
-            barrier_init(&sh.looked[w], 2 * kTile);
+            barrier_init(&sh.looked[w], 8);
             for (int i = 0; i < 3; ++i) sh.odd[w][i] = 0;
         }
         sh.broken = 0;
@@ -92,7 +95,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
             int n = 0;           // tiles copied, K and V counted apart
             bool good = true;
             for (int t = t_begin; t < t_end && good; ++t) {
-                if (state(0, t) == kHidden && state(1, t) == kHidden) continue;
+                if (!seen(0, t) && !seen(1, t)) continue;
                 for (int i = 0; i < 2 && good; ++i, ++n) {
                     const int s = n % STAGES;
                     if (n >= STAGES) good = barrier_wait(&sh.kv_empty[s], (n / STAGES - 1) & 1, &sh.broken);
@@ -113,46 +116,49 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
         if (elected()) {
             const int steps = (p.d + 15) / 16;
             const uint32_t score_kind = product_kind<T>(kTile, false), value_kind = product_kind<T>(steps * 16, true);
-            const uint32_t q_at[2] = {shared_address(sh.q[0]), shared_address(sh.q[1])}, kv_at = shared_address(sh.kv[0]);
+            const uint64_t query[2] = {channel_operand(shared_address(sh.q[0])), channel_operand(shared_address(sh.q[1]))};
+            const uint64_t keys = channel_operand(shared_address(sh.kv[0])), values_at = row_operand(shared_address(sh.kv[0]));
             int used[2] = {0, 0}, n = 0;            // tiles that each query tile has taken; buffers
-            int last_state[2] = {kHidden, kHidden}, last_v = 0;
+            bool last[2] = {false, false};          // which saw the tile before
+            int last_v = 0;
             bool good = barrier_wait(&sh.q_full, 0, &sh.broken);
             // O += P V of the tile before, for query tile w
             const auto values = [&](int w) {
-                if (last_state[w] == kHidden || !good) return;
+                if (!last[w] || !good) return;
                 good = barrier_wait(&sh.p_full[w], (used[w] - 1) & 1, &sh.broken);
                 if (!good) return;
                 tmem_after();
                 if (!*static_cast<volatile int *>(&sh.by_hand[w])) {
-                    const uint32_t v = kv_at + last_v * kTileBytes<DP>, out = tmem + 256 + w * kTile, prob = tmem + w * kTile;
+                    const uint64_t v = values_at + static_cast<uint32_t>(last_v * (kTileBytes<DP> >> 4));
+                    const uint32_t out = tmem + 256 + w * kTile, prob = tmem + w * kTile;
+                    const bool add = used[w] > 1;
 #pragma unroll
-                    for (int s = 0; s < kTile / 16; ++s) product_ts(out, prob + 8 * s + (s >= 4 ? 32 : 0), by_rows(v, s), value_kind, used[w] > 1 || s > 0);
+                    for (int s = 0; s < kTile / 16; ++s) product_ts(out, prob + 8 * s + (s >= 4 ? 32 : 0), tile_rows(v, s), value_kind, add || s > 0);
                 }
             };
             for (int t = t_begin; t < t_end && good; ++t) {
-                const int now[2] = {state(0, t), state(1, t)};
-                if (now[0] == kHidden && now[1] == kHidden) continue;
+                const bool now[2] = {seen(0, t), seen(1, t)};
+                if (!now[0] && !now[1]) continue;
                 const int k = n % STAGES, v = (n + 1) % STAGES;
+                const uint64_t key = keys + static_cast<uint32_t>(k * (kTileBytes<DP> >> 4));
                 good = barrier_wait(&sh.kv_full[k], (n / STAGES) & 1, &sh.broken);
-                bool waited = n == 0;
-                for (int w = 0; w < 2 && good; ++w) {
-                    if (!waited && last_state[w] != kHidden) {
-                        // the values of the tile before have landed
-                        good = barrier_wait(&sh.kv_full[last_v], ((n - 1) / STAGES) & 1, &sh.broken);
-                        waited = true;
-                    }
-                    if (good) values(w);
-                    if (now[w] == kHidden || !good) continue;
-                    const uint32_t scores = tmem + w * kTile, key = kv_at + k * kTileBytes<DP>;
-                    tmem_after();
-                    for (int s = 0; s < steps; ++s) product_ss(scores, by_channels(q_at[w], s), by_channels(key, s), score_kind, s > 0);
+                // the values of the tile before have landed
+                if (n > 0 && good) good = barrier_wait(&sh.kv_full[last_v], ((n - 1) / STAGES) & 1, &sh.broken);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    values(w);
+                    if (!now[w] || !good) continue;
+                    const uint32_t scores = tmem + w * kTile;
+#pragma unroll
+                    for (int s = 0; s < DP / 16; ++s)
+                        if (s < steps) product_ss(scores, tile_channels(query[w], s), tile_channels(key, s), score_kind, s > 0);
                     products_done(&sh.s_full[w]);
                     ++used[w];
                 }
                 if (!good) break;
                 if (n > 0) products_done(&sh.kv_empty[last_v]);
                 products_done(&sh.kv_empty[k]);
-                last_state[0] = now[0], last_state[1] = now[1];
+                last[0] = now[0], last[1] = now[1];
                 last_v = v;
                 n += 2;
             }
@@ -269,8 +275,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
             float high = probabilities(ref == -INFINITY ? 0.0f : ref);
             // the two halves of a row agree on its largest score
             sh.high[used & 1][w][half][row] = high;
-            __syncwarp();
-            if (lane == 0) barrier_arrive(&sh.agreed[w][warp & 3]);
+            warp_arrive(&sh.agreed[w][warp & 3]);
             good = barrier_wait(&sh.agreed[w][warp & 3], used & 1, &sh.broken);
             high = fmaxf(high, sh.high[used & 1][w][half ^ 1][row]);
             const bool grown = high > ref + kSlack;
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                 // (the slot after this one was last read two looks ago)
                 if (row == 0 && half == 0) *static_cast<volatile int *>(&sh.odd[w][(looks + 1) % 3]) = 0;
                 tmem_before();
-                barrier_arrive(&sh.looked[w]);
+                warp_arrive(&sh.looked[w]);
                 good = good && barrier_wait(&sh.looked[w], looks & 1, &sh.broken);
                 tmem_after();
                 hand = __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[w][looks % 3]) != 0);
@@ -312,14 +317,13 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
             }
             if (row == 0 && half == 0) sh.by_hand[w] = hand;
             tmem_before();
-            barrier_arrive(&sh.p_full[w]);
+            warp_arrive(&sh.p_full[w]);
             ++used;
             buffers += 2;
         }
         // the sum of the row's halves
         sh.high[used & 1][w][half][row] = sum;
-        __syncwarp();
-        if (lane == 0) barrier_arrive(&sh.agreed[w][warp & 3]);
+        warp_arrive(&sh.agreed[w][warp & 3]);
         good = good && barrier_wait(&sh.agreed[w][warp & 3], used & 1, &sh.broken);
         sum += sh.high[used & 1][w][half ^ 1][row];
         if (good) good = barrier_wait(&sh.o_full[w], 0, &sh.broken);

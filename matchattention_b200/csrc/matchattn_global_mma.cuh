@@ -46,6 +46,13 @@ __device__ __forceinline__ void barrier_arrive(uint64_t *bar)
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
 }
 
+// One arrival for a whole warp, after all of it (a barrier serves the arrivals of 256 threads one by one, for a microsecond).
+__device__ __forceinline__ void warp_arrive(uint64_t *bar)
+{
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) barrier_arrive(bar);
+}
+
 __device__ __forceinline__ bool barrier_test(uint64_t *bar, uint32_t parity)
 {
     uint32_t done;
@@ -131,10 +138,13 @@ __device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t half_dist
            static_cast<uint64_t>(1024 >> 4) << 32 | 1ULL << 46 | 2ULL << 61;
 }
 
-// channels [16 s, 16 s + 16) of a tile, summed over
-__device__ __forceinline__ uint64_t by_channels(uint32_t tile, int s) { return operand(tile + (s >> 2) * kHalfBytes + (s & 3) * 32, 16); }
-// rows [16 s, 16 s + 16) of a tile, summed over
-__device__ __forceinline__ uint64_t by_rows(uint32_t tile, int s) { return operand(tile + s * 2048, kHalfBytes); }
+// A tile as an operand that is summed over its channels, 16 at a time: channels [16 s, 16 s + 16).  (One thread issues all products, and
+// the instructions between them are its time: an operand is one addition.)
+__device__ __forceinline__ uint64_t channel_operand(uint32_t tile) { return operand(tile, 16); }
+__device__ __forceinline__ uint64_t tile_channels(uint64_t tile, int s) { return tile + static_cast<uint32_t>(((s >> 2) * kHalfBytes + (s & 3) * 32) >> 4); }
+// ... over its rows: rows [16 s, 16 s + 16)
+__device__ __forceinline__ uint64_t row_operand(uint32_t tile) { return operand(tile, kHalfBytes); }
+__device__ __forceinline__ uint64_t tile_rows(uint64_t tile, int s) { return tile + static_cast<uint32_t>(s * 2048 >> 4); }
 
 // Shape and types of a product of 128 rows: float32 sums; b_rows: the second operand is summed over its rows.
 template <typename T>
@@ -412,6 +422,15 @@ __device__ __forceinline__ int tile_state(const GlobalMask &m, int N, int n0, in
     const DocRange q = *qr, k = *kr;
     if (k.high < q.low || k.low > q.high || q.high < 0 || k.high < 0) return kHidden;
     return whole && q.pure && k.pure && q.low == q.high && k.low == k.high ? kWhole : kPartial;
+}
+
+// Whether queries whose last key tile is before `end` see anything of key tile t; with documents by their ranges.
+__device__ __forceinline__ bool tile_seen(int t, int end, const DocRange *qr, const DocRange *kr)
+{
+    if (t >= end) return false;
+    if (kr == nullptr) return true;
+    const DocRange q = *qr, k = kr[t];
+    return !(k.high < q.low || k.low > q.high || q.high < 0 || k.high < 0);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------
