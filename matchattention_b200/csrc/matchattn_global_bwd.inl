@@ -9,8 +9,8 @@
 // products where one pass with dQ added up in global memory has five, but the sums have one order and no atomics.
 //
 // A block has a fixed pair of tiles (keys: K, V; queries: Q, dO) and a moving pair (Q, dO; K, V).  The scores and dP of
-// fixed by moving rows come to tensor memory; a thread holds a fixed row and half of the 128 moving ones (warps 0-3 and 4-7), and puts P
-// over S and dS over dP, rounded to the type, as first operands of the products that add up the moving rows.  Order of the
+// fixed by moving rows come to tensor memory; a thread holds a fixed row and 32 of the 128 moving ones (warps 0-15), and puts P over S
+// and dS over dP, rounded to the type, as first operands of the products that add up the moving rows.  Order of the
 // matrix unit: dV(i-1), S(i), dK(i-1), dP(i): while threads take exponentials of tile i it forms dK(i-1) and dP(i), while
 // they form dS(i) it forms dV(i) and S(i+1).
 //
@@ -24,15 +24,16 @@
 namespace matchattn {
 namespace {
 
-constexpr int kBackThreads = 320;
+constexpr int kBackThreads = 576;
+constexpr int kPart = 32;                // moving rows of a thread
 
 template <int DP>
 struct BackShared {
     static constexpr int kStages = DP == 128 ? 2 : 3;
     uint8_t fixed[2][kTileBytes<DP>];
     uint8_t moving[kStages][2][kTileBytes<DP>];
-    float4 lse[8][16], delta[8][16], across[8][16], down[8][16];      // per warp, for its 64 moving rows; column and row on the map
-    int4 docs[8][16];
+    float4 lse[16][8], delta[16][8], across[16][8], down[16][8];      // per warp, for its 32 moving rows; column and row on the map
+    int4 docs[16][8];
     uint64_t fixed_full, full[kStages], empty[kStages], s_full, p_full, dp_full, ds_full, done, looked, stored;
     uint32_t tmem;
     int broken, by_hand[2], odd[2][3];
@@ -74,23 +75,23 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         barrier_init(&sh.s_full, 1);
         barrier_init(&sh.dp_full, 1);
         barrier_init(&sh.done, 1);
-        barrier_init(&sh.p_full, 8);
-        barrier_init(&sh.ds_full, 8);
-        barrier_init(&sh.looked, 8);
-        barrier_init(&sh.stored, 8);
+        barrier_init(&sh.p_full, 16);
+        barrier_init(&sh.ds_full, 16);
+        barrier_init(&sh.looked, 16);
+        barrier_init(&sh.stored, 16);
         sh.broken = 0;
         for (int i = 0; i < 3; ++i) sh.odd[0][i] = sh.odd[1][i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 9) tmem_take(&sh.tmem);
+    if (warp == 17) tmem_take(&sh.tmem);
     tmem_before();
     __syncthreads();
     tmem_after();
     const uint32_t tmem = sh.tmem;
     const uint32_t scores = tmem, slopes = tmem + 128, sum_v = tmem + 256, sum_k = tmem + 384;       // sum_k: dK or dQ
 
-    if (warp == 8) {
+    if (warp == 16) {
         // ---- copies
         if (elected()) {
             barrier_expect(&sh.fixed_full, 2 * kTileBytes<DP>);
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         // ---- products
         if (elected()) {
             const int steps = (p.d + 15) / 16;
@@ -128,10 +129,10 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
             const auto moving = [&](uint64_t first, int n, int which) {
                 return first + static_cast<uint32_t>((n % STAGES * 2 + which) * (kTileBytes<DP> >> 4));
             };
-            // columns of a first operand: 64 moving rows in 32 words, the other 64 behind the first half's place of scores
+            // columns of a first operand: 32 moving rows in the first 16 words of every 32
             const auto add_up = [&](uint32_t sums, uint32_t weights, uint64_t tile, bool add) {
 #pragma unroll
-                for (int s = 0; s < kTile / 16; ++s) product_ts(sums, weights + 8 * s + (s >= 4 ? 32 : 0), tile_rows(tile, s), sum_kind, add || s > 0);
+                for (int s = 0; s < kTile / 16; ++s) product_ts(sums, weights + 32 * (s / 2) + 8 * (s % 2), tile_rows(tile, s), sum_kind, add || s > 0);
             };
             const auto scores_of = [&](uint32_t to, uint64_t a, uint64_t b) {
 #pragma unroll
@@ -175,9 +176,9 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         __syncwarp();
     } else {
         // ---- probabilities and slopes
-        const int w = warp >> 2, f = f0 + (tid & 127);                          // half of the moving rows; the fixed row
+        const int w = warp >> 2, f = f0 + (tid & 127);                          // quarter of the moving rows; the fixed row
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
-        const uint32_t my_scores = scores + lanes + w * 64, my_slopes = slopes + lanes + w * 64;
+        const uint32_t my_scores = scores + lanes + w * kPart, my_slopes = slopes + lanes + w * kPart;
         const float factor = p.scale * kLog2e, inverse_cap = CAP ? p.scale / p.cap : 0.0f, outer = p.cap * kLog2e;
         // dS is held times 2^(lift - kLift), the sums of dS times 2^-lift
         int lift = 0;
@@ -201,52 +202,65 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
             lse = p.lse[line] - kLift;
             delta = p.delta[line];
         }
-        int i = 0, looks = 0, stores = 0;
+        // what a lane fetches of a tile's moving rows, one row of the warp's 32; a tile ahead, because it takes as long as a tile
+        float next_lse = 0.0f, next_delta = 0.0f;
+        int next_doc = -1;
+        const auto fetch = [&](int r, int t) {
+            const int m = t * kTile + w * kPart + lane;
+            if (KEYS) {
+                const long long line = (static_cast<long long>(b) * p.h + kh * p.g + r) * p.N + m;
+                next_lse = m < p.N ? p.lse[line] - kLift : INFINITY;
+                next_delta = m < p.N ? p.delta[line] : 0.0f;
+            }
+            if (p.q_docs) {
+                const int rows = KEYS ? p.N : p.M;
+                next_doc = m < rows ? (KEYS ? p.q_docs : p.k_docs)[static_cast<long long>(b) * rows + m] : -1;
+            }
+        };
+        // the visible tile after (r, t)
+        const auto advance = [&](int &r, int &t) {
+            do {
+                if (++t >= t_end) t = t_begin, ++r;
+            } while (r < rounds && state(t) == kHidden);
+        };
+        int i = 0, looks = 0, stores = 0, r = 0, t = t_begin - 1;
         bool good = true;
-        for (int r = 0; r < rounds && good; ++r) {
-            const int head = KEYS ? kh * p.g + r : own;
-            const float slope = BIAS != kNoBias ? p.slopes[head] * kLog2e : 0.0f;
-            for (int t = t_begin; t < t_end; ++t) {
-                const int now = state(t);
-                if (now == kHidden) continue;
-                const int m0 = t * kTile + w * 64;                              // first of the warp's moving rows
-#pragma unroll
-                for (int e = lane; e < 64; e += 32) {
-                    const int m = m0 + e;
-                    if (KEYS) {
-                        const long long line = (static_cast<long long>(b) * p.h + head) * p.N + m;
-                        reinterpret_cast<float *>(sh.lse[warp])[e] = m < p.N ? p.lse[line] - kLift : INFINITY;
-                        reinterpret_cast<float *>(sh.delta[warp])[e] = m < p.N ? p.delta[line] : 0.0f;
-                    }
-                    if (p.q_docs && now == kPartial) {
-                        const int rows = KEYS ? p.N : p.M;
-                        reinterpret_cast<int *>(sh.docs[warp])[e] = m < rows ? (KEYS ? p.q_docs : p.k_docs)[static_cast<long long>(b) * rows + m] : -1;
-                    }
-                    if (BIAS == kMapBias) {
-                        const float2 at = map_place(KEYS ? m + mask.shift : m, p.width);
-                        reinterpret_cast<float *>(sh.across[warp])[e] = at.x;
-                        reinterpret_cast<float *>(sh.down[warp])[e] = at.y;
-                    }
+        if (t_begin < t_end) advance(r, t);
+        else r = rounds;
+        if (r < rounds) fetch(r, t);
+        for (; r < rounds;) {
+            {
+                const int head = KEYS ? kh * p.g + r : own, now = state(t);
+                const float slope = BIAS != kNoBias ? p.slopes[head] * kLog2e : 0.0f;
+                const int m0 = t * kTile + w * kPart;                           // first of the warp's moving rows
+                if (KEYS) {
+                    reinterpret_cast<float *>(sh.lse[warp])[lane] = next_lse;
+                    reinterpret_cast<float *>(sh.delta[warp])[lane] = next_delta;
+                }
+                if (p.q_docs) reinterpret_cast<int *>(sh.docs[warp])[lane] = next_doc;
+                if (BIAS == kMapBias) {
+                    const float2 at = map_place(KEYS ? m0 + lane + mask.shift : m0 + lane, p.width);
+                    reinterpret_cast<float *>(sh.across[warp])[lane] = at.x;
+                    reinterpret_cast<float *>(sh.down[warp])[lane] = at.y;
                 }
                 __syncwarp();
+                advance(r, t);
+                if (r < rounds) fetch(r, t);
                 good = good && barrier_wait(&sh.s_full, i & 1, &sh.broken);
                 if (!good) break;
                 tmem_after();
-                float prob[64];                                                 // P, then P (1 - tanh^2)
+                float prob[kPart];                                              // P, then P (1 - tanh^2)
                 uint32_t *raw = reinterpret_cast<uint32_t *>(prob);
                 tmem_load32(my_scores, raw);
-                tmem_load32(my_scores + 32, raw + 32);
                 tmem_loaded32(raw);
-                tmem_loaded32(raw + 32);
                 const float from = here.y - static_cast<float>(KEYS ? m0 + mask.shift : m0);
                 const int bar = (KEYS ? first : limit) - m0;                    // keys: the moving rows from it on are seen; queries: those below
-#pragma unroll
-                for (int c = 0; c < 64; c += 32) {
+                {
                     uint32_t packed[16];
-                    if (CAP) tanh_all<32>(prob + c, inverse_cap);
+                    if (CAP) tanh_all<32>(prob, inverse_cap);
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
-                        const int four = (c + e) / 4;
+                        const int four = e / 4;
                         float level[4], value[4];
                         float4 row_lse, across, down;
                         int4 docs;
@@ -255,7 +269,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                         if (now == kPartial && p.q_docs) docs = sh.docs[warp][four];
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
-                            const int at = c + e + u;
+                            const int at = e + u;
                             level[u] = KEYS ? element(row_lse, u) : lse;
                             if (BIAS == kMapBias) level[u] = fmaf(slope, fabsf(here.x - element(across, u)) + fabsf(here.y - element(down, u)), level[u]);
                             if (BIAS == kSequenceBias) level[u] = fmaf(slope, fabsf(from - static_cast<float>(at)), level[u]);
@@ -277,17 +291,18 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                         packed[e / 2] = pack_two<T>(value[0], value[1]);
                         packed[e / 2 + 1] = pack_two<T>(value[2], value[3]);
                     }
-                    if (KEYS) tmem_store16(my_scores + c / 2, packed);
+                    if (KEYS) tmem_store16(my_scores, packed);
                 }
                 if (KEYS) tmem_stored();
-                // a partly hidden tile's moving rows are looked through: warps 0-3 the first tile, 4-7 the second
+                // a partly hidden tile's moving rows are looked through: warps 0-7 the first tile, 8-15 the second
                 bool hand_v = false, hand_k = false;
                 if (now == kPartial) {
                     const int s = i % STAGES;
                     good = barrier_wait(&sh.full[s], (i / STAGES) & 1, &sh.broken);
-                    if (good && (KEYS || w == 0) && (row_tainted<T, DP>(sh.moving[s][w], tid & 127, 0) || row_tainted<T, DP>(sh.moving[s][w], tid & 127, 1))) *static_cast<volatile int *>(&sh.odd[w][looks % 3]) = 1;
+                    if (good && (KEYS || w < 2) && row_tainted<T, DP>(sh.moving[s][w >> 1], tid & 127, w & 1))
+                        *static_cast<volatile int *>(&sh.odd[w >> 1][looks % 3]) = 1;
                     // (the slot after this one was last read two looks ago)
-                    if ((tid & 127) == 0) *static_cast<volatile int *>(&sh.odd[w][(looks + 1) % 3]) = 0;
+                    if ((tid & 255) == 0) *static_cast<volatile int *>(&sh.odd[w >> 1][(looks + 1) % 3]) = 0;
                     tmem_before();
                     warp_arrive(&sh.looked);
                     good = good && barrier_wait(&sh.looked, looks & 1, &sh.broken);
@@ -295,7 +310,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     hand_k = __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[0][looks % 3]) != 0);
                     hand_v = KEYS && __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[1][looks % 3]) != 0);
                     ++looks;
-                    if (hand_v && w == 0) add_rows<T, DP>(sum_v + lanes, scores + lanes, 32, sh.moving[s][1], i > 0);
+                    if (hand_v && w == 0) add_rows<T, DP, kPart>(sum_v + lanes, scores + lanes, sh.moving[s][1], i > 0);
                 }
                 if (tid == 0) sh.by_hand[0] = hand_v;
                 tmem_before();
@@ -303,19 +318,18 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 good = good && barrier_wait(&sh.dp_full, i & 1, &sh.broken);
                 if (!good) break;
                 tmem_after();
-#pragma unroll
-                for (int c = 0; c < 64; c += 32) {
+                {
                     uint32_t dp[32], packed[16];
-                    tmem_load32(my_slopes + c, dp);
+                    tmem_load32(my_slopes, dp);
                     tmem_loaded32(dp);
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         float4 row_delta;
-                        if (KEYS) row_delta = sh.delta[warp][(c + e) / 4];
+                        if (KEYS) row_delta = sh.delta[warp][e / 4];
                         float value[4];
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
-                            const int at = c + e + u;
+                            const int at = e + u;
                             const float off = __uint_as_float(dp[e + u]) - (KEYS ? element(row_delta, u) : delta);
                             value[u] = prob[at] * (HALF ? off * hold : off);
                             if (now == kPartial && prob[at] == 0.0f) value[u] = 0.0f;
@@ -323,7 +337,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                         packed[e / 2] = pack_two<T>(value[0], value[1]);
                         packed[e / 2 + 1] = pack_two<T>(value[2], value[3]);
                     }
-                    tmem_store16(my_slopes + c / 2, packed);
+                    tmem_store16(my_slopes, packed);
                 }
                 tmem_stored();
                 if (hand_k) {
@@ -332,7 +346,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     good = barrier_wait(&sh.stored, stores & 1, &sh.broken);
                     tmem_after();
                     ++stores;
-                    if (w == 1) add_rows<T, DP>(sum_k + lanes, slopes + lanes, 32, sh.moving[i % STAGES][0], i > 0);
+                    if (w == 1) add_rows<T, DP, kPart>(sum_k + lanes, slopes + lanes, sh.moving[i % STAGES][0], i > 0);
                 }
                 if (tid == 0) sh.by_hand[1] = hand_k;
                 tmem_before();
@@ -342,13 +356,13 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         }
         if (good) good = barrier_wait(&sh.done, 0, &sh.broken);
         tmem_after();
-        // ---- results: dV by warps 0-3 and dK by 4-7, or dQ's channels in turn
+        // ---- results: dV by warps 0-7 and dK by 8-15, or dQ by all, the channels in turn
         const int rows = KEYS ? p.M : p.N;
-        const float times = KEYS && w == 0 ? (HALF ? 1.0f / 4096.0f : 1.0f) : p.scale * ldexpf(1.0f, -lift);
-        T *to = static_cast<T *>(KEYS ? (w == 0 ? p.d_v : p.d_k) : p.d_q) + ((static_cast<long long>(b) * rows + f) * heads + own) * p.d;
-        const uint32_t from = (KEYS && w == 0 ? sum_v : sum_k) + lanes;
+        const float times = KEYS && w < 2 ? (HALF ? 1.0f / 4096.0f : 1.0f) : p.scale * ldexpf(1.0f, -lift);
+        T *to = static_cast<T *>(KEYS ? (w < 2 ? p.d_v : p.d_k) : p.d_q) + ((static_cast<long long>(b) * rows + f) * heads + own) * p.d;
+        const uint32_t from = (KEYS && w < 2 ? sum_v : sum_k) + lanes;
 #pragma unroll 1
-        for (int c = KEYS ? 0 : w * 32; c < DP && c < p.d; c += KEYS ? 32 : 64) {
+        for (int c = 32 * (KEYS ? w & 1 : w); c < DP && c < p.d; c += KEYS ? 64 : 128) {
             uint32_t raw[32] = {};
             if (i > 0) {
                 tmem_load32(from + c, raw);
@@ -367,7 +381,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
     }
     tmem_before();
     __syncthreads();
-    if (warp == 9) tmem_give(tmem);
+    if (warp == 17) tmem_give(tmem);
 }
 
 template <typename T, int DP, bool CAP, GlobalBias BIAS, bool KEYS>

@@ -362,11 +362,11 @@ __device__ __forceinline__ bool row_tainted(const uint8_t *tile, int row, int pa
     return tainted<T>(acc);
 }
 
-// The product of the weights in tensor memory (128 x 16 bits per row at `weights`, `gap` words between the halves) and a tile's rows, added to the thread's row
+// The product of the weights in tensor memory (128 x 16 bits per row from `weights` on, RUN of them side by side in every RUN columns) and a tile's rows, added to the thread's row
 // of sums at `sums` term by term, leaving out the terms of weight zero: in place of the matrix instruction where the tile holds
 // infinite or NaN values that some rows do not see.  A warp's 32 rows; rare, and slow.
-template <typename T, int DP>
-static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, int gap, const uint8_t *tile, bool add)
+template <typename T, int DP, int RUN>
+static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, const uint8_t *tile, bool add)
 {
     for (int c = 0; c < DP; c += 8) {
         uint32_t raw[8] = {};
@@ -378,7 +378,7 @@ static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, in
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] = __uint_as_float(raw[i]);
         for (int j = 0; j < kTile; j += 2) {
-            uint32_t w = tmem_load1(weights + j / 2 + (j >= kTile / 2 ? gap : 0));
+            uint32_t w = tmem_load1(weights + j / RUN * RUN + j % RUN / 2);
             tmem_loaded1(w);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
