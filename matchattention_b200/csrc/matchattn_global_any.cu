@@ -9,7 +9,7 @@
 //
 // A value that no row of a tile may see can still be infinite or NaN, and 0 * NaN is NaN: a tile that holds such a value is
 // accumulated term by term, leaving out the terms of weight zero.
-#include "matchattn_global.cuh"
+#include "matchattn_global_mma.cuh"
 
 #include <type_traits>
 
@@ -35,30 +35,60 @@ __device__ __forceinline__ void load_four(const T *p, int n, bool vec, float (&x
     }
 }
 
-// dst[channel][row] = row(r)[channel]; rows that `row` has no address for, and channels from d on, are zero.  True if a value is
-// infinite or NaN.
+// A tile of ROWS rows between global and shared memory, in registers: four channels of a row at a time.  Fetched ahead of its place
+// in shared memory falling free, it is on its way while the tile before it is computed.
+template <typename T, int DP, int ROWS>
+struct Tile {
+    static constexpr int kPieces = (ROWS * (DP / 4) + kAnyThreads - 1) / kAnyThreads;
+    float x[kPieces][4];
+
+    // rows that `row` has no address for, and channels from d on, are zero
+    template <typename Row>
+    __device__ __forceinline__ void fetch(int d, bool vec, Row row)
+    {
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            const int i = threadIdx.x + k * kAnyThreads, r = i % ROWS, c = i / ROWS * 4;
+            const T *src = i < ROWS * (DP / 4) && c < d ? row(r) : nullptr;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[k][j] = 0.0f;
+            if (src != nullptr) load_four<T>(src + c, d - c, vec, x[k]);
+        }
+    }
+
+    // dst[channel][row]; true if a value is infinite or NaN
+    __device__ __forceinline__ bool put(float *dst) const
+    {
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            const int i = threadIdx.x + k * kAnyThreads, r = i % ROWS, c = i / ROWS * 4;
+            if (i >= ROWS * (DP / 4)) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                bad |= !(fabsf(x[k][j]) <= 3.402823466e38f);
+                dst[(c + j) * (ROWS + 4) + r] = x[k][j];
+            }
+        }
+        return bad;
+    }
+};
+
 template <typename T, int DP, int ROWS, typename Row>
 __device__ __forceinline__ bool load_transposed(float *dst, int d, bool vec, Row row)
 {
-    bool bad = false;
-    for (int i = threadIdx.x; i < ROWS * (DP / 4); i += kAnyThreads) {
-        const int r = i % ROWS, c = i / ROWS * 4;
-        const T *src = row(r);
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (src != nullptr && c < d) load_four<T>(src + c, d - c, vec, x);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            bad |= !(fabsf(x[j]) <= 3.402823466e38f);
-            dst[(c + j) * (ROWS + 4) + r] = x[j];
-        }
-    }
-    return bad;
+    Tile<T, DP, ROWS> tile;
+    tile.fetch(d, vec, row);
+    return tile.put(dst);
 }
 
 template <int R>
 __device__ __forceinline__ void read_run(const float *p, float (&x)[R])
 {
-    if constexpr (R == 4) {
+    if constexpr (R == 8) {
+        const float4 t = *reinterpret_cast<const float4 *>(p), u = *reinterpret_cast<const float4 *>(p + 4);
+        x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w, x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
+    } else if constexpr (R == 4) {
         const float4 t = *reinterpret_cast<const float4 *>(p);
         x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
     } else if constexpr (R == 2) {
@@ -121,17 +151,30 @@ __device__ __forceinline__ void accumulate(float (&acc)[RA][NC], const float *w,
     }
 }
 
-// The score in units of log2 of a pair whose scaled product is x, and the slope of the cap there.
-__device__ __forceinline__ float any_score(const GlobalParams &p, float product, float &slant)
+// tanh(x / cap) of every element in place, for products x / scale.  (A block takes the polynomial where all of a warp's scores are well
+// below the cap; the library's function is long, and a copy of it per element.)
+template <int RA, int RB>
+__device__ __forceinline__ void capped(float (&s)[RA][RB], float inverse_cap)
 {
-    float x = product * p.scale;
-    slant = 1.0f;
-    if (p.cap != 0.0f) {
-        const float t = tanhf(x / p.cap);
-        slant = 1.0f - t * t;
-        x = p.cap * t;
+    float big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < RA; ++i)
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+            s[i][j] *= inverse_cap;
+            big = fmaxf(big, fabsf(s[i][j]));
+        }
+    if (__all_sync(0xffffffffu, big <= kSmallTanh)) {
+#pragma unroll
+        for (int i = 0; i < RA; ++i)
+#pragma unroll
+            for (int j = 0; j < RB; ++j) s[i][j] = tanh_small(s[i][j]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < RA; ++i)
+#pragma unroll
+            for (int j = 0; j < RB; ++j) s[i][j] = fabsf(s[i][j]) <= kSmallTanh ? tanh_small(s[i][j]) : tanh_of(2.0f * kLog2e * s[i][j]);
     }
-    return x * kLog2e;
 }
 
 struct RowOf {
@@ -202,8 +245,15 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_forward_kernel(const G
         doc_of[i] = p.q_docs ? p.q_docs[static_cast<long long>(b) * p.N + t.n] : 0;
     }
     const int end = key_end(mask, (min(r0 + BM, rows) - 1) / p.g);
+    const int whole = p.q_docs ? -1 : key_end(mask, r0 / p.g);         // tiles that end below it are seen by all rows
     const int t_end = p.splits > 1 ? min((end + BN - 1) / BN, (split + 1) * p.tiles_per_split) : (end + BN - 1) / BN;
-    for (int t = split * p.tiles_per_split; t < t_end; ++t) {
+    Tile<T, DP, BN> tile;
+    const auto fetch = [&](const void *base, const long long (&stride)[3], int j0) {
+        tile.fetch(p.d, p.vec, [&](int r) -> const T * { return j0 + r < mask.len ? at<T>(base, stride, b, j0 + r, kh) : nullptr; });
+    };
+    const int t_begin = split * p.tiles_per_split;
+    if (!p.k_docs && t_begin < t_end) fetch(p.k, p.ks, t_begin * BN);
+    for (int t = t_begin; t < t_end; ++t) {
         const int j0 = t * BN;
         __syncthreads();
         bool any = true;
@@ -218,47 +268,63 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_forward_kernel(const G
         } else if (p.k_docs) {
             any = false;
         }
-        if (p.k_docs && !__syncthreads_or(any)) continue;
-        load_transposed<T, DP, BN>(kvt, p.d, p.vec, [&](int r) -> const T * {
-            return j0 + r < mask.len ? at<T>(p.k, p.ks, b, j0 + r, kh) : nullptr;
-        });
+        if (p.k_docs) {
+            if (!__syncthreads_or(any)) continue;
+            fetch(p.k, p.ks, j0);
+        }
+        tile.put(kvt);
         __syncthreads();
+        fetch(p.v, p.vs, j0);
         float s[RM][RN] = {};
         products<RM, RN, PM, PN>(s, qt, kvt, p.d, ty, tx);
+        // scores in units of log2; what only some calls or tiles have stands in loops of its own
+        if (p.cap != 0.0f) capped(s, p.scale / p.cap);
+        const float unit = (p.cap != 0.0f ? p.cap : p.scale) * kLog2e;
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+            for (int j = 0; j < RN; ++j) s[i][j] *= unit;
+        if (p.slopes) {
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                const float2 there = place[RN * tx + j];
+#pragma unroll
+                for (int i = 0; i < RM; ++i) s[i][j] -= slope[i] * map_distance(here[i], there);
+            }
+        }
+        if (j0 + BN > whole) {
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                const int c = RN * tx + j, id = p.k_docs ? doc[c] : 0;
+#pragma unroll
+                for (int i = 0; i < RM; ++i)
+                    if (!sees(mask, n_of[i], j0 + c) || id != doc_of[i] || id < 0) s[i][j] = -INFINITY;
+            }
+        }
         float high[RM];
 #pragma unroll
         for (int i = 0; i < RM; ++i) {
             high[i] = top[i];
 #pragma unroll
-            for (int j = 0; j < RN; ++j) {
-                const int c = RN * tx + j;
-                float slant;
-                float x = any_score(p, s[i][j], slant);
-                if (p.slopes) x -= slope[i] * map_distance(here[i], place[c]);
-                const bool seen = sees(mask, n_of[i], j0 + c) && (!p.k_docs || (doc[c] == doc_of[i] && doc[c] >= 0));
-                s[i][j] = seen ? x : -INFINITY;
-                high[i] = fmaxf(high[i], s[i][j]);
-            }
+            for (int j = 0; j < RN; ++j) high[i] = fmaxf(high[i], s[i][j]);
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], o));
             const float ref = high[i] == -INFINITY ? 0.0f : high[i];
-            const float shrink = exp2f(top[i] - ref);
+            const float shrink = exp2_fast(top[i] - ref);
             top[i] = high[i];
             sum[i] *= shrink;
 #pragma unroll
             for (int c = 0; c < NC; ++c) acc[i][c] *= shrink;
 #pragma unroll
             for (int j = 0; j < RN; ++j) {
-                const float e = exp2f(s[i][j] - ref);
+                const float e = exp2_fast(s[i][j] - ref);
                 sum[i] += e;
                 w[(RM * ty + i) * PN + RN * tx + j] = e;
             }
         }
         __syncthreads();
-        const bool odd = load_transposed<T, DP, BN>(kvt, p.d, p.vec, [&](int r) -> const T * {
-            return j0 + r < mask.len ? at<T>(p.v, p.vs, b, j0 + r, kh) : nullptr;
-        });
-        const bool bad = __syncthreads_or(odd);
+        const bool bad = __syncthreads_or(tile.put(kvt));
+        if (!p.k_docs && t + 1 < t_end) fetch(p.k, p.ks, j0 + BN);
         accumulate<RM, NC, BN>(acc, w, kvt, ty, tx, bad);
     }
 #pragma unroll
@@ -288,46 +354,36 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_forward_kernel(const G
     }
 }
 
-// dS of a pair from its scaled product, dP and the row's figures; p is the probability.
-__device__ __forceinline__ float any_slope(const GlobalParams &p, float product, float dp, float bias, float lse, float delta, bool seen,
-                                           float &prob)
-{
-    float slant;
-    const float x = any_score(p, product, slant) - bias;
-    prob = seen ? exp2f(x - lse) : 0.0f;
-    return seen ? prob * slant * (dp - delta) : 0.0f;
-}
-
-// dQ: the rows of the forward kernel, scores and probabilities recomputed.
-template <typename T, int DP, int R>
+// dQ: the rows of the forward kernel, scores and probabilities recomputed.  K and V take turns in one place, K twice.
+template <typename T, int DP, int RM, int RN>
 __global__ void __launch_bounds__(kAnyThreads) global_any_dq_kernel(const GlobalParams p)
 {
     chain_begin();
-    constexpr int BT = 16 * R, P = BT + 4, NC = DP / 16;
+    constexpr int BM = 16 * RM, BN = 16 * RN, PM = BM + 4, PN = BN + 4, NC = DP / 16;
     extern __shared__ __align__(16) float smem[];
-    float *qt = smem, *dot = qt + DP * P, *kt = dot + DP * P, *vt = kt + DP * P, *w = vt + DP * P;
-    float2 *place = reinterpret_cast<float2 *>(w + BT * P);
-    int *doc = reinterpret_cast<int *>(place + BT), *range = doc + BT;
+    float *qt = smem, *dot = qt + DP * PM, *kvt = dot + DP * PM, *w = kvt + DP * PN;
+    float2 *place = reinterpret_cast<float2 *>(w + BM * PN);
+    int *doc = reinterpret_cast<int *>(place + BN), *range = doc + BN;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int r0 = blockIdx.x * BT, kh = blockIdx.y, b = blockIdx.z, rows = p.N * p.g;
+    const int r0 = blockIdx.x * BM, kh = blockIdx.y, b = blockIdx.z, rows = p.N * p.g;
     const GlobalMask mask = global_mask(p, b);
-    load_transposed<T, DP, BT>(qt, p.d, p.vec, [&](int r) -> const T * {
+    load_transposed<T, DP, BM>(qt, p.d, p.vec, [&](int r) -> const T * {
         if (r0 + r >= rows) return nullptr;
         const RowOf t = row_of(p, kh, r0 + r);
         return at<T>(p.q, p.qs, b, t.n, t.head);
     });
-    load_transposed<T, DP, BT>(dot, p.d, p.vec, [&](int r) -> const T * {
+    load_transposed<T, DP, BM>(dot, p.d, p.vec, [&](int r) -> const T * {
         if (r0 + r >= rows) return nullptr;
         const RowOf t = row_of(p, kh, r0 + r);
         return static_cast<const T *>(p.d_out) + ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
     });
-    if (p.q_docs) row_documents(p, b, r0, BT, range);
-    float acc[R][NC] = {}, lse[R], delta[R], slope[R];
-    float2 here[R];
-    int n_of[R], doc_of[R];
+    if (p.q_docs) row_documents(p, b, r0, BM, range);
+    float acc[RM][NC] = {}, lse[RM], delta[RM], slope[RM];
+    float2 here[RM];
+    int n_of[RM], doc_of[RM];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const RowOf t = row_of(p, kh, min(r0 + R * ty + i, rows - 1));
+    for (int i = 0; i < RM; ++i) {
+        const RowOf t = row_of(p, kh, min(r0 + RM * ty + i, rows - 1));
         const long long row = (static_cast<long long>(b) * p.h + t.head) * p.N + t.n;
         lse[i] = p.lse[row];
         delta[i] = p.delta[row];
@@ -336,11 +392,17 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dq_kernel(const Global
         here[i] = map_place(t.n + mask.shift, p.width);
         doc_of[i] = p.q_docs ? p.q_docs[static_cast<long long>(b) * p.N + t.n] : 0;
     }
-    const int end = key_end(mask, (min(r0 + BT, rows) - 1) / p.g);
-    for (int j0 = 0; j0 < end; j0 += BT) {
+    const int end = key_end(mask, (min(r0 + BM, rows) - 1) / p.g);
+    const int whole = p.q_docs ? -1 : key_end(mask, r0 / p.g);         // tiles that end below it are seen by all rows
+    Tile<T, DP, BN> tile;
+    const auto fetch = [&](const void *base, const long long (&stride)[3], int j0) {
+        tile.fetch(p.d, p.vec, [&](int r) -> const T * { return j0 + r < mask.len ? at<T>(base, stride, b, j0 + r, kh) : nullptr; });
+    };
+    if (!p.k_docs && end > 0) fetch(p.k, p.ks, 0);
+    for (int j0 = 0; j0 < end; j0 += BN) {
         __syncthreads();
         bool any = true;
-        if (tid < BT) {
+        if (tid < BN) {
             const int j = j0 + tid;
             place[tid] = map_place(j, p.width);
             if (p.k_docs) {
@@ -351,33 +413,69 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dq_kernel(const Global
         } else if (p.k_docs) {
             any = false;
         }
-        if (p.k_docs && !__syncthreads_or(any)) continue;
-        const bool odd = load_transposed<T, DP, BT>(kt, p.d, p.vec, [&](int r) -> const T * {
-            return j0 + r < mask.len ? at<T>(p.k, p.ks, b, j0 + r, kh) : nullptr;
-        });
-        load_transposed<T, DP, BT>(vt, p.d, p.vec, [&](int r) -> const T * {
-            return j0 + r < mask.len ? at<T>(p.v, p.vs, b, j0 + r, kh) : nullptr;
-        });
-        const bool bad = __syncthreads_or(odd);
-        float s[R][R] = {}, dp[R][R] = {};
-        products<R, R, P, P>(s, qt, kt, p.d, ty, tx);
-        products<R, R, P, P>(dp, dot, vt, p.d, ty, tx);
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                const int c = R * tx + j;
-                const float bias = p.slopes ? slope[i] * map_distance(here[i], place[c]) : 0.0f;
-                const bool seen = sees(mask, n_of[i], j0 + c) && (!p.k_docs || (doc[c] == doc_of[i] && doc[c] >= 0));
-                float prob;
-                w[(R * ty + i) * P + c] = any_slope(p, s[i][j], dp[i][j], bias, lse[i], delta[i], seen, prob);
-            }
+        if (p.k_docs) {
+            if (!__syncthreads_or(any)) continue;
+            fetch(p.k, p.ks, j0);
+        }
+        tile.put(kvt);
         __syncthreads();
-        accumulate<R, NC, BT>(acc, w, kt, ty, tx, bad);
+        fetch(p.v, p.vs, j0);
+        float s[RM][RN] = {}, dp[RM][RN] = {};
+        products<RM, RN, PM, PN>(s, qt, kvt, p.d, ty, tx);
+        __syncthreads();
+        tile.put(kvt);
+        __syncthreads();
+        fetch(p.k, p.ks, j0);
+        products<RM, RN, PM, PN>(dp, dot, kvt, p.d, ty, tx);
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+            for (int j = 0; j < RN; ++j) dp[i][j] -= delta[i];
+        if (p.cap != 0.0f) {
+            capped(s, p.scale / p.cap);
+#pragma unroll
+            for (int i = 0; i < RM; ++i)
+#pragma unroll
+                for (int j = 0; j < RN; ++j) dp[i][j] *= fmaf(-s[i][j], s[i][j], 1.0f);
+        }
+        const float unit = (p.cap != 0.0f ? p.cap : p.scale) * kLog2e;
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+            for (int j = 0; j < RN; ++j) s[i][j] *= unit;
+        if (p.slopes) {
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                const float2 there = place[RN * tx + j];
+#pragma unroll
+                for (int i = 0; i < RM; ++i) s[i][j] -= slope[i] * map_distance(here[i], there);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+            for (int j = 0; j < RN; ++j) dp[i][j] *= exp2_fast(s[i][j] - lse[i]);
+        if (j0 + BN > whole) {
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                const int c = RN * tx + j, id = p.k_docs ? doc[c] : 0;
+#pragma unroll
+                for (int i = 0; i < RM; ++i)
+                    if (!sees(mask, n_of[i], j0 + c) || id != doc_of[i] || id < 0) dp[i][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+            for (int j = 0; j < RN; ++j) w[(RM * ty + i) * PN + RN * tx + j] = dp[i][j];
+        __syncthreads();
+        const bool bad = __syncthreads_or(tile.put(kvt));
+        if (!p.k_docs && j0 + BN < end) fetch(p.k, p.ks, j0 + BN);
+        accumulate<RM, NC, BN>(acc, w, kvt, ty, tx, bad);
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int r = r0 + R * ty + i;
+    for (int i = 0; i < RM; ++i) {
+        const int r = r0 + RM * ty + i;
         if (r >= rows) continue;
         const RowOf t = row_of(p, kh, r);
         T *out = static_cast<T *>(p.d_q) + ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
@@ -387,33 +485,29 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dq_kernel(const Global
     }
 }
 
-// dK and dV: a block owns a tile of keys of one key head and walks the query rows of all heads that share it.
-template <typename T, int DP, int R>
+// dK and dV: a block owns a tile of keys of one key head and walks the query rows of all heads that share it.  Q and dO take turns
+// in one place, Q twice.
+template <typename T, int DP, int RM, int RN>
 __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const GlobalParams p)
 {
     chain_begin();
-    constexpr int BT = 16 * R, P = BT + 4, NC = DP / 16;
+    constexpr int BM = 16 * RM, BN = 16 * RN, PM = BM + 4, PN = BN + 4, NC = DP / 16;
     extern __shared__ __align__(16) float smem[];
-    float *qt = smem, *dot = qt + DP * P, *kt = dot + DP * P, *vt = kt + DP * P, *w = vt + DP * P;
-    float2 *place = reinterpret_cast<float2 *>(w + BT * P);
-    float *lse = reinterpret_cast<float *>(place + BT), *delta = lse + BT, *slope = delta + BT;
-    int *n_of = reinterpret_cast<int *>(slope + BT), *doc = n_of + BT, *range = doc + BT;
+    float *kt = smem, *vt = kt + DP * PM, *qot = vt + DP * PM, *w = qot + DP * PN;
+    float2 *place = reinterpret_cast<float2 *>(w + BM * PN);
+    float *lse = reinterpret_cast<float *>(place + BN), *delta = lse + BN, *slope = delta + BN;
+    int *n_of = reinterpret_cast<int *>(slope + BN), *doc = n_of + BN, *range = doc + BN;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int j0 = blockIdx.x * BT, kh = blockIdx.y, b = blockIdx.z, rows = p.N * p.g;
+    const int j0 = blockIdx.x * BM, kh = blockIdx.y, b = blockIdx.z, rows = p.N * p.g;
     const GlobalMask mask = global_mask(p, b);
-    const bool odd_k = load_transposed<T, DP, BT>(kt, p.d, p.vec, [&](int r) -> const T * {
-        return j0 + r < mask.len ? at<T>(p.k, p.ks, b, j0 + r, kh) : nullptr;
-    });
-    static_cast<void>(odd_k);
-    load_transposed<T, DP, BT>(vt, p.d, p.vec, [&](int r) -> const T * {
-        return j0 + r < mask.len ? at<T>(p.v, p.vs, b, j0 + r, kh) : nullptr;
-    });
-    float acc_k[R][NC] = {}, acc_v[R][NC] = {};
-    float2 here[R];
-    int doc_of[R];
+    load_transposed<T, DP, BM>(kt, p.d, p.vec, [&](int r) -> const T * { return j0 + r < mask.len ? at<T>(p.k, p.ks, b, j0 + r, kh) : nullptr; });
+    load_transposed<T, DP, BM>(vt, p.d, p.vec, [&](int r) -> const T * { return j0 + r < mask.len ? at<T>(p.v, p.vs, b, j0 + r, kh) : nullptr; });
+    float acc_k[RM][NC] = {}, acc_v[RM][NC] = {};
+    float2 here[RM];
+    int doc_of[RM];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int j = j0 + R * ty + i;
+    for (int i = 0; i < RM; ++i) {
+        const int j = j0 + RM * ty + i;
         here[i] = map_place(j, p.width);
         doc_of[i] = p.k_docs && j < p.M ? p.k_docs[static_cast<long long>(b) * p.M + j] : p.k_docs ? -1 : 0;
     }
@@ -422,7 +516,7 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
         __syncthreads();
         if (tx == 0) {
 #pragma unroll
-            for (int i = 0; i < R; ++i)
+            for (int i = 0; i < RM; ++i)
                 if (doc_of[i] >= 0) {
                     atomicMin(range, doc_of[i]);
                     atomicMax(range + 1, doc_of[i]);
@@ -431,10 +525,20 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
         __syncthreads();
     }
     const long long first = static_cast<long long>(query_begin(mask, j0)) * p.g;
-    for (int r0 = first < rows ? static_cast<int>(first) / BT * BT : rows; r0 < rows; r0 += BT) {
+    Tile<T, DP, BN> tile;
+    const auto fetch_q = [&](int r0) {
+        tile.fetch(p.d, p.vec, [&](int r) -> const T * {
+            if (r0 + r >= rows) return nullptr;
+            const RowOf t = row_of(p, kh, r0 + r);
+            return at<T>(p.q, p.qs, b, t.n, t.head);
+        });
+    };
+    const int r_begin = first < rows ? static_cast<int>(first) / BN * BN : rows;
+    if (!p.q_docs && r_begin < rows) fetch_q(r_begin);
+    for (int r0 = r_begin; r0 < rows; r0 += BN) {
         __syncthreads();
         bool any = true;
-        if (tid < BT) {
+        if (tid < BN) {
             const bool in = r0 + tid < rows;
             const RowOf t = row_of(p, kh, min(r0 + tid, rows - 1));
             const long long row = (static_cast<long long>(b) * p.h + t.head) * p.N + t.n;
@@ -451,45 +555,83 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
         } else if (p.q_docs) {
             any = false;
         }
-        if (p.q_docs && !__syncthreads_or(any)) continue;
-        const bool odd_q = load_transposed<T, DP, BT>(qt, p.d, p.vec, [&](int r) -> const T * {
-            if (r0 + r >= rows) return nullptr;
-            const RowOf t = row_of(p, kh, r0 + r);
-            return at<T>(p.q, p.qs, b, t.n, t.head);
-        });
-        const bool odd_o = load_transposed<T, DP, BT>(dot, p.d, p.vec, [&](int r) -> const T * {
+        if (p.q_docs) {
+            if (!__syncthreads_or(any)) continue;
+            fetch_q(r0);
+        }
+        const bool odd_q = tile.put(qot);
+        __syncthreads();
+        tile.fetch(p.d, p.vec, [&](int r) -> const T * {
             if (r0 + r >= rows) return nullptr;
             const RowOf t = row_of(p, kh, r0 + r);
             return static_cast<const T *>(p.d_out) + ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
         });
+        float s[RM][RN] = {}, dp[RM][RN] = {};
+        products<RM, RN, PM, PN>(s, kt, qot, p.d, ty, tx);
+        __syncthreads();
+        const bool odd_o = tile.put(qot);
         const bool bad = __syncthreads_or(odd_q || odd_o);
-        float s[R][R] = {}, dp[R][R] = {};
-        products<R, R, P, P>(s, kt, qt, p.d, ty, tx);
-        products<R, R, P, P>(dp, vt, dot, p.d, ty, tx);
+        fetch_q(r0);
+        products<RM, RN, PM, PN>(dp, vt, qot, p.d, ty, tx);
+        if (p.cap != 0.0f) capped(s, p.scale / p.cap);
+        const float unit = (p.cap != 0.0f ? p.cap : p.scale) * kLog2e;
+        // (queries that stand before all of the tile's keys, or behind the last row, need the masks)
+        const bool whole = !p.q_docs && r0 + BN <= rows && j0 + BM <= key_end(mask, r0 / p.g);
 #pragma unroll
-        for (int i = 0; i < R; ++i)
+        for (int j = 0; j < RN; ++j) {
+            const int c = RN * tx + j;
+            const float less = delta[c], level = lse[c];
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-                const int c = R * tx + j;
-                const float bias = p.slopes ? slope[c] * map_distance(here[i], place[c]) : 0.0f;
-                const bool seen = n_of[c] >= 0 && sees(mask, n_of[c], j0 + R * ty + i) && (!p.k_docs || (doc[c] == doc_of[i] && doc[c] >= 0));
-                float prob;
-                dp[i][j] = any_slope(p, s[i][j], dp[i][j], bias, lse[c], delta[c], seen, prob);
-                w[(R * ty + i) * P + c] = prob;
+            for (int i = 0; i < RM; ++i) {
+                dp[i][j] -= less;
+                if (p.cap != 0.0f) dp[i][j] *= fmaf(-s[i][j], s[i][j], 1.0f);
+                s[i][j] = fmaf(s[i][j], unit, -level);
             }
+        }
+        if (p.slopes) {
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                const float2 there = place[RN * tx + j];
+                const float steep = slope[RN * tx + j];
+#pragma unroll
+                for (int i = 0; i < RM; ++i) s[i][j] -= steep * map_distance(here[i], there);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                s[i][j] = exp2_fast(s[i][j]);
+                dp[i][j] *= s[i][j];
+            }
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                const int c = RN * tx + j, id = p.k_docs ? doc[c] : 0, n = n_of[c];
+#pragma unroll
+                for (int i = 0; i < RM; ++i)
+                    if (n < 0 || !sees(mask, n, j0 + RM * ty + i) || id != doc_of[i] || id < 0) s[i][j] = dp[i][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+            for (int j = 0; j < RN; ++j) w[(RM * ty + i) * PN + RN * tx + j] = s[i][j];
         __syncthreads();
-        accumulate<R, NC, BT>(acc_v, w, dot, ty, tx, bad);
+        accumulate<RM, NC, BN>(acc_v, w, qot, ty, tx, bad);
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < R; ++i)
+        for (int i = 0; i < RM; ++i)
 #pragma unroll
-            for (int j = 0; j < R; ++j) w[(R * ty + i) * P + R * tx + j] = dp[i][j];
+            for (int j = 0; j < RN; ++j) w[(RM * ty + i) * PN + RN * tx + j] = dp[i][j];
+        tile.put(qot);
         __syncthreads();
-        accumulate<R, NC, BT>(acc_k, w, qt, ty, tx, bad);
+        if (!p.q_docs && r0 + BN < rows) fetch_q(r0 + BN);
+        accumulate<RM, NC, BN>(acc_k, w, qot, ty, tx, bad);
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int j = j0 + R * ty + i;
+    for (int i = 0; i < RM; ++i) {
+        const int j = j0 + RM * ty + i;
         if (j >= p.M) continue;
         const long long o = ((static_cast<long long>(b) * p.M + j) * p.hk + kh) * p.d;
 #pragma unroll
@@ -520,24 +662,56 @@ cudaError_t forward_one(const GlobalParams &p, cudaStream_t stream)
     return launch_any(global_any_forward_kernel<T, DP, RM, RN>, grid, smem, stream, p);
 }
 
+// Blocks of 128 rows, eight per thread, read shared memory half as often per multiplication as blocks of 64; they pay once they
+// fill the chip.
+bool any_fills(const GlobalParams &p, int rows, int block) { return 1LL * ((rows + block - 1) / block) * p.hk * p.B >= sm_count() * 3 / 4; }
+
 template <typename T, int DP>
 cudaError_t forward_width(const GlobalParams &p, cudaStream_t stream)
 {
     // sixteen rows or fewer (single tokens): a block of sixteen rows
     if (p.N * p.g <= 16) return forward_one<T, DP, 1, 4>(p, stream);
     if constexpr (DP > 128) return forward_one<T, DP, 2, 2>(p, stream);
-    else return forward_one<T, DP, 4, 4>(p, stream);
+    else return any_fills(p, p.N * p.g, 128) && p.splits == 1 ? forward_one<T, DP, 8, 4>(p, stream) : forward_one<T, DP, 4, 4>(p, stream);
 }
 
+template <int DP, int RM, int RN>
+constexpr size_t backward_shared()
+{
+    constexpr int BM = 16 * RM, BN = 16 * RN;
+    constexpr size_t smem = sizeof(float) * (2 * DP * (BM + 4) + DP * (BN + 4) + BM * (BN + 4) + 7 * BN + 2);
+    static_assert(smem <= 227 * 1024, "shared memory of a block");
+    return smem;
+}
+
+template <typename T, int DP, int RM, int RN>
+cudaError_t dq_one(const GlobalParams &p, cudaStream_t stream)
+{
+    return launch_any(global_any_dq_kernel<T, DP, RM, RN>, dim3((p.N * p.g + 16 * RM - 1) / (16 * RM), p.hk, p.B), backward_shared<DP, RM, RN>(), stream, p);
+}
+
+template <typename T, int DP, int RM, int RN>
+cudaError_t dkv_one(const GlobalParams &p, cudaStream_t stream)
+{
+    return launch_any(global_any_dkv_kernel<T, DP, RM, RN>, dim3((p.M + 16 * RM - 1) / (16 * RM), p.hk, p.B), backward_shared<DP, RM, RN>(), stream, p);
+}
+
+// Each pass has the largest blocks that fill the chip: 128 rows, 64 or 32.
 template <typename T, int DP>
 cudaError_t backward_width(const GlobalParams &p, cudaStream_t stream)
 {
-    constexpr int R = DP > 128 ? 2 : 4, BT = 16 * R;
-    constexpr size_t smem = sizeof(float) * (4 * DP * (BT + 4) + BT * (BT + 4) + 7 * BT + 2);
-    static_assert(smem <= 227 * 1024, "shared memory of a block");
-    cudaError_t err = launch_any(global_any_dq_kernel<T, DP, R>, dim3((p.N * p.g + BT - 1) / BT, p.hk, p.B), smem, stream, p);
-    if (err != cudaSuccess) return err;
-    return launch_any(global_any_dkv_kernel<T, DP, R>, dim3((p.M + BT - 1) / BT, p.hk, p.B), smem, stream, p);
+    if constexpr (DP > 128) {
+        const cudaError_t err = dq_one<T, DP, 2, 2>(p, stream);
+        return err != cudaSuccess ? err : dkv_one<T, DP, 2, 2>(p, stream);
+    } else {
+        const cudaError_t err = any_fills(p, p.N * p.g, 128)  ? dq_one<T, DP, 8, 4>(p, stream)
+                                : any_fills(p, p.N * p.g, 64) ? dq_one<T, DP, 4, 4>(p, stream)
+                                                              : dq_one<T, DP, 2, 4>(p, stream);
+        if (err != cudaSuccess) return err;
+        return any_fills(p, p.M, 128)  ? dkv_one<T, DP, 8, 4>(p, stream)
+               : any_fills(p, p.M, 64) ? dkv_one<T, DP, 4, 4>(p, stream)
+                                       : dkv_one<T, DP, 2, 4>(p, stream);
+    }
 }
 
 template <typename T>
