@@ -36,6 +36,8 @@ struct GlobalParams {
     const void *d_out;                  // [B, N, h, d]
     void *d_q, *d_k, *d_v;              // [B, N, h, d], [B, M, hk, d]
     float *delta;                       // [B, h, N] sum of d_out * out of a row
+    int head_splits;                    // blocks of dK and dV that share out the query heads of a key head; their parts are joined after
+    float *part_k, *part_v;             // [head_splits, B, M, hk, d]
     float *norms;                       // float16: the largest row norms of d_out and of v (rows with infinite or NaN values left out)
 };
 
@@ -96,6 +98,9 @@ __device__ __forceinline__ void store_result(const GlobalParams &p, long long at
     store_one<T>(out, x);
     if (sizeof(T) == 2 && p.low != nullptr) store_one<T>(static_cast<T *>(p.low) + at, x - DT<T>::rnd(x));
 }
+
+// Query heads (of the g that share a key head) of one of the blocks that share them out.
+__device__ __forceinline__ int first_head(const GlobalParams &p, int split) { return split * p.g / p.head_splits; }
 
 cudaError_t run_global_any_forward(const GlobalParams &p, int dtype, cudaStream_t stream);
 cudaError_t run_global_any_backward(const GlobalParams &p, int dtype, cudaStream_t stream);

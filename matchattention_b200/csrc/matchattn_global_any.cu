@@ -181,11 +181,14 @@ struct RowOf {
     int n, head;
 };
 
-__device__ __forceinline__ RowOf row_of(const GlobalParams &p, int kh, int r)
+// Row r of key head kh, of the g heads from h_begin on that are walked.
+__device__ __forceinline__ RowOf row_of(const GlobalParams &p, int kh, int r, int g, int h_begin)
 {
-    const int n = r / p.g;
-    return {n, kh * p.g + r - n * p.g};
+    const int n = r / g;
+    return {n, kh * p.g + h_begin + r - n * g};
 }
+
+__device__ __forceinline__ RowOf row_of(const GlobalParams &p, int kh, int r) { return row_of(p, kh, r, p.g, 0); }
 
 template <typename T>
 __device__ __forceinline__ const T *at(const void *base, const long long (&s)[3], int b, int n, int head)
@@ -498,7 +501,8 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
     float *lse = reinterpret_cast<float *>(place + BN), *delta = lse + BN, *slope = delta + BN;
     int *n_of = reinterpret_cast<int *>(slope + BN), *doc = n_of + BN, *range = doc + BN;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int j0 = blockIdx.x * BM, kh = blockIdx.y, b = blockIdx.z, rows = p.N * p.g;
+    const int j0 = blockIdx.x * BM, kh = blockIdx.y, b = blockIdx.z % p.B, split = blockIdx.z / p.B;
+    const int h_begin = first_head(p, split), g = first_head(p, split + 1) - h_begin, rows = p.N * g;
     const GlobalMask mask = global_mask(p, b);
     load_transposed<T, DP, BM>(kt, p.d, p.vec, [&](int r) -> const T * { return j0 + r < mask.len ? at<T>(p.k, p.ks, b, j0 + r, kh) : nullptr; });
     load_transposed<T, DP, BM>(vt, p.d, p.vec, [&](int r) -> const T * { return j0 + r < mask.len ? at<T>(p.v, p.vs, b, j0 + r, kh) : nullptr; });
@@ -524,12 +528,12 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
         }
         __syncthreads();
     }
-    const long long first = static_cast<long long>(query_begin(mask, j0)) * p.g;
+    const long long first = static_cast<long long>(query_begin(mask, j0)) * g;
     Tile<T, DP, BN> tile;
     const auto fetch_q = [&](int r0) {
         tile.fetch(p.d, p.vec, [&](int r) -> const T * {
             if (r0 + r >= rows) return nullptr;
-            const RowOf t = row_of(p, kh, r0 + r);
+            const RowOf t = row_of(p, kh, r0 + r, g, h_begin);
             return at<T>(p.q, p.qs, b, t.n, t.head);
         });
     };
@@ -540,7 +544,7 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
         bool any = true;
         if (tid < BN) {
             const bool in = r0 + tid < rows;
-            const RowOf t = row_of(p, kh, min(r0 + tid, rows - 1));
+            const RowOf t = row_of(p, kh, min(r0 + tid, rows - 1), g, h_begin);
             const long long row = (static_cast<long long>(b) * p.h + t.head) * p.N + t.n;
             place[tid] = map_place(t.n + mask.shift, p.width);
             lse[tid] = p.lse[row];
@@ -563,7 +567,7 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
         __syncthreads();
         tile.fetch(p.d, p.vec, [&](int r) -> const T * {
             if (r0 + r >= rows) return nullptr;
-            const RowOf t = row_of(p, kh, r0 + r);
+            const RowOf t = row_of(p, kh, r0 + r, g, h_begin);
             return static_cast<const T *>(p.d_out) + ((static_cast<long long>(b) * p.N + t.n) * p.h + t.head) * p.d;
         });
         float s[RM][RN] = {}, dp[RM][RN] = {};
@@ -576,7 +580,7 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
         if (p.cap != 0.0f) capped(s, p.scale / p.cap);
         const float unit = (p.cap != 0.0f ? p.cap : p.scale) * kLog2e;
         // (queries that stand before all of the tile's keys, or behind the last row, need the masks)
-        const bool whole = !p.q_docs && r0 + BN <= rows && j0 + BM <= key_end(mask, r0 / p.g);
+        const bool whole = !p.q_docs && r0 + BN <= rows && j0 + BM <= key_end(mask, r0 / g);
 #pragma unroll
         for (int j = 0; j < RN; ++j) {
             const int c = RN * tx + j;
@@ -637,8 +641,14 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
 #pragma unroll
         for (int c = 0; c < NC; ++c)
             if (tx + 16 * c < p.d) {
-                store_one<T>(static_cast<T *>(p.d_k) + o + tx + 16 * c, acc_k[i][c] * p.scale);
-                store_one<T>(static_cast<T *>(p.d_v) + o + tx + 16 * c, acc_v[i][c]);
+                if (p.head_splits > 1) {
+                    const long long part = static_cast<long long>(split) * p.B * p.M * p.hk * p.d + o + tx + 16 * c;
+                    p.part_k[part] = acc_k[i][c] * p.scale;
+                    p.part_v[part] = acc_v[i][c];
+                } else {
+                    store_one<T>(static_cast<T *>(p.d_k) + o + tx + 16 * c, acc_k[i][c] * p.scale);
+                    store_one<T>(static_cast<T *>(p.d_v) + o + tx + 16 * c, acc_v[i][c]);
+                }
             }
     }
 }
@@ -664,7 +674,10 @@ cudaError_t forward_one(const GlobalParams &p, cudaStream_t stream)
 
 // Blocks of 128 rows, eight per thread, read shared memory half as often per multiplication as blocks of 64; they pay once they
 // fill the chip.
-bool any_fills(const GlobalParams &p, int rows, int block) { return 1LL * ((rows + block - 1) / block) * p.hk * p.B >= sm_count() * 3 / 4; }
+bool any_fills(const GlobalParams &p, int rows, int block, int splits = 1)
+{
+    return 1LL * ((rows + block - 1) / block) * p.hk * p.B * splits >= sm_count() * 3 / 4;
+}
 
 template <typename T, int DP>
 cudaError_t forward_width(const GlobalParams &p, cudaStream_t stream)
@@ -693,7 +706,7 @@ cudaError_t dq_one(const GlobalParams &p, cudaStream_t stream)
 template <typename T, int DP, int RM, int RN>
 cudaError_t dkv_one(const GlobalParams &p, cudaStream_t stream)
 {
-    return launch_any(global_any_dkv_kernel<T, DP, RM, RN>, dim3((p.M + 16 * RM - 1) / (16 * RM), p.hk, p.B), backward_shared<DP, RM, RN>(), stream, p);
+    return launch_any(global_any_dkv_kernel<T, DP, RM, RN>, dim3((p.M + 16 * RM - 1) / (16 * RM), p.hk, p.B * p.head_splits), backward_shared<DP, RM, RN>(), stream, p);
 }
 
 // Each pass has the largest blocks that fill the chip: 128 rows, 64 or 32.
@@ -708,9 +721,9 @@ cudaError_t backward_width(const GlobalParams &p, cudaStream_t stream)
                                 : any_fills(p, p.N * p.g, 64) ? dq_one<T, DP, 4, 4>(p, stream)
                                                               : dq_one<T, DP, 2, 4>(p, stream);
         if (err != cudaSuccess) return err;
-        return any_fills(p, p.M, 128)  ? dkv_one<T, DP, 8, 4>(p, stream)
-               : any_fills(p, p.M, 64) ? dkv_one<T, DP, 4, 4>(p, stream)
-                                       : dkv_one<T, DP, 2, 4>(p, stream);
+        return any_fills(p, p.M, 128, p.head_splits)  ? dkv_one<T, DP, 8, 4>(p, stream)
+               : any_fills(p, p.M, 64, p.head_splits) ? dkv_one<T, DP, 4, 4>(p, stream)
+                                                      : dkv_one<T, DP, 2, 4>(p, stream);
     }
 }
 

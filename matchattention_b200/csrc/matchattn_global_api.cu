@@ -121,6 +121,23 @@ cudaError_t find_delta(const GlobalParams &p, bool wide, cudaStream_t stream)
                 : launch_chained(global_delta_kernel<T, 1>, grid, 256, 0, stream, p, lanes);
 }
 
+// dK and dV as the sums of their parts over the blocks that shared out the query heads, four elements per thread (one at the end).
+template <typename T>
+__global__ void __launch_bounds__(256) global_join_heads_kernel(const GlobalParams p)
+{
+    chain_begin();
+    const long long n = static_cast<long long>(p.B) * p.M * p.hk * p.d, i0 = (blockIdx.x * 256LL + threadIdx.x) * 4;
+    const float *part = blockIdx.y ? p.part_v : p.part_k;
+    T *to = static_cast<T *>(blockIdx.y ? p.d_v : p.d_k);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (i0 + e >= n) return;
+        float sum = 0.0f;
+        for (int s = 0; s < p.head_splits; ++s) sum += part[s * n + i0 + e];
+        store_one<T>(to + i0 + e, sum);
+    }
+}
+
 // What the ids of a block of 128 tokens span: blocks of queries of all items, then blocks of keys.
 __global__ void __launch_bounds__(kTile) global_ranges_kernel(const GlobalParams p, DocRange *ranges)
 {
@@ -308,7 +325,7 @@ GlobalParams params_of(const matchattn_global_args *a)
     p.slopes = a->slopes, p.prefix = a->prefix, p.lengths = a->lengths, p.q_docs = a->q_docs, p.k_docs = a->k_docs;
     p.B = a->B, p.N = a->N, p.M = a->M, p.h = a->h, p.hk = a->hk, p.g = a->h / a->hk, p.d = a->d;
     p.causal = a->causal != 0, p.width = a->width, p.scale = a->scale, p.cap = a->cap;
-    p.splits = 1;
+    p.splits = p.head_splits = 1;
     const size_t run = 4 * (a->dtype == MATCHATTN_F32 ? 4 : 2);
     bool vec = a->d % 4 == 0 && aligned(a->q, run) && aligned(a->k, run) && aligned(a->v, run);
     for (int i = 0; i < 3; ++i) vec = vec && a->q_stride[i] % 4 == 0 && a->k_stride[i] % 4 == 0 && a->v_stride[i] % 4 == 0;
@@ -316,9 +333,31 @@ GlobalParams params_of(const matchattn_global_args *a)
     return p;
 }
 
-// Scratch of the backward call: two norms, the documents of the tiles, delta.
+// Scratch of the backward call: two norms, the documents of the tiles, parts of dK and dV, delta.
 size_t backward_floats(const matchattn_global_args *a) { return static_cast<size_t>(a->B) * a->h * a->N; }
-size_t backward_bytes(const matchattn_global_args *a) { return 16 + range_count(a) * sizeof(DocRange) + sizeof(float) * backward_floats(a); }
+
+// Blocks that share out the query heads of a key head in the pass for dK and dV, where its tiles of 128 keys leave SMs idle.
+int head_splits(const matchattn_global_args *a)
+{
+    const int g = a->h / a->hk;
+    const long long blocks = 1LL * ((a->M + kTile - 1) / kTile) * a->hk * a->B;
+    if (g == 1 || blocks >= sm_count()) return 1;
+    long long s = (sm_count() * 3LL / 2 + blocks - 1) / blocks;
+    while (s > 1 && s * a->B > 65535) --s;
+    return static_cast<int>(s < g ? s : g);
+}
+
+size_t part_floats(const matchattn_global_args *a)
+{
+    const int s = head_splits(a);
+    return s > 1 ? static_cast<size_t>(s) * a->B * a->M * a->hk * a->d : 0;
+}
+
+// (the parts come before delta, on 16 bytes)
+size_t backward_bytes(const matchattn_global_args *a)
+{
+    return 16 + range_count(a) * sizeof(DocRange) + sizeof(float) * (2 * ((part_floats(a) + 3) / 4 * 4) + backward_floats(a));
+}
 
 }  // namespace
 }  // namespace matchattn
@@ -386,7 +425,10 @@ extern "C" int matchattn_global_backward(const matchattn_global_args *a, const v
     p.vec = p.vec && aligned(d_out, 4 * size);
     p.d_out = d_out, p.d_q = d_q, p.d_k = d_k, p.d_v = d_v;
     DocRange *ranges = reinterpret_cast<DocRange *>(static_cast<char *>(scratch) + 16);
-    p.delta = reinterpret_cast<float *>(ranges + range_count(a));
+    p.head_splits = head_splits(a);
+    p.part_k = reinterpret_cast<float *>(ranges + range_count(a));
+    p.part_v = p.part_k + (part_floats(a) + 3) / 4 * 4;
+    p.delta = p.part_v + (part_floats(a) + 3) / 4 * 4;
     const bool matrix = matrix_call(a) && aligned(d_out, 16) && aligned(d_q, 16) && aligned(d_k, 16) && aligned(d_v, 16);
     cudaError_t err = cudaSuccess;
     if (matrix && a->dtype == MATCHATTN_F16) {
@@ -405,6 +447,10 @@ extern "C" int matchattn_global_backward(const matchattn_global_args *a, const v
         if (err == cudaSuccess) err = a->dtype == MATCHATTN_F16 ? run_global_backward<__half>(p, maps, stream) : run_global_backward<__nv_bfloat16>(p, maps, stream);
     } else if (err == cudaSuccess) {
         err = run_global_any_backward(p, a->dtype, stream);
+    }
+    if (err == cudaSuccess && p.head_splits > 1) {
+        const unsigned blocks = static_cast<unsigned>((static_cast<size_t>(a->B) * a->M * a->hk * a->d + 1023) / 1024);
+        err = by_type(a->dtype, [&](auto t) { return launch_chained(global_join_heads_kernel<decltype(t)>, dim3(blocks, 2), 256, 0, stream, p); });
     }
     return status_of(err);
 }

@@ -51,7 +51,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
     BackShared<DP> &sh = *reinterpret_cast<BackShared<DP> *>(raw_shared + (1024 - (shared_address(raw_shared) & 1023)) % 1024);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int heads = KEYS ? p.hk : p.h;
-    const int lot = p.B * heads, turn = blockIdx.x / lot, b = blockIdx.x % lot / heads, own = blockIdx.x % lot % heads, kh = KEYS ? own : own / p.g;
+    const int each = p.B * heads, lot = KEYS ? each * p.head_splits : each;
+    const int turn = blockIdx.x / lot, split = blockIdx.x % lot / each, b = blockIdx.x % each / heads, own = blockIdx.x % each % heads, kh = KEYS ? own : own / p.g;
     // causal: the first keys are seen by most queries, the last queries see most keys: their blocks begin first
     const int f0 = (KEYS ? turn : gridDim.x / lot - 1 - turn) * kTile;
     const GlobalMask mask = global_mask(p, b);
@@ -62,7 +63,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         const int n0 = KEYS ? t * kTile : f0, j0 = KEYS ? f0 : t * kTile;
         return tile_state(mask, p.N, n0, j0, qr ? qr + n0 / kTile : nullptr, kr ? kr + j0 / kTile : nullptr);
     };
-    const int rounds = KEYS ? p.g : 1;                     // heads that are walked
+    // heads that are walked
+    const int r_begin = KEYS ? first_head(p, split) : 0, rounds = KEYS ? first_head(p, split + 1) : 1;
     const int t_begin = KEYS ? min(query_begin(mask, f0), p.N) / kTile : 0;
     const int t_end = KEYS ? query_tiles : (key_limit(mask, min(f0 + kTile, p.N) - 1) + kTile - 1) / kTile;
 
@@ -99,7 +101,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
             load_tile<DP>(sh.fixed[1], KEYS ? &maps.v : &maps.o, own, f0, b, &sh.fixed_full);
             int i = 0;
             bool good = true;
-            for (int r = 0; r < rounds && good; ++r)
+            for (int r = r_begin; r < rounds && good; ++r)
                 for (int t = t_begin; t < t_end; ++t) {
                     if (state(t) == kHidden) continue;
                     const int s = i % STAGES, head = KEYS ? kh * p.g + r : kh;
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 if (!*static_cast<volatile int *>(&sh.by_hand[1])) add_up(sum_k, slopes, moving(by_row, n, 0), n > 0);
                 products_done(&sh.empty[n % STAGES]);
             };
-            for (int r = 0; r < rounds && good; ++r)
+            for (int r = r_begin; r < rounds && good; ++r)
                 for (int t = t_begin; t < t_end && good; ++t) {
                     if (state(t) == kHidden) continue;
                     good = barrier_wait(&sh.full[i % STAGES], (i / STAGES) & 1, &sh.broken);
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 if (++t >= t_end) t = t_begin, ++r;
             } while (r < rounds && state(t) == kHidden);
         };
-        int i = 0, looks = 0, stores = 0, r = 0, t = t_begin - 1;
+        int i = 0, looks = 0, stores = 0, r = r_begin, t = t_begin - 1;
         bool good = true;
         if (t_begin < t_end) advance(r, t);
         else r = rounds;
@@ -374,7 +376,16 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 for (int e = 0; e < 32; ++e) y[e] = good ? __uint_as_float(raw[e]) * times : NAN;
 #pragma unroll
                 for (int e = 0; e < 32; e += 8)
-                    if (c + e < p.d) store_eight<T>(to + c + e, y + e);
+                    if (c + e < p.d) {
+                        if (KEYS && p.head_splits > 1) {
+                            float4 *part = reinterpret_cast<float4 *>((w < 2 ? p.part_v : p.part_k) +
+                                                                      (((static_cast<long long>(split) * p.B + b) * rows + f) * heads + own) * p.d + c + e);
+                            part[0] = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                            part[1] = make_float4(y[e + 4], y[e + 5], y[e + 6], y[e + 7]);
+                        } else {
+                            store_eight<T>(to + c + e, y + e);
+                        }
+                    }
             }
             __syncwarp();
         }
@@ -392,7 +403,7 @@ cudaError_t backward_pass(const GlobalParams &p, const GlobalMaps &maps, cudaStr
     const auto kernel = global_backward_kernel<T, DP, CAP, BIAS, KEYS>;
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (err != cudaSuccess) return err;
-    const dim3 grid(static_cast<unsigned>(p.B) * (KEYS ? p.hk : p.h) * (((KEYS ? p.M : p.N) + kTile - 1) / kTile));
+    const dim3 grid(static_cast<unsigned>(p.B) * (KEYS ? p.hk * p.head_splits : p.h) * (((KEYS ? p.M : p.N) + kTile - 1) / kTile));
     return launch_chained(kernel, grid, kBackThreads, smem, stream, p, maps);
 }
 

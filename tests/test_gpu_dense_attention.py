@@ -45,6 +45,7 @@ SHAPES = [  # B, N, M, h, hk, d
     (1, 1, 1, 1, 1, 1), (2, 1, 7, 4, 2, 8), (1, 5, 3, 2, 2, 16), (2, 63, 65, 2, 1, 24), (1, 129, 127, 3, 3, 32), (1, 257, 384, 4, 1, 64),
     (2, 130, 130, 2, 2, 40), (1, 300, 261, 2, 2, 128), (1, 128, 128, 2, 1, 80), (1, 70, 90, 2, 1, 17), (1, 140, 150, 2, 2, 129),
     (1, 33, 200, 2, 1, 256), (1, 513, 640, 1, 1, 96),
+    (40, 140, 150, 4, 2, 64), (1, 200, 190, 12, 2, 64), (75, 20, 140, 3, 1, 20),
 ]
 
 
