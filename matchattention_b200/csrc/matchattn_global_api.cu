@@ -5,7 +5,7 @@ namespace matchattn {
 namespace {
 
 // out = sum over the splits of 2^(lse_s - lse) * part_s: a warp per row of a head.  Reads the parts once (float32), bound by
-// their latency: a row has few of them.
+// their latency: 256 rows of ten shares 9 us with a branch between a share's figure and its part.  At most 64 shares.
 template <typename T>
 __global__ void __launch_bounds__(256) global_join_kernel(const GlobalParams p)
 {
@@ -14,17 +14,23 @@ __global__ void __launch_bounds__(256) global_join_kernel(const GlobalParams p)
     const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
     if (row >= rows) return;
     const int lane = threadIdx.x & 31;
-    float top = -INFINITY;
-    for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_lse[s * rows + row]);
+    // a lane has the figures of up to two shares; one that holds no key that the row sees has minus infinity, and zeros
+    float x[2], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        x[i] = lane + 32 * i < p.splits ? p.part_lse[(lane + 32 * i) * rows + row] : -INFINITY;
+        top = fmaxf(top, x[i]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.0f, acc[8] = {};
     const float ref = top == -INFINITY ? 0.0f : top;
+    x[0] = exp2f(x[0] - ref), x[1] = exp2f(x[1] - ref);
+    float sum = x[0] + x[1], acc[8] = {};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
-        const float x = p.part_lse[s * rows + row];
-        if (x == -INFINITY) continue;          // that share of the keys holds none that the row sees
-        const float w = exp2f(x - ref);
-        sum += w;
+        const float w = __shfl_sync(0xffffffffu, s < 32 ? x[0] : x[1], s & 31);
         const float *part = p.part_out + (s * rows + row) * p.d;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -239,8 +245,9 @@ Plan plan_forward(const matchattn_global_args *a)
     if (p.token) {
         blocks = 1LL * a->hk * a->B;
         tiles = (a->M + kTile - 1) / kTile;
-        // several blocks per SM one after another, because caches are filled unevenly, of four runs of keys per warp at least
-        const long long most = tiles / 4, wanted = (4LL * sm_count() + blocks - 1) / blocks;
+        // two blocks per SM, of eight runs of keys per warp at least.  8 items of 2048 to 8192 keys, 32 heads on 8 key heads x 128, bf16,
+        // with the join: two blocks per SM 52 us, four 60, eight 69
+        const long long most = tiles / 4, wanted = (2LL * sm_count() + blocks - 1) / blocks;
         p.splits = static_cast<int>(wanted < most ? wanted : most);
         if (p.splits > 64) p.splits = 64;
     } else if (p.matrix) {

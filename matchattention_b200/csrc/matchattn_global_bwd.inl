@@ -17,6 +17,10 @@
 // float16 has few exponents: P is held times 2^12 (P of a row of 10^5 tokens is not subnormal), dS times the power of two that
 // brings the largest value that row norms of dO and V allow, |dS| <= 2 |dO| |V|, to between 2^14 and 2^15; both leave the sums exactly.
 //
+// Measured, one B200: 2 x 4096 tokens, 16 heads x 128 on 4 key heads, bfloat16, causal and capped 369 us (dK, dV) and 323 us (dQ); 8160
+// tokens, 8 heads x 16, float16, map bias 681 and 560.  Bound by the steps that a tile goes through one after another (scores, P,
+// dP, dS); with eight warps of 64 rows each and the rows' figures fetched within the tile 497 + 407 and 843 + 650.
+//
 // As in the forward pass, tiles that are partly hidden are looked through for infinite and NaN values, and added term by term
 // where they have some.
 #include "matchattn_global_mma.cuh"

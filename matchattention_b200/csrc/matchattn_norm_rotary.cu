@@ -12,8 +12,11 @@
 //
 // Bound by memory: x in, y out (backward: x, dy in, dx out).  A group of lanes owns a token's row of a head: a lane holds V
 // channels and the V they are paired with, so the rotation stays in the lane, a row is read once, and mean and rotation work from
-// registers; V channels are one load of up to 16 bytes.  The group takes several heads of its token in turn, because the angles (a
-// sincospif per pair, as many instructions as a head's row altogether) are the token's.  All sums are float32, results are rounded once.
+// registers; V channels are one load of up to 16 bytes, and the next row is on its way while one is computed.  The groups of a warp take
+// heads of the same token side by side and in turn: a head's rows are one run of memory, and the token's angles (a sincospif per pair,
+// as many instructions as a head's row altogether) are formed once, each group a share.  All sums are float32, results are
+// rounded once.  Measured, one B200: 16384 tokens, 40 heads x 128, bfloat16 69 us (4.9 TB/s), backward 106 us (4.7 TB/s) and 6 for the
+// weights; 384 x 384 tokens, 16 heads x 16, float16 55 us (2.7 TB/s; 511 instructions per warp and row, issue 68 %).
 // The weights' gradients are summed per lane over the rows of a block, then over the block, then over the blocks by a second
 // kernel, always in the same order: no atomics.
 #include "matchattn_kernels.cuh"
