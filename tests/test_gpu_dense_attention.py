@@ -249,6 +249,32 @@ def test_small_gradients_in_float16():
         assert_within(g, w, b + 2.0 ** -25, name)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("N", [1, 130])
+def test_offsets_beyond_32_bits(N, dtype):
+    """A cache of 2^31 values and more: zeros (scores of 0, values of 0) but for its first and last keys, whose share of every
+    row is known: 2^24 - 64 exponentials of 0 beside theirs."""
+    M, d, n = 2 ** 24, 129 if dtype == torch.float32 else 128, 32
+    q = make(22, 1, N, 1, 1, 1, d, dtype)[0]
+    k, v = torch.zeros(2, 1, M, 1, d, dtype=dtype, device="cuda")
+    ends = make(23, 1, 1, 2 * n, 1, 1, d, dtype)
+    for cache, x, by in ((k, ends[1], 4.0), (v, ends[2], 1.0)):
+        cache[:, :n], cache[:, -n:] = x[:, :n] * by, x[:, n:] * by
+    some = [torch.cat((c[:, :n], c[:, -n:]), 1)[0, :, 0].double() for c in (k, v)]
+    x = q[0, :, 0].double() @ some[0].T * d ** -0.5
+    top = x.amax(-1, keepdim=True).clamp_min(0)
+    p = torch.exp(x - top)
+    p = p / (p.sum(-1, keepdim=True) + (M - 2 * n) * torch.exp(-top))
+    got = ma().global_attention(q, k, v)[0, :, 0].double()
+    want = p @ some[1]
+    # probabilities off by u and by their exponents' 2 (d + 16) f |q||k|, the sum of 2^24 of them by 2^24 / 64 steps of 2^-24 at most
+    # (a thread adds 64 of a tile before they meet a running sum), and u of the result
+    u = torch.finfo(dtype).eps / 2
+    far = 2 * (d + 16) * _dense.F * (q[0, :, 0].double().abs() @ some[0].T.abs() * d ** -0.5).amax(-1, keepdim=True)
+    bound = (far + u + 2.0 ** -6) * (p @ some[1].abs()) + u * want.abs() + 2.0 ** -24
+    assert_within(got, want, bound, "out")
+
+
 def test_empty_calls():
     for B, N, M in ((0, 4, 4), (2, 0, 5), (2, 3, 0)):
         q, k, v, dout = make(14, B, N, M, 4, 2, 16, torch.float16)
