@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                             if (now == kPartial) {
                                 bool seen = KEYS ? at >= bar : at < bar;
                                 if (p.q_docs) seen = seen && element(docs, u) == doc;
-                                value[u] = seen ? value[u] : -INFINITY;
+                                // (a hidden score may be NaN, and so its tanh)
+                                if (!seen) value[u] = -INFINITY, slant = 1.0f;
                             }
                             value[u] = exp2_fast(value[u]);
                             prob[at] = CAP ? value[u] * slant : value[u];

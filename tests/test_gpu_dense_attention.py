@@ -129,7 +129,8 @@ def test_values_in_masked_places_do_not_matter(N, d, dtype):
     clean = make(7, B, N, M, h, hk, d, dtype)
     q, k, v, dout = (t.clone() for t in clean)
     k[0, 205:], v[0, 205:] = float("nan"), float("inf")
-    for options in (dict(causal=True, lengths=ints([205, 333])), dict(lengths=ints([205, 333]))):
+    for options in (dict(causal=True, lengths=ints([205, 333])), dict(lengths=ints([205, 333])), dict(lengths=ints([205, 333]), cap=3.0),
+                    dict(causal=True, lengths=ints([205, 333]), slopes=slopes_of(h), width=11)):
         got, want = check((q, k, v, dout), options)
         assert all(bool(torch.isfinite(w).all()) for w in want)
     q, k, v, dout = (t.clone() for t in clean)
@@ -140,8 +141,9 @@ def test_values_in_masked_places_do_not_matter(N, d, dtype):
         docs_q[:, 150:160], docs_q[:, 160:] = -1, 1
         q[:, 150:160], dout[:, 150:160] = float("nan"), float("-inf")
     k[:, 100:130], v[:, 100:130] = float("inf"), float("nan")
-    got, want = check((q, k, v, dout), dict(documents=(docs_q, docs_k)))
-    assert all(bool(torch.isfinite(w).all()) for w in want)
+    for options in (dict(), dict(cap=3.0)):
+        got, want = check((q, k, v, dout), dict(documents=(docs_q, docs_k), **options))
+        assert all(bool(torch.isfinite(w).all()) for w in want)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
