@@ -38,7 +38,9 @@ struct GlobalParams {
     float *delta;                       // [B, h, N] sum of d_out * out of a row
     int head_splits;                    // blocks of dK and dV that share out the query heads of a key head; their parts are joined after
     float *part_k, *part_v;             // [head_splits, B, M, hk, d]
-    float *norms;                       // float16: the largest row norms of d_out and of v (rows with infinite or NaN values left out)
+    // float16, matrix kernels: per tile of 128 tokens of a head, the largest row norm of d_out and the largest delta, and of keys the largest
+    // row norm of v
+    float *level_o, *level_delta, *level_v;      // [B, h, query tiles] twice, [B, hk, key tiles]
 };
 
 // What an item's masks say.

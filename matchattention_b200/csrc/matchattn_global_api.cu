@@ -61,19 +61,15 @@ __device__ __forceinline__ void read_channels(const T *p, float (&x)[V])
 }
 
 // delta = sum over the channels of d_out * out (with what its rounding left): `lanes` lanes per row, V channels at a time (16 bytes, or
-// one element).  With `norms` also the largest norm of a row of d_out and, by the rows after those, of v (maxima do not depend on their
-// order).  Bound by memory; 2 x 4096 tokens, 16 heads x 128, bfloat16, by single elements and a warp per row 36 us.
+// one element).  Bound by memory; 2 x 4096 tokens, 16 heads x 128, bfloat16, by single elements and a warp per row 36 us.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) global_delta_kernel(const GlobalParams p, int lanes)
 {
     chain_begin();
-    const long long rows = static_cast<long long>(p.B) * p.N * p.h, more = p.norms ? static_cast<long long>(p.B) * p.M * p.hk : 0;
+    const long long rows = static_cast<long long>(p.B) * p.N * p.h;
     const long long row = static_cast<long long>(blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
     const int lane = threadIdx.x & (lanes - 1);
-    __shared__ int largest[2];
-    if (threadIdx.x < 2) largest[threadIdx.x] = 0;
-    __syncthreads();
-    float square = 0.0f, sum = 0.0f;
+    float sum = 0.0f;
     if (row < rows) {
         const T *o = static_cast<const T *>(p.out) + row * p.d, *g = static_cast<const T *>(p.d_out) + row * p.d;
         const T *low = p.low ? static_cast<const T *>(p.low) + row * p.d : nullptr;
@@ -83,35 +79,13 @@ __global__ void __launch_bounds__(256) global_delta_kernel(const GlobalParams p,
             read_channels<T, V>(g + c, y);
             if (low) read_channels<T, V>(low + c, z);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sum = fmaf(x[i], y[i], fmaf(z[i], y[i], sum));
-                square = fmaf(y[i], y[i], square);
-            }
-        }
-    } else if (row < rows + more) {
-        const long long bj = (row - rows) / p.hk, head = row - rows - bj * p.hk, b = bj / p.M, j = bj - b * p.M;
-        const T *v = static_cast<const T *>(p.v) + b * p.vs[0] + j * p.vs[1] + head * p.vs[2];
-        for (int c = lane * V; c < p.d; c += lanes * V) {
-            float x[V];
-            read_channels<T, V>(v + c, x);
-#pragma unroll
-            for (int i = 0; i < V; ++i) square = fmaf(x[i], x[i], square);
+            for (int i = 0; i < V; ++i) sum = fmaf(x[i], y[i], fmaf(z[i], y[i], sum));
         }
     }
-    for (int i = lanes / 2; i > 0; i >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, i);
-        square += __shfl_xor_sync(0xffffffffu, square, i);
-    }
+    for (int i = lanes / 2; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
     if (row < rows && lane == 0) {
         const long long bn = row / p.h, head = row - bn * p.h, b = bn / p.N, n = bn - b * p.N;
         p.delta[(b * p.h + head) * p.N + n] = sum;
-    }
-    if (p.norms) {
-        const float norm = sqrtf(square);
-        // floats that are not negative are ordered as their bits
-        if (lane == 0 && norm <= 3.402823466e38f) atomicMax(largest + (row >= rows), __float_as_int(norm));
-        __syncthreads();
-        if (threadIdx.x < 2 && largest[threadIdx.x] > 0) atomicMax(reinterpret_cast<int *>(p.norms) + threadIdx.x, largest[threadIdx.x]);
     }
 }
 
@@ -121,10 +95,77 @@ cudaError_t find_delta(const GlobalParams &p, bool wide, cudaStream_t stream)
     constexpr int V = 16 / sizeof(T);
     int lanes = 32;
     while (wide && lanes > 1 && lanes / 2 * V >= p.d) lanes /= 2;
-    const long long rows = 1LL * p.B * p.N * p.h + (p.norms ? 1LL * p.B * p.M * p.hk : 0);
+    const long long rows = 1LL * p.B * p.N * p.h;
     const dim3 grid(static_cast<unsigned>((rows + 256 / lanes - 1) / (256 / lanes)));
     return wide ? launch_chained(global_delta_kernel<T, V>, grid, 256, 0, stream, p, lanes)
                 : launch_chained(global_delta_kernel<T, 1>, grid, 256, 0, stream, p, lanes);
+}
+
+// Whether some query sees key j of item b.  Without documents the last query sees every key there is.
+__device__ __forceinline__ bool key_seen(const GlobalParams &p, const GlobalMask &mask, int b, int j, int query_tiles)
+{
+    if (j >= mask.len) return false;
+    if (p.k_docs == nullptr) return true;
+    const int id = p.k_docs[static_cast<long long>(b) * p.M + j], first = query_begin(mask, j), own = j - mask.shift;
+    if (id < 0) return false;
+    const int *ids = p.q_docs + static_cast<long long>(b) * p.N;
+    // (mostly the query that stands at the key)
+    if (own >= first && own < p.N && ids[own] == id) return true;
+    for (int t = first / kTile; t < query_tiles; ++t) {
+        const DocRange r = p.ranges[b * query_tiles + t];
+        if (id < r.low || id > r.high) continue;
+        for (int n = max(first, t * kTile); n < min((t + 1) * kTile, p.N); ++n)
+            if (ids[n] == id) return true;
+    }
+    return false;
+}
+
+// float16: what bounds dS, per tile of 128 tokens of a head (level_o, level_delta, level_v): blocks of query tiles, then of key tiles, two
+// lanes to a row.  Only tokens that take part in a visible pair count (what is hidden has no say in how the rest is held), and of those only
+// finite figures: infinities and NaN reach the results whatever they are held by.  Bound by memory.
+__global__ void __launch_bounds__(2 * kTile) global_levels_kernel(const GlobalParams p)
+{
+    chain_begin();
+    const int query_tiles = (p.N + kTile - 1) / kTile, key_tiles = (p.M + kTile - 1) / kTile, query_blocks = p.B * p.h * query_tiles;
+    const bool keys = static_cast<int>(blockIdx.x) >= query_blocks;
+    const int i = keys ? blockIdx.x - query_blocks : blockIdx.x, tiles = keys ? key_tiles : query_tiles, heads = keys ? p.hk : p.h;
+    const int bh = i / tiles, row = (i - bh * tiles) * kTile + threadIdx.x / 2, b = bh / heads, head = bh - b * heads;
+    const __half *x = nullptr;
+    float square = 0.0f, delta = 0.0f;
+    if (keys) {
+        if (key_seen(p, global_mask(p, b), b, row, query_tiles)) x = static_cast<const __half *>(p.v) + b * p.vs[0] + row * p.vs[1] + head * p.vs[2];
+    } else if (row < p.N) {
+        const long long line = static_cast<long long>(bh) * p.N + row;
+        // (a query that sees nothing has an infinite lse)
+        if (p.lse[line] != INFINITY) {
+            x = static_cast<const __half *>(p.d_out) + ((static_cast<long long>(b) * p.N + row) * p.h + head) * p.d;
+            delta = fabsf(p.delta[line]);
+        }
+    }
+    if (x != nullptr)
+        for (int c = threadIdx.x % 2 * 8; c < p.d; c += 16) {
+            float y[8];
+            read_channels<__half, 8>(x + c, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) square = fmaf(y[e], y[e], square);
+        }
+    square += __shfl_xor_sync(0xffffffffu, square, 1);
+    float norm = sqrtf(square);
+    norm = norm <= 3.402823466e38f ? norm : 0.0f;
+    delta = delta <= 3.402823466e38f ? delta : 0.0f;
+    for (int o = 16; o > 1; o >>= 1) {
+        norm = fmaxf(norm, __shfl_xor_sync(0xffffffffu, norm, o));
+        delta = fmaxf(delta, __shfl_xor_sync(0xffffffffu, delta, o));
+    }
+    __shared__ float most[2][kTile / 16];
+    if (threadIdx.x % 32 == 0) most[0][threadIdx.x / 32] = norm, most[1][threadIdx.x / 32] = delta;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        float level = 0.0f;
+        for (int w = 0; w < kTile / 16; ++w) level = fmaxf(level, most[threadIdx.x][w]);
+        if (keys && threadIdx.x == 0) p.level_v[i] = level;
+        if (!keys) (threadIdx.x == 0 ? p.level_o : p.level_delta)[i] = level;
+    }
 }
 
 // dK and dV as the sums of their parts over the blocks that shared out the query heads, four elements per thread (one at the end).
@@ -340,7 +381,7 @@ GlobalParams params_of(const matchattn_global_args *a)
     return p;
 }
 
-// Scratch of the backward call: two norms, the documents of the tiles, parts of dK and dV, delta.
+// Scratch of the backward call: the documents of the tiles, parts of dK and dV, delta, in float16 the levels of the tiles.
 size_t backward_floats(const matchattn_global_args *a) { return static_cast<size_t>(a->B) * a->h * a->N; }
 
 // Blocks that share out the query heads of a key head in the pass for dK and dV, where its tiles of 128 keys leave SMs idle.
@@ -360,10 +401,18 @@ size_t part_floats(const matchattn_global_args *a)
     return s > 1 ? static_cast<size_t>(s) * a->B * a->M * a->hk * a->d : 0;
 }
 
+// float16: of the query tiles twice, of the key tiles once
+size_t query_levels(const matchattn_global_args *a) { return static_cast<size_t>(a->B) * a->h * ((a->N + kTile - 1) / kTile); }
+
+size_t level_floats(const matchattn_global_args *a)
+{
+    return a->dtype == MATCHATTN_F16 ? 2 * query_levels(a) + static_cast<size_t>(a->B) * a->hk * ((a->M + kTile - 1) / kTile) : 0;
+}
+
 // (the parts come before delta, on 16 bytes)
 size_t backward_bytes(const matchattn_global_args *a)
 {
-    return 16 + range_count(a) * sizeof(DocRange) + sizeof(float) * (2 * ((part_floats(a) + 3) / 4 * 4) + backward_floats(a));
+    return range_count(a) * sizeof(DocRange) + sizeof(float) * (2 * ((part_floats(a) + 3) / 4 * 4) + backward_floats(a) + level_floats(a));
 }
 
 }  // namespace
@@ -431,26 +480,26 @@ extern "C" int matchattn_global_backward(const matchattn_global_args *a, const v
     GlobalParams p = params_of(a);
     p.vec = p.vec && aligned(d_out, 4 * size);
     p.d_out = d_out, p.d_q = d_q, p.d_k = d_k, p.d_v = d_v;
-    DocRange *ranges = reinterpret_cast<DocRange *>(static_cast<char *>(scratch) + 16);
+    DocRange *ranges = static_cast<DocRange *>(scratch);
     p.head_splits = head_splits(a);
     p.part_k = reinterpret_cast<float *>(ranges + range_count(a));
     p.part_v = p.part_k + (part_floats(a) + 3) / 4 * 4;
     p.delta = p.part_v + (part_floats(a) + 3) / 4 * 4;
     const bool matrix = matrix_call(a) && aligned(d_out, 16) && aligned(d_q, 16) && aligned(d_k, 16) && aligned(d_v, 16);
-    cudaError_t err = cudaSuccess;
-    if (matrix && a->dtype == MATCHATTN_F16) {
-        p.norms = static_cast<float *>(scratch);
-        err = cudaMemsetAsync(scratch, 0, 16, stream);
-    }
-    // (the rows of v are read for the matrix kernels alone, which have them aligned)
     const bool wide = a->d % (16 / static_cast<int>(size)) == 0 && aligned(a->out, 16) && aligned(a->out_low, 16) && aligned(d_out, 16);
-    if (err == cudaSuccess) err = by_type(a->dtype, [&](auto t) { return find_delta<decltype(t)>(p, wide, stream); });
+    cudaError_t err = by_type(a->dtype, [&](auto t) { return find_delta<decltype(t)>(p, wide, stream); });
     if (err == cudaSuccess && matrix) {
         GlobalMaps maps{};
         const long long stride[3] = {1LL * a->N * a->h * a->d, 1LL * a->h * a->d, a->d};
         err = operand_maps(maps, a);
         if (err == cudaSuccess) err = tile_map(&maps.o, d_out, stride, a->B, a->N, a->h, a->d, a->dtype);
         if (err == cudaSuccess) err = find_ranges(p, ranges, stream);
+        if (err == cudaSuccess && a->dtype == MATCHATTN_F16) {
+            p.level_o = p.delta + backward_floats(a);
+            p.level_delta = p.level_o + query_levels(a);
+            p.level_v = p.level_delta + query_levels(a);
+            err = launch_chained(global_levels_kernel, dim3(static_cast<unsigned>(level_floats(a) - query_levels(a))), 2 * kTile, 0, stream, p);
+        }
         if (err == cudaSuccess) err = a->dtype == MATCHATTN_F16 ? run_global_backward<__half>(p, maps, stream) : run_global_backward<__nv_bfloat16>(p, maps, stream);
     } else if (err == cudaSuccess) {
         err = run_global_any_backward(p, a->dtype, stream);

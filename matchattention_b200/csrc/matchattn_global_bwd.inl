@@ -15,7 +15,9 @@
 // they form dS(i) it forms dV(i) and S(i+1).
 //
 // float16 has few exponents: P is held times 2^12 (P of a row of 10^5 tokens is not subnormal), dS times the power of two that
-// brings the largest value that row norms of dO and V allow, |dS| <= 2 |dO| |V|, to between 2^14 and 2^15; both leave the sums exactly.
+// brings the largest value that |dS| <= |dO| |V| + |delta| allows over the tiles that the block meets to between 2^14 and 2^15; both leave
+// the sums exactly.  The bound knows only tokens of visible pairs (global_levels_kernel): what is hidden, another item, another key
+// head, or a tile that the block never meets, however large, takes no digits from a sum.
 //
 // Measured, one B200: 2 x 4096 tokens, 16 heads x 128 on 4 key heads, bfloat16, causal and capped 369 us (dK, dV) and 323 us (dQ); 8160
 // tokens, 8 heads x 16, float16, map bias 681 and 560.  Bound by the steps that a tile goes through one after another (scores, P,
@@ -41,6 +43,7 @@ struct BackShared {
     uint64_t fixed_full, full[kStages], empty[kStages], s_full, p_full, dp_full, ds_full, done, looked, stored;
     uint32_t tmem;
     int broken, by_hand[2], odd[2][3];
+    float level[16];             // float16: what a warp has found of the bound of |dS|
 };
 
 // KEYS: the pass for dK and dV
@@ -72,6 +75,21 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
     const int t_begin = KEYS ? min(query_begin(mask, f0), p.N) / kTile : 0;
     const int t_end = KEYS ? query_tiles : (key_limit(mask, min(f0 + kTile, p.N) - 1) + kTile - 1) / kTile;
 
+    if (HALF && warp < 16) {
+        // the largest |dS| that the norms of the tiles allow
+        float most = 0.0f;
+        const int walk = t_end - t_begin;
+        for (long long e = tid; e < static_cast<long long>(rounds - r_begin) * walk; e += 512) {
+            const int r = r_begin + static_cast<int>(e / walk), t = t_begin + static_cast<int>(e % walk);
+            if (state(t) == kHidden) continue;
+            const long long query = (static_cast<long long>(b) * p.h + (KEYS ? kh * p.g + r : own)) * query_tiles + (KEYS ? t : f0 / kTile);
+            const long long key = (static_cast<long long>(b) * p.hk + kh) * key_tiles + (KEYS ? f0 / kTile : t);
+            most = fmaxf(most, fmaf(p.level_o[query], p.level_v[key], p.level_delta[query]));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (lane == 0) sh.level[warp] = most;
+    }
     if (tid == 0) {
         barrier_init(&sh.fixed_full, 1);
         for (int i = 0; i < STAGES; ++i) {
@@ -189,7 +207,9 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
         // dS is held times 2^(lift - kLift), the sums of dS times 2^-lift
         int lift = 0;
         if (HALF) {
-            const float bound = 2.0f * p.norms[0] * p.norms[1];
+            float bound = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) bound = fmaxf(bound, sh.level[e]);
             if (bound > 0.0f && bound <= 3.402823466e38f) lift = min(max(14 - ilogbf(bound), -60), 60);
         }
         const float hold = ldexpf(1.0f, lift) * (HALF ? 1.0f / 4096.0f : 1.0f);
