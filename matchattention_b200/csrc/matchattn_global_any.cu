@@ -174,7 +174,7 @@ __device__ __forceinline__ void capped(float (&s)[RA][RB], float inverse_cap)
 #pragma unroll
         for (int i = 0; i < RA; ++i)
 #pragma unroll
-            for (int j = 0; j < RB; ++j) s[i][j] = fabsf(s[i][j]) <= kSmallTanh ? tanh_small(s[i][j]) : tanh_of(2.0f * kLog2e * s[i][j]);
+            for (int j = 0; j < RB; ++j) s[i][j] = tanh_one(s[i][j]);
     }
 }
 

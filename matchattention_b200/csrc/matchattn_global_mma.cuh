@@ -290,8 +290,12 @@ __device__ __forceinline__ float tanh_small(float y)
     return y * fmaf(u, r, 1.0f);
 }
 
-// x[i] = tanh(x[i] * inverse_cap).  Scores are mostly well below their cap: where all of a warp's are, the polynomial leaves the two
-// special-function instructions of the other form out, which bound the kernels (16 a clock on an SM).
+// An element's form depends on the element alone: a result does not change with the other scores of a warp, hidden ones among them, and the
+// backward pass repeats the forward's.  The error stays relative to the score, however far the cap lies above it.
+__device__ __forceinline__ float tanh_one(float y) { return fabsf(y) <= kSmallTanh ? tanh_small(y) : tanh_of(2.0f * kLog2e * y); }
+
+// x[i] = tanh(x[i] * inverse_cap).  Scores are mostly well below their cap: where all of a warp's are, the other form's two
+// special-function instructions, which bound the kernels (16 a clock on an SM), are left out.
 template <int N>
 __device__ __forceinline__ void tanh_all(float *x, float inverse_cap)
 {
@@ -303,9 +307,8 @@ __device__ __forceinline__ void tanh_all(float *x, float inverse_cap)
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = tanh_small(x[i] * inverse_cap);
     } else {
-        const float inner = 2.0f * kLog2e * inverse_cap;
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = tanh_of(x[i] * inner);
+        for (int i = 0; i < N; ++i) x[i] = tanh_one(x[i] * inverse_cap);
     }
 }
 

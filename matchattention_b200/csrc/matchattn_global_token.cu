@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
     const int rows = p.N * p.g;
     const GlobalMask mask = global_mask(p, b);
     const T *keys = static_cast<const T *>(p.k) + b * p.ks[0] + kh * p.ks[2], *values = static_cast<const T *>(p.v) + b * p.vs[0] + kh * p.vs[2];
-    const float factor = p.scale * kLog2e, inner = p.cap != 0.0f ? 2.0f * factor / p.cap : 0.0f, outer = p.cap * kLog2e;
+    const float factor = p.scale * kLog2e, inverse_cap = p.cap != 0.0f ? p.scale / p.cap : 0.0f, outer = p.cap * kLog2e;
 
     // rows quad and quad + 8 of the sixteen
     int limit[2], doc[2];
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     float x = s[i][2 * r + e];
-                    x = p.cap != 0.0f ? outer * tanh_of(x * inner) : x * factor;
+                    x = p.cap != 0.0f ? outer * tanh_one(x * inverse_cap) : x * factor;
                     if (p.slopes) x = fmaf(-slope[r], map_distance(here[r], there), x);
                     s[i][2 * r + e] = j < limit[r] && j < j_end && id == doc[r] ? x : -INFINITY;
                 }

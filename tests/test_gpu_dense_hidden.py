@@ -91,3 +91,38 @@ def test_documents_of_unlike_gradients():
         want, bound = _dense.attention(part(q), part(k), part(v), dout=part(dout), causal=True)
         for name, g, w, e in zip(NAMES, got, want, bound):
             assert_within(part(g), w, e, f"{name} of document {i}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [1, 4, 200])
+@pytest.mark.parametrize("cap", [1e6, 1e4, 2.0])
+def test_caps_far_above_the_scores(cap, N, dtype):
+    """A cap costs no digits of scores below it: c tanh(x / c) is off by a few 2^-24 of x, so the bounds of calls without a cap hold."""
+    tensors = make(34, 2, N, 300, 4, 2, 64, dtype)
+    want, _ = _dense.attention(*tensors[:3], dout=tensors[3], cap=cap)
+    _, bound = _dense.attention(*tensors[:3], dout=tensors[3])
+    if cap == 2.0:
+        # the slope of the tanh and what it does to the other figures are in the bounds with a cap
+        bound[1:] = _dense.attention(*tensors[:3], dout=tensors[3], cap=cap)[1][1:]
+    for name, *three in zip(NAMES, step(tensors, dict(cap=cap)), want, bound):
+        assert_within(*three, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [1, 4, 200])
+@pytest.mark.parametrize("cap", [0.0, 4.0])
+def test_bits_do_not_depend_on_hidden_keys_or_other_queries(cap, N, dtype):
+    q, k, v, dout = make(35, 1, N, 333, 4, 2, 64, dtype)
+    q = q * 0.3         # (scores well below the cap, but for those that are changed)
+    options = dict(cap=cap, lengths=ints([300]), causal=True)
+    first = step((q, k, v, dout), options)
+    k2, v2 = k.clone(), v.clone()
+    k2[:, 300:], v2[:, 300:] = k[:, 300:] * 50, 1000.0
+    again = step((q, k2, v2, dout), options)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    if N > 1:
+        q2 = q.clone()
+        q2[:, 1] = q[:, 1] * 50
+        again = step((q2, k, v, dout), options)
+        rest = [n for n in range(N) if n != 1]
+        assert all(torch.equal(a[:, rest], b[:, rest]) for a, b in zip(first[:2], again[:2]))
