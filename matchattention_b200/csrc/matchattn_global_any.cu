@@ -9,7 +9,7 @@
 // step 1330, of which dK and dV 660 and dQ 405: slower than a library's products over a stored score matrix (855) at that size.
 //
 // A value that no row of a tile may see can still be infinite or NaN, and 0 * NaN is NaN: a tile that holds such a value is
-// accumulated term by term, leaving out the terms of weight zero.
+// accumulated term by term, leaving out the hidden terms.
 #include "matchattn_global_mma.cuh"
 
 #include <type_traits>
@@ -118,9 +118,9 @@ __device__ __forceinline__ void products(float (&s)[RA][RB], const float *a, con
     }
 }
 
-// acc[i][c] += sum over the K columns of w[RA * ty + i][column] * b[tx + 16 c][column]
-template <int RA, int NC, int K>
-__device__ __forceinline__ void accumulate(float (&acc)[RA][NC], const float *w, const float *b, int ty, int tx, bool bad)
+// acc[i][c] += sum over the K columns of w[RA * ty + i][column] * b[tx + 16 c][column]; with `bad` only over those that seen(i, column)
+template <int RA, int NC, int K, typename Seen>
+__device__ __forceinline__ void accumulate(float (&acc)[RA][NC], const float *w, const float *b, int ty, int tx, bool bad, Seen seen)
 {
     constexpr int P = K + 4;
     w += RA * ty * P;
@@ -145,7 +145,7 @@ __device__ __forceinline__ void accumulate(float (&acc)[RA][NC], const float *w,
 #pragma unroll
         for (int i = 0; i < RA; ++i) {
             const float x = w[i * P + j];
-            if (x == 0.0f) continue;
+            if (!seen(i, j)) continue;
 #pragma unroll
             for (int c = 0; c < NC; ++c) acc[i][c] = fmaf(x, b[16 * c * P + j], acc[i][c]);
         }
@@ -330,7 +330,10 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_forward_kernel(const G
         __syncthreads();
         const bool bad = __syncthreads_or(tile.put(kvt));
         if (!p.k_docs && t + 1 < t_end) fetch(p.k, p.ks, j0 + BN);
-        accumulate<RM, NC, BN>(acc, w, kvt, ty, tx, bad);
+        accumulate<RM, NC, BN>(acc, w, kvt, ty, tx, bad, [&](int i, int c) {
+            const int id = p.k_docs ? doc[c] : 0;
+            return sees(mask, n_of[i], j0 + c) && id == doc_of[i] && id >= 0;
+        });
     }
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
@@ -477,7 +480,10 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dq_kernel(const Global
         __syncthreads();
         const bool bad = __syncthreads_or(tile.put(kvt));
         if (!p.k_docs && j0 + BN < end) fetch(p.k, p.ks, j0 + BN);
-        accumulate<RM, NC, BN>(acc, w, kvt, ty, tx, bad);
+        accumulate<RM, NC, BN>(acc, w, kvt, ty, tx, bad, [&](int i, int c) {
+            const int id = p.k_docs ? doc[c] : 0;
+            return sees(mask, n_of[i], j0 + c) && id == doc_of[i] && id >= 0;
+        });
     }
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
@@ -584,6 +590,10 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
         const float unit = (p.cap != 0.0f ? p.cap : p.scale) * kLog2e;
         // (queries that stand before all of the tile's keys, or behind the last row, need the masks)
         const bool whole = !p.q_docs && r0 + BN <= rows && j0 + BM <= key_end(mask, r0 / g);
+        const auto seen = [&](int i, int c) {
+            const int id = p.k_docs ? doc[c] : 0, n = n_of[c];
+            return n >= 0 && sees(mask, n, j0 + RM * ty + i) && id == doc_of[i] && id >= 0;
+        };
 #pragma unroll
         for (int j = 0; j < RN; ++j) {
             const int c = RN * tx + j;
@@ -625,7 +635,7 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
 #pragma unroll
             for (int j = 0; j < RN; ++j) w[(RM * ty + i) * PN + RN * tx + j] = s[i][j];
         __syncthreads();
-        accumulate<RM, NC, BN>(acc_v, w, qot, ty, tx, bad);
+        accumulate<RM, NC, BN>(acc_v, w, qot, ty, tx, bad, seen);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < RM; ++i)
@@ -634,7 +644,7 @@ __global__ void __launch_bounds__(kAnyThreads) global_any_dkv_kernel(const Globa
         tile.put(qot);
         __syncthreads();
         if (!p.q_docs && r0 + BN < rows) fetch_q(r0 + BN);
-        accumulate<RM, NC, BN>(acc_k, w, qot, ty, tx, bad);
+        accumulate<RM, NC, BN>(acc_k, w, qot, ty, tx, bad, seen);
     }
 #pragma unroll
     for (int i = 0; i < RM; ++i) {

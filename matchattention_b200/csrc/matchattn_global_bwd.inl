@@ -44,6 +44,7 @@ struct BackShared {
     uint32_t tmem;
     int broken, by_hand[2], odd[2][3];
     float level[16];             // float16: what a warp has found of the bound of |dS|
+    int begin[16];               // the tile's first moving row, for the rare path (a register less)
 };
 
 // KEYS: the pass for dK and dV
@@ -264,6 +265,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     reinterpret_cast<float *>(sh.delta[warp])[lane] = next_delta;
                 }
                 if (p.q_docs) reinterpret_cast<int *>(sh.docs[warp])[lane] = next_doc;
+                if (lane == 0) sh.begin[warp] = t * kTile;
                 if (BIAS == kMapBias) {
                     const float2 at = map_place(KEYS ? m0 + lane + mask.shift : m0 + lane, p.width);
                     reinterpret_cast<float *>(sh.across[warp])[lane] = at.x;
@@ -281,6 +283,12 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 tmem_loaded32(raw);
                 const float from = here.y - static_cast<float>(KEYS ? m0 + mask.shift : m0);
                 const int bar = (KEYS ? first : limit) - m0;                    // keys: the moving rows from it on are seen; queries: those below
+                const auto seen_rows = [&] {
+                    const int tile0 = sh.begin[warp];
+                    const int *ids = KEYS ? p.q_docs : p.k_docs;
+                    if (ids != nullptr) ids += static_cast<long long>(b) * (KEYS ? p.N : p.M) + tile0;
+                    return KEYS ? SeenRows{first - tile0, p.N - tile0, ids, doc} : SeenRows{0, limit - tile0, ids, doc};
+                };
                 {
                     uint32_t packed[16];
                     if (CAP) tanh_all<32>(prob, inverse_cap);
@@ -309,8 +317,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                             if (now == kPartial) {
                                 bool seen = KEYS ? at >= bar : at < bar;
                                 if (p.q_docs) seen = seen && element(docs, u) == doc;
-                                // (a hidden score may be NaN, and so its tanh)
-                                if (!seen) value[u] = -INFINITY, slant = 1.0f;
+                                if (!seen) value[u] = -INFINITY;
                             }
                             value[u] = exp2_fast(value[u]);
                             prob[at] = CAP ? value[u] * slant : value[u];
@@ -337,7 +344,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     hand_k = __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[0][looks % 3]) != 0);
                     hand_v = KEYS && __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[1][looks % 3]) != 0);
                     ++looks;
-                    if (hand_v && w == 0) add_rows<T, DP, kPart>(sum_v + lanes, scores + lanes, sh.moving[s][1], i > 0);
+                    if (hand_v && w == 0) add_rows<T, DP, kPart>(sum_v + lanes, scores + lanes, sh.moving[s][1], i > 0, seen_rows());
                 }
                 if (tid == 0) sh.by_hand[0] = hand_v;
                 tmem_before();
@@ -359,10 +366,23 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                             const int at = e + u;
                             const float off = __uint_as_float(dp[e + u]) - (KEYS ? element(row_delta, u) : delta);
                             value[u] = prob[at] * (HALF ? off * hold : off);
-                            if (now == kPartial && prob[at] == 0.0f) value[u] = 0.0f;
                         }
                         packed[e / 2] = pack_two<T>(value[0], value[1]);
                         packed[e / 2 + 1] = pack_two<T>(value[2], value[3]);
+                    }
+                    if (now == kPartial) {
+                        // hidden pairs, whose figures may be NaN: zeros (in a loop of its own: within the one above it cost every tile 5 %)
+                        const int begin = (KEYS ? first : limit) - sh.begin[warp] - w * kPart;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            int4 docs;
+                            if (p.q_docs) docs = sh.docs[warp][e / 4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const bool seen = (KEYS ? e + u >= begin : e + u < begin) && (!p.q_docs || element(docs, u) == doc);
+                                if (!seen) packed[(e + u) / 2] &= u & 1 ? 0x0000ffffu : 0xffff0000u;
+                            }
+                        }
                     }
                     tmem_store16(my_slopes, packed);
                 }
@@ -373,7 +393,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     good = barrier_wait(&sh.stored, stores & 1, &sh.broken);
                     tmem_after();
                     ++stores;
-                    if (w == 1) add_rows<T, DP, kPart>(sum_k + lanes, slopes + lanes, sh.moving[i % STAGES][0], i > 0);
+                    if (w == 1) add_rows<T, DP, kPart>(sum_k + lanes, slopes + lanes, sh.moving[i % STAGES][0], i > 0, seen_rows());
                 }
                 if (tid == 0) sh.by_hand[1] = hand_k;
                 tmem_before();

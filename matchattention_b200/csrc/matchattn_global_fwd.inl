@@ -329,7 +329,10 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                 tmem_after();
                 hand = __any_sync(0xffffffffu, good && *static_cast<volatile int *>(&sh.odd[w][looks % 3]) != 0);
                 ++looks;
-                if (hand && half == 0) add_rows<T, DP, 64>(out, scores, sh.kv[s], used > 0);
+                if (hand && half == 0) {
+                    const int *ids = p.k_docs ? p.k_docs + static_cast<long long>(b) * p.M + t * kTile : nullptr;
+                    add_rows<T, DP, 64>(out, scores, sh.kv[s], used > 0, SeenRows{0, limit - t * kTile, ids, doc});
+                }
             }
             if (row == 0 && half == 0) sh.by_hand[w] = hand;
             tmem_before();

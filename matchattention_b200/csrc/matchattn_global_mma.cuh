@@ -365,11 +365,20 @@ __device__ __forceinline__ bool row_tainted(const uint8_t *tile, int row, int pa
     return tainted<T>(acc);
 }
 
-// The product of the weights in tensor memory (128 x 16 bits per row from `weights` on, RUN of them side by side in every RUN columns) and a tile's rows, added to the thread's row
-// of sums at `sums` term by term, leaving out the terms of weight zero: in place of the matrix instruction where the tile holds
-// infinite or NaN values that some rows do not see.  A warp's 32 rows; rare, and slow.
+// The rows of a tile that a thread's own row sees (or is seen by): those from `from` on, below `to`, and with documents of its id.
+struct SeenRows {
+    int from, to;
+    const int *ids;       // of the tile's rows, or null
+    int id;
+    __device__ __forceinline__ bool operator()(int j) const { return j >= from && j < to && (ids == nullptr || ids[j] == id); }
+};
+
+// The product of the weights in tensor memory (128 x 16 bits per row from `weights` on, RUN of them side by side in every RUN columns) and a
+// tile's rows, added to the thread's row of sums at `sums` term by term, leaving out the hidden terms (and no visible one, though its
+// weight may be zero): in place of the matrix instruction where the tile holds infinite or NaN values that some rows do not see.  A warp's
+// 32 rows; rare, and slow.
 template <typename T, int DP, int RUN>
-static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, const uint8_t *tile, bool add)
+static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, const uint8_t *tile, bool add, SeenRows seen)
 {
     for (int c = 0; c < DP; c += 8) {
         uint32_t raw[8] = {};
@@ -389,7 +398,7 @@ static __device__ __noinline__ void add_rows(uint32_t sums, uint32_t weights, co
                 const int row = j + e;
                 const uint4 y = *reinterpret_cast<const uint4 *>(tile + c / 64 * kHalfBytes + row * 128 + ((c % 64 / 8 ^ (row & 7)) << 4));
                 const uint32_t words[4] = {y.x, y.y, y.z, y.w};
-                if (x != 0.0f) {
+                if (seen(row)) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) acc[i] = fmaf(x, DT<T>::unpack(words[i / 2], i % 2), acc[i]);
                 }

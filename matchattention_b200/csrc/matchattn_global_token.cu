@@ -179,20 +179,24 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
                                     __byte_perm(word(value[c][2], t / 2), word(value[c][3], t / 2), pick));
                 }
         } else {
-            // values that are no numbers, and rows that do not see them: term by term, without the terms of weight zero
+            // values that are no numbers, and rows that do not see them: term by term, without the hidden terms (marked by -1)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) sh.prob[warp][quad + 8 * r][8 * i + 2 * part + e] = DT<T>::unpack(prob[2 * i + r], e);
+                    for (int e = 0; e < 2; ++e) {
+                        const int j = j0 + 8 * i + 2 * part + e;
+                        const bool seen = j < limit[r] && j < j_end && (p.k_docs == nullptr || p.k_docs[static_cast<long long>(b) * p.M + j] == doc[r]);
+                        sh.prob[warp][quad + 8 * r][8 * i + 2 * part + e] = seen ? DT<T>::unpack(prob[2 * i + r], e) : -1.0f;
+                    }
             __syncwarp();
             for (int e = 0; e < kRun && j0 + e < j_end; ++e) {
                 const T *row = values + static_cast<long long>(j0 + e) * p.vs[1];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const float x = sh.prob[warp][quad + 8 * r][e];
-                    if (x == 0.0f) continue;
+                    if (x < 0.0f) continue;
 #pragma unroll
                     for (int t = 0; t < GROUPS * 8; ++t)
 #pragma unroll

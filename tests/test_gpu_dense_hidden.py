@@ -126,3 +126,27 @@ def test_bits_do_not_depend_on_hidden_keys_or_other_queries(cap, N, dtype):
         again = step((q2, k, v, dout), options)
         rest = [n for n in range(N) if n != 1]
         assert all(torch.equal(a[:, rest], b[:, rest]) for a, b in zip(first[:2], again[:2]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [4, 200])
+@pytest.mark.parametrize("ahead", [60.0, 400.0])
+def test_a_value_that_is_seen_with_hardly_any_weight(ahead, N, dtype):
+    """A NaN value reaches all that see it, whatever the weight that the softmax leaves it: exp(-60) and exp(-400) of the largest
+    round to zero in float16, and in every type.  The other document stays as it is."""
+    M, h, d = 200, 2, 64
+    q, k, v, dout = make(36, 1, N, M, h, h, d, dtype)
+    documents = torch.zeros(1, M, dtype=torch.int32, device="cuda")
+    documents[:, M // 2:] = 1
+    if N < M:
+        documents[:, :] = 0
+    k[..., 0], q[..., 0] = 0.0, 8.0
+    k[:, 0, :, 0] = ahead            # with q's 8 and a scale of 1/8: ahead above the others
+    v[0, M - 3 if N < M else 5, 1, 3] = float("nan")
+    options = dict(causal=True, documents=(documents[:, M - N:].contiguous(), documents), scale=0.125)
+    want, bound = _dense.attention(q, k, v, dout=dout, **options)
+    got = step((q, k, v, dout), options)
+    assert bool(want[0].isnan().any()) and not bool(want[0].isnan().all())
+    for name, g, w in zip(NAMES, got, want):
+        assert torch.equal(g.isnan(), w.isnan()), name
+    assert_within(got[0], want[0], bound[0], "out")
