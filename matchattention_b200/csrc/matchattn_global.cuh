@@ -30,6 +30,7 @@ struct GlobalParams {
     // forward with few queries: each split takes a share of the keys, a second kernel joins them
     int splits, tiles_per_split;
     int block_rows;                     // matrix kernels: queries of a block
+    float held;                         // matrix kernels, float16: log2 of what probabilities are held by
     const DocRange *ranges;      // with documents: of the blocks of 128 queries, then of keys, item by item
     float *part_out, *part_lse;         // [splits, B, h, N, d], [splits, B, h, N]
     // backward

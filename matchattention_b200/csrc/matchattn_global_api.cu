@@ -256,6 +256,10 @@ int splits_of(long long blocks, int tiles, int B)
 // Queries times sharing heads up to which a call counts as one of single tokens: the rows of a warp's matrix instruction.
 constexpr int kTokenRows = 16;
 
+// Keys from which the matrix kernel holds float16 probabilities by more (matchattn_global_fwd.inl).  What a key's weight loses to rounding
+// is 2^-33 of the largest at most, of so many keys 2^-17: a thirty-second of a half step of the type, against the largest value.
+constexpr int kManyKeys = 1 << 16;
+
 bool matrix_call(const matchattn_global_args *a)
 {
     return a->dtype != MATCHATTN_F32 && a->d <= 128 && a->d % 8 == 0 && aligned(a->out, 16) && aligned(a->out_low, 16) && rows_fit(a->q, a->q_stride, a->B, a->N, a->h) &&
@@ -440,6 +444,7 @@ extern "C" int matchattn_global_forward(const matchattn_global_args *a, void *sc
     }
     const Plan plan = plan_forward(a);
     p.splits = plan.splits, p.tiles_per_split = plan.tiles_per_split, p.block_rows = plan.block_rows;
+    p.held = a->M < kManyKeys ? 7.0f : 11.0f;
     if (plan.bytes() != 0) {
         if (scratch == nullptr) return MATCHATTN_ERR_NULL;
         if (scratch_bytes < plan.bytes()) return MATCHATTN_ERR_SCRATCH_LIMIT;

@@ -8,7 +8,9 @@
 //
 // The softmax keeps a reference per row, not the running maximum itself: probabilities are taken with the reference as it stands,
 // and O, the sum and the probabilities only change to a new one when a score exceeds it by 2^8.  They stay below 2^8, O in
-// tensor memory is hardly ever touched between products, and nothing waits for a maximum.
+// tensor memory is hardly ever touched between products, and nothing waits for a maximum.  float16 has few exponents: P, the sum and O are
+// held times 2^7 there, the room that the type leaves above 2^8, and over keys without end, whose small weights add up, times 2^11,
+// with a reference that moves at 2^4 (for every call that would cost: 48 x 48 tokens with a map bias 62 us for 51).
 // P is rounded to the type of V (a half step of it, relative, as torch rounds a softmax's result); scores, reference, sums and O are
 // float32.  For training O is divided by the sum of the rounded probabilities: their errors then weigh differences of values and not
 // the values (8160 tokens of 8 heads x 16, float16: 2.8e-4 from the exact result, 2.9e-4 without), which the row sums of the backward
@@ -27,7 +29,6 @@ namespace matchattn {
 namespace {
 
 constexpr int kForwardThreads = 576;
-constexpr float kSlack = 8.0f;           // log2 of what a probability may exceed one by
 
 template <int DP>
 struct ForwardShared {
@@ -49,6 +50,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
     chain_begin();
     constexpr int STAGES = ForwardShared<DP>::kStages;
     constexpr bool GENERAL = CAP || BIAS != kNoBias;
+    // log2 of what P is held by, and of what it may exceed that by: together at most 2^15 in float16
+    const float held = std::is_same<T, __half>::value ? p.held : 0.0f, slack = std::is_same<T, __half>::value ? 15.0f - held : 8.0f;
     extern __shared__ uint8_t raw_shared[];
     ForwardShared<DP> &sh = *reinterpret_cast<ForwardShared<DP> *>(raw_shared + (1024 - (shared_address(raw_shared) & 1023)) % 1024);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -280,13 +283,13 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                 const float most = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
                 return GENERAL ? most : most * factor;
             };
-            float high = probabilities(ref == -INFINITY ? 0.0f : ref);
+            float high = probabilities((ref == -INFINITY ? 0.0f : ref) - held);
             // the two halves of a row agree on its largest score
             sh.high[used & 1][w][half][row] = high;
             warp_arrive(&sh.agreed[w][warp & 3]);
             good = barrier_wait(&sh.agreed[w][warp & 3], used & 1, &sh.broken);
             high = fmaxf(high, sh.high[used & 1][w][half ^ 1][row]);
-            const bool grown = high > ref + kSlack;
+            const bool grown = high > ref + slack;
             if (__any_sync(0xffffffffu, grown)) {
                 // (a row that has seen nothing so far has zeros in O and sum: any factor does)
                 const float shrink = grown ? (ref == -INFINITY ? 0.0f : exp2_fast(ref - high)) : 1.0f;
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
                         tmem_store32(out + c, o);
                     }
                 }
-                probabilities(ref == -INFINITY ? 0.0f : ref);
+                probabilities((ref == -INFINITY ? 0.0f : ref) - held);
             }
             tmem_store32(scores, packed);
             sum += part[0] + part[1];
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) global_forward_kernel(cons
         if (n0 + w * kTile < p.N && w < tiles) {          // whole warps
             const long long line = (static_cast<long long>(b) * p.h + head) * p.N + n;
             const long long part = static_cast<long long>(split) * p.B * p.h * p.N + line;
-            const float lse = ref + log2f(sum);
+            const float lse = ref + log2f(sum) - held;
             if (n < p.N && half == 0) {
                 if (p.splits > 1) p.part_lse[part] = empty ? -INFINITY : lse;
                 else if (p.lse) p.lse[line] = empty ? INFINITY : lse;

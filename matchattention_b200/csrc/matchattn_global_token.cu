@@ -15,13 +15,16 @@
 // keys, 8 heads x 64, float16 4.6 us.  255 registers hold 8 KB per warp on their way, eight warps per SM.
 //
 // Each warp keeps its own maximum, sum and output; the warps are joined in shared memory, the shares of the keys by a second
-// kernel.  Everything is float32 but the probabilities, which are rounded to the type for the product with V.
+// kernel.  Everything is float32 but the probabilities, which are rounded to the type for the product with V; in float16 they and their sum are
+// held times 2^15, the most that the type has room for: the many small weights of a long cache count.
 #include "matchattn_global_mma.cuh"
 
 namespace matchattn {
 namespace {
 
 constexpr int kTokenWarps = 4, kTokenThreads = 32 * kTokenWarps, kRun = 16;
+template <typename T>
+constexpr float kHeld = std::is_same<T, __half>::value ? 15.0f : 0.0f;
 
 template <typename T>
 __device__ __forceinline__ void warp_product(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -143,8 +146,9 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
             float high = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
             high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
             high = fmaxf(fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2)), top[r]);
-            base[r] = high == -INFINITY ? 0.0f : high;
-            const float shrink = exp2_fast(top[r] - base[r]);
+            const float ref = high == -INFINITY ? 0.0f : high;
+            const float shrink = exp2_fast(top[r] - ref);
+            base[r] = ref - kHeld<T>;
             top[r] = high;
             sum[r] *= shrink;
 #pragma unroll
@@ -246,10 +250,10 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
         const float result = empty ? 0.0f : x / total;
         if (p.splits > 1) {
             const long long at = static_cast<long long>(split) * p.B * p.h * p.N + line;
-            if (c == 0) p.part_lse[at] = empty ? -INFINITY : ref + log2f(total);
+            if (c == 0) p.part_lse[at] = empty ? -INFINITY : ref + log2f(total) - kHeld<T>;
             if (c < p.d) p.part_out[at * p.d + c] = result;
         } else {
-            if (c == 0 && p.lse) p.lse[line] = empty ? INFINITY : ref + log2f(total);
+            if (c == 0 && p.lse) p.lse[line] = empty ? INFINITY : ref + log2f(total) - kHeld<T>;
             if (c < p.d) store_result<T>(p, ((static_cast<long long>(b) * p.N + n) * p.h + head) * p.d + c, result);
         }
     }
