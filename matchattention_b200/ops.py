@@ -546,8 +546,10 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
     N == M, or a pair for queries and keys; a query sees keys of its own id, and a negative id sees and shows nothing.
     A query that sees no key gives zeros.  What no query sees, NaN included, does not reach a result.
 
-    Scores, softmax and sums are float32; 16-bit calls round the probabilities to the type for the product with v.  Equal calls
-    give equal bits."""
+    Scores, softmax and sums are float32.  16-bit calls round the probabilities to the type for the products with v and its gradient,
+    and the scores' gradients for theirs; calls of at most sixteen query rows per key head (N * h / hk) take the probabilities as two terms.
+    Equal calls give equal bits (a call that forms gradients divides by the sum of the rounded probabilities, and can differ from one
+    that does not in the last place)."""
     q_docs, k_docs = documents if isinstance(documents, (tuple, list)) and len(documents) == 2 else (documents, documents)
     if scale is None:
         scale = q.size(-1) ** -0.5

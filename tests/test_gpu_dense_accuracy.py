@@ -1,0 +1,34 @@
+"""global_attention: what a form keeps beyond the bounds that all forms share (_dense.py)."""
+import pytest
+import torch
+
+import _dense
+from _dense import assert_within
+
+pytestmark = pytest.mark.gpu
+HALVES = [torch.float16, torch.bfloat16]
+
+
+def ma():
+    import matchattention_b200
+    return matchattention_b200
+
+
+def make(seed, B, N, M, h, hk, d, dtype):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(shape, generator=gen).to(dtype).cuda() for shape in ((B, N, h, d), (B, M, hk, d), (B, M, hk, d), (B, N, h, d))]
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("N,h,hk", [(1, 8, 8), (1, 8, 2), (3, 4, 1)])
+def test_single_tokens_lose_nothing_to_rounded_probabilities(N, h, hk, d, dtype):
+    """Probabilities enter the product with v as two terms: float32's bounds, u of the result, and u^2 of the terms of a sum twice."""
+    u, last = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    for M in (1, 40, 700, 3000):
+        q, k, v, _ = make(41, 2, N, M, h, hk, d, dtype)
+        options = dict(lengths=torch.tensor([M, (M + 1) // 2], dtype=torch.int32, device="cuda"))
+        got = ma().global_attention(q, k, v, **options)
+        (want,), (bound,) = _dense.attention(q.float(), k.float(), v.float(), **options)
+        (terms,), _ = _dense.attention(q.float(), k.float(), v.float().abs(), **options)
+        assert_within(got, want, bound + u * want.abs() + 2 * u * u * terms + last, f"out over {M} keys")
