@@ -657,8 +657,12 @@ bool sized(const Tensor &t, at::ScalarType type, std::initializer_list<int64_t> 
     return !t.defined() || (t.scalar_type() == type && t.sizes() == at::IntArrayRef(shape.begin(), shape.size()) && t.is_contiguous());
 }
 
-// [B, N, h, d] of sizes that the entry points of the C ABI take (or empty)
-bool head_rows(const Tensor &t) { return t.dim() == 4 && dtype_code(t) >= 0 && t.size(3) > 0 && t.size(3) <= MATCHATTN_MAX_DENSE_D && t.size(2) > 0; }
+// [B, N, h, d] of sizes that the entry points of the C ABI take (or empty); theirs are 32-bit numbers
+bool head_rows(const Tensor &t)
+{
+    const auto fits = [&](int i) { return t.size(i) < (1LL << 31); };
+    return t.dim() == 4 && dtype_code(t) >= 0 && t.size(3) > 0 && t.size(3) <= MATCHATTN_MAX_DENSE_D && t.size(2) > 0 && fits(0) && fits(1) && fits(2);
+}
 
 // global_attention(q, k, v, scale, cap, slopes, width, causal, prefix, lengths, q_docs, k_docs) -> out
 PyObject *global_attention(PyObject *const *a, Py_ssize_t n)

@@ -506,6 +506,8 @@ def _head_rows(name: str, t):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected [items, tokens, heads, channels]")
     if t.size(2) < 1 or not 1 <= t.size(3) <= _lib.MAX_DENSE_D:
         raise ValueError(f"{name} has shape {tuple(t.shape)}: one head or more of 1 to {_lib.MAX_DENSE_D} channels")
+    if max(t.shape) >= 2 ** 31:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}: sizes below 2^31")
 
 
 def _aside(name: str, t, dtypes, shapes, like):
@@ -570,8 +572,8 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
     scale, cap, width = float(scale), float(cap), int(width)
     if not 0 < scale < float("inf") or not 0 <= cap < float("inf"):
         raise ValueError(f"scale must be positive and finite and cap 0 or positive and finite, got {scale} and {cap}")
-    if width < 1:
-        raise ValueError(f"width must be at least 1, got {width}")
+    if not 1 <= width < 2 ** 31:
+        raise ValueError(f"width must be at least 1 and below 2^31, got {width}")
     if prefix is not None and not causal:
         raise ValueError("prefix needs causal=True: without it every key is seen already")
     if slopes is not None and slopes.requires_grad:
