@@ -362,7 +362,8 @@ MATCHATTN_API int matchattn_flow_init(const void *correlation, void *prob, void 
  *   lse [B, h, N] float32, written: log2 of the sum of 2^(x log2 e) of a row, for the backward pass; may be NULL without one
  *   out_low [B, N, h, d], contiguous, written in 16-bit types: what the rounding of out left, for the backward pass, whose row sums
  *     of d_out * out would lose half their digits without it; may be NULL (not used in float32)
- *   d <= MATCHATTN_MAX_DENSE_D; 0 <= M <= 2^24; 0 < N <= 2^24; scale > 0; cap >= 0 (0: none); prefix needs causal.
+ *   d <= MATCHATTN_MAX_DENSE_D; 0 <= M <= 2^24; 0 < N <= 2^24; scale > 0; cap >= 0 (0: none), both and scale / cap between
+ *   2^-126 and 2.3e38; prefix needs causal.
  * Scores, softmax and sums are float32.  The sums do not depend on timing: equal calls give equal bits.
  */
 #define MATCHATTN_MAX_DENSE_D 256

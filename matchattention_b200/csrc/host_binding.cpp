@@ -664,6 +664,13 @@ bool head_rows(const Tensor &t)
     return t.dim() == 4 && dtype_code(t) >= 0 && t.size(3) > 0 && t.size(3) <= MATCHATTN_MAX_DENSE_D && t.size(2) > 0 && fits(0) && fits(1) && fits(2);
 }
 
+// scale, cap and their quotient within float32, as matchattn_global_forward has them
+bool scores_fit(double scale, double cap)
+{
+    constexpr double least = 0x1p-126, most = 2.3e38;
+    return scale >= least && scale <= most && (cap == 0.0 || (cap >= least && cap <= most && scale / cap >= least && scale / cap <= most));
+}
+
 // global_attention(q, k, v, scale, cap, slopes, width, causal, prefix, lengths, q_docs, k_docs) -> out
 PyObject *global_attention(PyObject *const *a, Py_ssize_t n)
 {
@@ -685,7 +692,7 @@ PyObject *global_attention(PyObject *const *a, Py_ssize_t n)
     const int64_t B = c.q.size(0), N = c.q.size(1), M = c.k.size(1);
     if (!sized(c.slopes, at::kFloat, {c.q.size(2)}) || (c.slopes.defined() && c.slopes.requires_grad()) || !sized(c.prefix, at::kInt, {B}) ||
         !sized(c.lengths, at::kInt, {B}) || c.q_docs.defined() != c.k_docs.defined() || !sized(c.q_docs, at::kInt, {B, N}) ||
-        !sized(c.k_docs, at::kInt, {B, M}) || (c.prefix.defined() && !c.causal) || !(c.scale > 0) || !(c.cap >= 0) || !std::isfinite(c.scale) || !std::isfinite(c.cap) || N > (1 << 24) || M > (1 << 24))
+        !sized(c.k_docs, at::kInt, {B, M}) || (c.prefix.defined() && !c.causal) || !scores_fit(c.scale, c.cap) || N > (1 << 24) || M > (1 << 24))
         return not_covered();
     Tensor out;
     {

@@ -226,8 +226,11 @@ int check_global(const matchattn_global_args *a)
     if (a->B <= 0 || a->N <= 0 || a->M < 0 || a->h <= 0 || a->hk <= 0 || a->h % a->hk != 0 || a->d <= 0 || a->d > MATCHATTN_MAX_DENSE_D ||
         a->width <= 0)
         return MATCHATTN_ERR_SHAPE;
-    // written so that NaN fails
-    if (!(a->scale > 0.0f && a->scale <= 3.402823466e38f && a->cap >= 0.0f && a->cap <= 3.402823466e38f)) return MATCHATTN_ERR_SHAPE;
+    // The kernels work with scale, cap and their quotient in units of log2: what these make infinite, zero or less than a normal number would
+    // give NaN, or another function.  (Written so that NaN fails.)
+    constexpr float least = 1.175494351e-38f, most = 3.402823466e38f / kLog2e;
+    if (!(a->scale >= least && a->scale <= most)) return MATCHATTN_ERR_SHAPE;
+    if (a->cap != 0.0f && !(a->cap >= least && a->cap <= most && a->scale / a->cap >= least && a->scale / a->cap <= most)) return MATCHATTN_ERR_SHAPE;
     if (a->prefix && !a->causal) return MATCHATTN_ERR_SHAPE;
     if (a->dtype < MATCHATTN_F32 || a->dtype > MATCHATTN_BF16) return MATCHATTN_ERR_DTYPE;
     const size_t size = a->dtype == MATCHATTN_F32 ? 4 : 2;

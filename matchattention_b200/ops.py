@@ -570,8 +570,10 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
     if h % hk:
         raise ValueError(f"{h} query heads cannot share {hk} key heads evenly")
     scale, cap, width = float(scale), float(cap), int(width)
-    if not 0 < scale < float("inf") or not 0 <= cap < float("inf"):
-        raise ValueError(f"scale must be positive and finite and cap 0 or positive and finite, got {scale} and {cap}")
+    least, most = 2.0 ** -126, 2.3e38
+    if not least <= scale <= most or not (cap == 0 or (least <= cap <= most and least <= scale / cap <= most)):
+        raise ValueError("scale must be positive, cap 0 or positive, and both and their quotient between 2^-126 and 2.3e38, "
+                         f"got {scale} and {cap}")
     if not 1 <= width < 2 ** 31:
         raise ValueError(f"width must be at least 1 and below 2^31, got {width}")
     if prefix is not None and not causal:
