@@ -554,7 +554,8 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
     that does not in the last place)."""
     q_docs, k_docs = documents if isinstance(documents, (tuple, list)) and len(documents) == 2 else (documents, documents)
     if scale is None:
-        scale = q.size(-1) ** -0.5
+        # (what has no channels is refused below)
+        scale = q.size(-1) ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.size(-1) else 1.0
     done = _host.global_attention(q, k, v, scale, cap, slopes, width, causal, prefix, lengths, q_docs, k_docs)
     if done is not None:
         return done
@@ -578,11 +579,11 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
         raise ValueError(f"width must be at least 1 and below 2^31, got {width}")
     if prefix is not None and not causal:
         raise ValueError("prefix needs causal=True: without it every key is seen already")
-    if slopes is not None and slopes.requires_grad:
-        raise NotImplementedError("slopes are constant: no gradient is formed for them")
     if (q_docs is None) != (k_docs is None):
         raise ValueError("documents are ids of the queries and of the keys, or of both at once")
     slopes = _aside("slopes", slopes, (torch.float32,), [(h,)], q)
+    if slopes is not None and slopes.requires_grad:
+        raise NotImplementedError("slopes are constant: no gradient is formed for them")
     prefix = _aside("prefix", prefix, (torch.int32,), [(B,)], q)
     lengths = _aside("lengths", lengths, (torch.int32,), [(B,)], q)
     q_docs = _aside("documents of the queries", q_docs, (torch.int32,), [(B, N)], q)

@@ -46,3 +46,19 @@ def test_the_largest_cap(dtype):
         got = ma().global_attention(q[:, :n], q, q, scale=0.25, cap=2.0 ** 123)
         # c tanh(x / c) is x then, but for an operation or two
         assert torch.allclose(got.float(), want.float(), rtol=2 * torch.finfo(dtype).eps, atol=2.0 ** -12)
+
+
+def test_arguments_that_are_no_tensors_or_have_no_channels():
+    q = torch.zeros(1, 2, 2, 16, device="cuda")
+    f = ma().global_attention
+    with pytest.raises(TypeError):
+        f("q", q, q)
+    with pytest.raises(TypeError):
+        f(q, None, q)
+    with pytest.raises(TypeError):
+        f(q, q, q, slopes=[0.5, 0.25])
+    for x in (q[..., :0], q[:, :, :0], torch.zeros((), device="cuda")):
+        with pytest.raises(ValueError):
+            f(x, x, x)
+        with pytest.raises(ValueError):
+            ma().norm_rotary(x)
