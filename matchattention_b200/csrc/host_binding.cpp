@@ -690,7 +690,7 @@ PyObject *global_attention(PyObject *const *a, Py_ssize_t n)
         c.k.size(3) != c.q.size(3) || c.q.size(2) % c.k.size(2) != 0 || c.width <= 0)
         return not_covered();
     const int64_t B = c.q.size(0), N = c.q.size(1), M = c.k.size(1);
-    if (!sized(c.slopes, at::kFloat, {c.q.size(2)}) || (c.slopes.defined() && c.slopes.requires_grad()) || !sized(c.prefix, at::kInt, {B}) ||
+    if (!sized(c.slopes, at::kFloat, {c.q.size(2)}) || (c.slopes.defined() && c.slopes.requires_grad() && at::GradMode::is_enabled()) || !sized(c.prefix, at::kInt, {B}) ||
         !sized(c.lengths, at::kInt, {B}) || c.q_docs.defined() != c.k_docs.defined() || !sized(c.q_docs, at::kInt, {B, N}) ||
         !sized(c.k_docs, at::kInt, {B, M}) || (c.prefix.defined() && !c.causal) || !scores_fit(c.scale, c.cap) || N > (1 << 24) || M > (1 << 24))
         return not_covered();

@@ -582,7 +582,7 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
     if (q_docs is None) != (k_docs is None):
         raise ValueError("documents are ids of the queries and of the keys, or of both at once")
     slopes = _aside("slopes", slopes, (torch.float32,), [(h,)], q)
-    if slopes is not None and slopes.requires_grad:
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("slopes are constant: no gradient is formed for them")
     prefix = _aside("prefix", prefix, (torch.int32,), [(B,)], q)
     lengths = _aside("lengths", lengths, (torch.int32,), [(B,)], q)
