@@ -19,6 +19,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/PyInterpreter.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -245,6 +246,23 @@ constexpr const char *kNormName = "matchattn_b200::norm_rotary_op";
 // A tensor whose channels lie side by side, as the kernels read them.
 Tensor with_rows(const Tensor &t) { return t.numel() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
+// Gradients as a backward pass leaves them.  The kernels' results carry no graph: where one is asked for (create_graph=True), a second
+// pass through them, to what they depend on, is an error, and not a term that is silently missing.
+torch::autograd::variable_list gradients(torch::autograd::variable_list results, const torch::autograd::variable_list &depend_on)
+{
+    if (!at::GradMode::is_enabled()) return results;
+    for (Tensor &t : results) {
+        if (!t.defined()) continue;
+        torch::autograd::variable_list inputs{t};
+        for (const Tensor &d : depend_on)
+            if (d.defined() && d.requires_grad()) inputs.push_back(d);
+        const auto refuse = std::make_shared<torch::autograd::DelayedError>(
+            "matchattn_b200: gradients of the gradients of global_attention and norm_rotary are not formed", inputs.size());
+        t = (*refuse)(std::move(inputs))[0];
+    }
+    return results;
+}
+
 template <typename P>
 P *data_as(const Tensor &t) { return t.defined() ? static_cast<P *>(t.data_ptr()) : nullptr; }
 
@@ -322,7 +340,7 @@ struct GlobalAttentionFn : torch::autograd::Function<GlobalAttentionFn> {
             check_status(matchattn_global_backward(&a, d_out.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), data_as<void>(scratch),
                                                    bytes, c10::cuda::getCurrentCUDAStream(out.device().index()).stream()));
         }
-        return {d_q, d_k, d_v, Tensor()};
+        return gradients({d_q, d_k, d_v, Tensor()}, {s[0], s[1], s[2], grads[0]});
     }
 };
 
@@ -406,7 +424,7 @@ struct NormRotaryFn : torch::autograd::Function<NormRotaryFn> {
                                                         data_as<void>(d_qw), data_as<void>(d_kw), data_as<void>(scratch), bytes,
                                                         c10::cuda::getCurrentCUDAStream(c.q.device().index()).stream()));
         }
-        return {d_q, d_k, d_qw, d_kw, Tensor()};
+        return gradients({d_q, d_k, d_qw, d_kw, Tensor()}, {s[0], s[1], s[2], s[3], grads[0], both ? grads[1] : Tensor()});
     }
 };
 

@@ -28,3 +28,22 @@ def test_slopes_that_train_elsewhere():
     for x in (q, q.clone().requires_grad_()):
         with pytest.raises(NotImplementedError):
             ma().global_attention(x, k, v, slopes=slopes)
+
+
+def test_second_derivatives_are_refused():
+    """Gradients with a graph are the same numbers; a second pass through them is an error, also where another term has one."""
+    for dtype in (torch.float32, torch.float16):
+        q, k, v, dout = (t.requires_grad_() for t in make((1, 40, 2, 16), (1, 50, 2, 16), (1, 50, 2, 16), (1, 40, 2, 16), dtype=dtype))
+        w = torch.ones(16, device="cuda", requires_grad=True)
+        calls = ((lambda: ma().global_attention(q, k, v), (q, k, v), dout), (lambda: ma().norm_rotary(q, q_weight=w), (q, w), dout))
+        for call, leaves, grad in calls:
+            want = torch.autograd.grad(call(), leaves, grad.detach())
+            got = torch.autograd.grad(call(), leaves, grad, create_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+            for g in got:
+                with pytest.raises(RuntimeError, match="gradients of the gradients"):
+                    torch.autograd.grad(g.float().square().sum() + q.float().square().sum(), q, retain_graph=True)
+        # a graph that does not lead back through the operator is left alone
+        loss = q.float().pow(3).sum()
+        (first,) = torch.autograd.grad(loss, q, create_graph=True)
+        assert torch.autograd.grad(first.float().sum(), q)[0].shape == q.shape
