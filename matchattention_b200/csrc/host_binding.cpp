@@ -670,6 +670,9 @@ bool optional_tensor(PyObject *o, const Tensor &like, Tensor &t)
     return cuda_tensor(o, t) && t.device() == like.device();
 }
 
+// Whether a tensor carries a tangent of forward-mode differentiation, which the kernels have no rule for.
+bool dual(const Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
+
 bool sized(const Tensor &t, at::ScalarType type, std::initializer_list<int64_t> shape)
 {
     return !t.defined() || (t.scalar_type() == type && t.sizes() == at::IntArrayRef(shape.begin(), shape.size()) && t.is_contiguous());
@@ -697,6 +700,7 @@ PyObject *global_attention(PyObject *const *a, Py_ssize_t n)
         !to_float(a[4], c.cap) || !optional_tensor(a[5], c.q, c.slopes) || !to_int(a[6], c.width) || !optional_tensor(a[8], c.q, c.prefix) ||
         !optional_tensor(a[9], c.q, c.lengths) || !optional_tensor(a[10], c.q, c.q_docs) || !optional_tensor(a[11], c.q, c.k_docs))
         return not_covered();
+    if (dual(c.q) || dual(c.k) || dual(c.v) || dual(c.slopes)) return not_covered();
     const int causal = PyObject_IsTrue(a[7]);
     if (causal < 0) {
         PyErr_Clear();
@@ -736,6 +740,7 @@ PyObject *norm_rotary(PyObject *const *a, Py_ssize_t n)
         !optional_tensor(a[3], c.q, c.positions) || !optional_tensor(a[4], c.q, c.q_weight) || !optional_tensor(a[5], c.q, c.k_weight) ||
         !to_float(a[6], c.eps) || !(c.eps >= 0) || !std::isfinite(c.eps) || !head_rows(c.q))
         return not_covered();
+    if (dual(c.q) || dual(c.k) || dual(c.q_weight) || dual(c.k_weight)) return not_covered();
     const int64_t B = c.q.size(0), N = c.q.size(1), d = c.q.size(3);
     if (c.k.defined() && (!head_rows(c.k) || c.k.scalar_type() != c.q.scalar_type() || c.k.size(0) != B || c.k.size(1) != N || c.k.size(3) != d))
         return not_covered();

@@ -527,6 +527,8 @@ def _eager_values(tensors):
     """Plain tensors with their values (for calls that a mode or a subclass kept from the extension)."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError("gradients are not available under tensor subclasses, modes and functional transforms")
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("tangents of forward-mode differentiation are not formed")
     return [t if t is None else (t.resolve_neg() if t.numel() == 0 or t.size(-1) == 1 or t.stride(-1) == 1 else t.contiguous().resolve_neg())
             for t in tensors]
 
@@ -591,7 +593,7 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
     again = _host.global_attention(q, k, v, scale, cap, slopes, width, bool(causal), prefix, lengths, q_docs, k_docs)
     if again is not None:
         return again
-    q, k, v = _eager_values((q, k, v))
+    q, k, v, slopes = _eager_values((q, k, v, slopes))
     out = q.new_empty(q.shape)
     if out.numel() == 0:
         return out

@@ -47,3 +47,45 @@ def test_second_derivatives_are_refused():
         loss = q.float().pow(3).sum()
         (first,) = torch.autograd.grad(loss, q, create_graph=True)
         assert torch.autograd.grad(first.float().sum(), q)[0].shape == q.shape
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation has no rule here: a dual tensor is refused, with and without gradients, and not stripped."""
+    import torch.autograd.forward_ad as forward_ad
+    q, k, v, t = make(*[(1, 9, 2, 16)] * 4)
+    w, tw = make((16,), (16,))
+    slopes, ts = make((2,), (2,))
+    with forward_ad.dual_level():
+        for name in ("q", "k", "v", "slopes"):
+            args = dict(q=q, k=k, v=v, slopes=slopes)
+            args[name] = forward_ad.make_dual(args[name], ts if name == "slopes" else t)
+            with pytest.raises(NotImplementedError):
+                ma().global_attention(**args)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                ma().global_attention(**args)
+        for args in (dict(q=forward_ad.make_dual(q, t)), dict(q=q, k=forward_ad.make_dual(k, t)), dict(q=q, q_weight=forward_ad.make_dual(w, tw))):
+            with pytest.raises(NotImplementedError):
+                ma().norm_rotary(**args)
+        # others that live in a dual level are not concerned
+        assert torch.equal(ma().norm_rotary(q), ma().norm_rotary(q.clone()))
+
+
+def test_transforms_and_modes_refuse_gradients():
+    """Under functional transforms and modes a gradient is refused, and inference under a mode gives the same numbers."""
+    from torch.overrides import TorchFunctionMode
+
+    class Mode(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    q, k, v = make(*[(1, 9, 2, 16)] * 3)
+    want = ma().global_attention(q, k, v)
+    with Mode():
+        assert torch.equal(ma().global_attention(q, k, v), want)
+        with pytest.raises(NotImplementedError):
+            ma().global_attention(q.clone().requires_grad_(), k, v)
+        with pytest.raises(NotImplementedError):
+            ma().norm_rotary(q.clone().requires_grad_())
+    for call in (lambda x: ma().global_attention(x, k, v).sum(), lambda x: ma().norm_rotary(x).sum()):
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.grad(call)(q)
