@@ -400,7 +400,8 @@ MATCHATTN_API int matchattn_global_backward(const matchattn_global_args *args, c
  *   q_weight, k_weight [d] in weight_dtype (float32 or dtype); NULL: ones
  *   positions: int32 or (positions_64) int64, [N, axes] for all items (positions_per_item 0) or [B, N, axes] (N * axes)
  *   freqs [rot/2]: turns per position in units of 2^-64, as 64-bit integers; with axes = 2 the first half belongs to the
- *     first coordinate of a position, the second half to the other (angles are exact to 2^-32 turns at any position)
+ *     first coordinate of a position, the second half to the other (angles are off by 2^-26 turns
+ *     at most, and by the table's own error times the position)
  *   d <= MATCHATTN_MAX_DENSE_D; rot <= d, a multiple of 2 * axes; rot = 0: no rotation (positions and freqs may be NULL)
  */
 typedef struct matchattn_norm_args {

@@ -5,8 +5,9 @@
 //   y[i + rot/2] = g[i + rot/2] cos(a_i) + g[i] sin(a_i)        channels from rot on: y = g
 //
 // The angle a_i is position * frequency.  A frequency is a 64-bit fraction of a turn per position: the product with the
-// position wraps at whole turns by itself, so what is left is exact to 2^-32 turns however far the position lies (a float32
-// product is off by 0.06 rad at position 10^6); its upper half goes to sincospif.
+// position wraps at whole turns by itself, so what is left is exact but for the table's rounding, 2^-65 turns per position, however far
+// that lies (a float32 product is off by 0.06 rad at position 10^6).  Its upper half goes to sincospif as a float32 of half turns: 2^-26
+// turns.
 //
 // Backward, from dy and x: dg = dy rotated back, dw = sum dg * u, e = dg * weight, dx = r (e - u mean(e u)).
 //

@@ -24,7 +24,7 @@ cover; the Python code here then handles the call or words the error.
 from __future__ import annotations
 
 import contextlib
-import math
+import decimal
 import os
 from typing import List, Optional, Tuple
 
@@ -610,6 +610,28 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
     return out
 
 
+def _turns(theta: float, n: int):
+    """theta ** (-j / n) / (2 pi) in units of 2^-64, right to half a unit (float64 would leave 2^-53 of it, far positions times as much)."""
+    digits = 60 + 2 * abs(decimal.Decimal(theta).adjusted())
+    one = 10 ** (digits + 10)
+
+    def arctan_of_inverse(x):       # in units of 1 / one, by its series
+        term = total = one // x
+        k = 1
+        while term:
+            term //= -x * x
+            k += 2
+            total += term // k
+        return total
+
+    with decimal.localcontext() as context:
+        context.prec = digits
+        context.Emax, context.Emin = decimal.MAX_EMAX, decimal.MIN_EMIN
+        pi = decimal.Decimal(4 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239))) / one        # Machin's formula
+        log = decimal.Decimal(theta).ln()
+        return [int(((-log * j / n).exp() * 2 ** 63 / pi).to_integral_value()) for j in range(n)]
+
+
 def rotary_frequencies(rot: int, theta: float = 10000.0, axes: int = 1, device=None) -> torch.Tensor:
     """The table of norm_rotary for ``rot`` rotated channels: ``theta ** (-j / n)`` radians per position, j < n = rot / 2 / axes, for
     each of the coordinates (1: sequences, 2: column and row of a map).  int64 [axes, n], turns per position in units of 2^-64
@@ -619,7 +641,7 @@ def rotary_frequencies(rot: int, theta: float = 10000.0, axes: int = 1, device=N
     if not 0 < theta < float("inf"):
         raise ValueError(f"theta must be positive and finite, got {theta}")
     n = rot // 2 // axes
-    turns = [round(theta ** (-j / n) / (2 * math.pi) * 2.0 ** 64) % 2 ** 64 for j in range(n)]
+    turns = [t % 2 ** 64 for t in _turns(float(theta), n)]
     row = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
     return torch.tensor([row] * axes, dtype=torch.int64, device=device).view(axes, n)
 
@@ -631,8 +653,8 @@ def norm_rotary(q, k=None, freqs=None, positions=None, *, q_weight=None, k_weigh
     q [B,N,h,d], k [B,N,hk,d] or None (any strides, as in global_attention); weights [d] in q's dtype or float32, or None (ones).
     ``freqs`` from rotary_frequencies(rot, axes=...) says how many channels turn: pairs ``(i, i + rot/2)`` by the angle of the token's
     position, channels from ``rot`` on are left as the norm gives them.  ``positions``: int32 or int64, [N] or [B,N], with two axes
-    [N,2] or [B,N,2] (column, row).  Without ``freqs`` and ``positions`` nothing turns.  Angles are exact to 2^-32 turns at any
-    position.  Returns (q, k), or q alone without k; contiguous, rounded once."""
+    [N,2] or [B,N,2] (column, row).  Without ``freqs`` and ``positions`` nothing turns.  Angles are off by 2^-26 turns
+    at most, and by what half a unit of the table makes over the position: 2^-65 turns each.  Returns (q, k), or q alone without k; contiguous, rounded once."""
     done = _host.norm_rotary(q, k, freqs, positions, q_weight, k_weight, eps)
     if done is not None:
         return done if k is not None else done[0]
