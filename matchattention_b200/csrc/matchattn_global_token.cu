@@ -15,10 +15,10 @@
 // keys, 8 heads x 64, float16 4.6 us.  255 registers hold 8 KB per warp on their way, eight warps per SM.
 //
 // Each warp keeps its own maximum, sum and output; the warps are joined in shared memory, the shares of the keys by a second
-// kernel.  Everything is float32 but the probabilities, which meet V as two terms of the type, rounded and what the rounding left (their
-// rounding alone would be the largest error of a call: 2.2e-3 of the result in bfloat16 for 1.7e-3; the second product costs the
-// eight caches above 53 us for 50.5); in float16 they and their sum are held times 2^15, the most that the type has room for: the many
-// small weights of a long cache count.
+// kernel.  Everything is float32 but the probabilities, which meet V as two terms of the type (rounded to it once they would make the largest
+// error of a call: 2.2e-3 of the result in bfloat16 for 1.7e-3).  Up to eight rows the second terms are the other eight rows of the
+// instruction, and cost nothing; beyond them they take a second one (32 heads on 8 key heads that way: 53 us for 50).  In float16 the
+// probabilities and their sum are held times 2^15, the most that the type has room for: the many small weights of a long cache count.
 #include "matchattn_global_mma.cuh"
 
 namespace matchattn {
@@ -39,6 +39,20 @@ __device__ __forceinline__ void warp_product(float (&d)[4], const uint32_t (&a)[
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x >= 0 in the type, rounded down, and what that left: not negative either, and for an x above 0 not zero, so that an infinite value meets
+// two terms of one sign (2^-24 in float16, where x is up to 2^15)
+template <typename T>
+__device__ __forceinline__ float cut(float x)
+{
+    if constexpr (std::is_same<T, __half>::value) return __half2float(__float2half_rz(x));
+    else return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+template <typename T>
+__device__ __forceinline__ float cut_off(float x)
+{
+    return x > 0.0f ? fmaxf(x - cut<T>(x), std::is_same<T, __half>::value ? 0x1p-24f : 0x1p-126f) : 0.0f;
 }
 
 __device__ __forceinline__ uint4 load_piece(const void *p, bool there)
@@ -65,6 +79,7 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, part = lane & 3;
     const int bk = blockIdx.x % (p.B * p.hk), split = blockIdx.x / (p.B * p.hk), b = bk / p.hk, kh = bk - b * p.hk;
     const int rows = p.N * p.g;
+    const bool few = rows <= 8;                 // rows 8 to 15 of the instruction have the second terms of the probabilities
     const GlobalMask mask = global_mask(p, b);
     const T *keys = static_cast<const T *>(p.k) + b * p.ks[0] + kh * p.ks[2], *values = static_cast<const T *>(p.v) + b * p.vs[0] + kh * p.vs[2];
     const float factor = p.scale * kLog2e, inverse_cap = p.cap != 0.0f ? p.scale / p.cap : 0.0f, outer = p.cap * kLog2e;
@@ -142,29 +157,32 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
                     s[i][2 * r + e] = j < limit[r] && j < j_end && id == doc[r] ? x : -INFINITY;
                 }
             }
-        float base[2];
+        float base[2], shrink[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             float high = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
             high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
             high = fmaxf(fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2)), top[r]);
             const float ref = high == -INFINITY ? 0.0f : high;
-            const float shrink = exp2_fast(top[r] - ref);
+            shrink[r] = exp2_fast(top[r] - ref);
             base[r] = ref - kHeld<T>;
             top[r] = high;
-            sum[r] *= shrink;
-#pragma unroll
-            for (int t = 0; t < GROUPS * 8; ++t) out[t][2 * r] *= shrink, out[t][2 * r + 1] *= shrink;
+            sum[r] *= shrink[r];
         }
-        uint32_t prob[4], rest[4];               // rounded, and what the rounding left
+        if (few) shrink[1] = shrink[0];
+#pragma unroll
+        for (int t = 0; t < GROUPS * 8; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[t][e] *= shrink[e / 2];
+        uint32_t prob[4], rest[4];               // in two terms
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const float e0 = exp2_fast(s[i][2 * r] - base[r]), e1 = exp2_fast(s[i][2 * r + 1] - base[r]);
                 sum[r] += e0 + e1;
-                prob[2 * i + r] = pack_two<T>(e0, e1);
-                rest[2 * i + r] = pack_two<T>(e0 - DT<T>::rnd(e0), e1 - DT<T>::rnd(e1));
+                prob[2 * i + r] = pack_two<T>(cut<T>(e0), cut<T>(e1));
+                rest[2 * i + r] = pack_two<T>(cut_off<T>(e0), cut_off<T>(e1));
             }
         bool by_hand = false;
         if (partly) {
@@ -176,7 +194,7 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
                     acc = taint<T>(value[c][e].x, taint<T>(value[c][e].y, taint<T>(value[c][e].z, taint<T>(value[c][e].w, acc))));
             by_hand = __any_sync(0xffffffffu, tainted<T>(acc));
         }
-        if (!by_hand) {
+        const auto add = [&](auto both) {
 #pragma unroll
             for (int c = 0; c < GROUPS; ++c)
 #pragma unroll
@@ -185,8 +203,16 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
                     const uint32_t low = __byte_perm(word(value[c][0], t / 2), word(value[c][1], t / 2), pick);
                     const uint32_t high = __byte_perm(word(value[c][2], t / 2), word(value[c][3], t / 2), pick);
                     warp_product<T>(out[8 * c + t], prob, low, high);
-                    warp_product<T>(out[8 * c + t], rest, low, high);
+                    if constexpr (decltype(both)::value) warp_product<T>(out[8 * c + t], rest, low, high);
                 }
+        };
+        if (!by_hand) {
+            if (few) {
+                prob[1] = rest[0], prob[3] = rest[2];
+                add(std::false_type());
+            } else {
+                add(std::true_type());
+            }
         } else {
             // values that are no numbers, and rows that do not see them: term by term, without the hidden terms (marked by -1)
 #pragma unroll
@@ -217,6 +243,10 @@ __global__ void __launch_bounds__(kTokenThreads, 2) global_token_kernel(const Gl
             }
             __syncwarp();
         }
+    }
+    if (few) {
+#pragma unroll
+        for (int t = 0; t < GROUPS * 8; ++t) out[t][0] += out[t][2], out[t][1] += out[t][3];
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {

@@ -32,3 +32,21 @@ def test_single_tokens_lose_nothing_to_rounded_probabilities(N, h, hk, d, dtype)
         (want,), (bound,) = _dense.attention(q.float(), k.float(), v.float(), **options)
         (terms,), _ = _dense.attention(q.float(), k.float(), v.float().abs(), **options)
         assert_within(got, want, bound + u * want.abs() + 2 * u * u * terms + last, f"out over {M} keys")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32] + HALVES)
+@pytest.mark.parametrize("N,h,hk", [(1, 8, 8), (2, 8, 2), (3, 4, 1), (40, 4, 2)])
+def test_infinite_values_that_all_see(N, h, hk, dtype):
+    """An infinite value stays an infinity of its sign in what it is added to, whatever its weight (a thousandth, or nearly all)."""
+    M, d = 300, 64
+    q, k, v, _ = make(42, 1, N, M, h, hk, d, dtype)
+    k[:, 77] = 0.0
+    for at, channel in enumerate(range(0, 48, 3)):
+        v[0, 13 * at + 1, at % hk, channel] = float("inf") if at % 2 else float("-inf")
+    want, bound = _dense.attention(q, k, v)
+    got = ma().global_attention(q, k, v)
+    assert int(got.isinf().sum()) >= N * 16
+    assert_within(got, want[0], bound[0], "out")
+    # one key of weight one: its second term is nothing but the sign
+    one = ma().global_attention(q, k[:, 77:78], v[:, 1:2])
+    assert torch.equal(one, v[:, 1:2].repeat_interleave(h // hk, 2).expand_as(one))
