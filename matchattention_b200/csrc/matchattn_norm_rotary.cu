@@ -18,8 +18,8 @@
 // as many instructions as a head's row altogether) are formed once, each group a share.  All sums are float32, results are
 // rounded once.  Measured, one B200: 16384 tokens, 40 heads x 128, bfloat16 69 us (4.9 TB/s), backward 106 us (4.7 TB/s) and 6 for the
 // weights; 384 x 384 tokens, 16 heads x 16, float16 55 us (2.7 TB/s; 511 instructions per warp and row, issue 68 %).
-// The weights' gradients are summed per lane over the rows of a block, then over the block, then over the blocks by a second
-// kernel, always in the same order: no atomics.
+// The weights' gradients are summed per lane over the rows of a block (float32, a dozen of them or so), then over the block, then over the
+// blocks by a second kernel (both in float64, whose few additions cost nothing), always in the same order: no atomics.
 #include "matchattn_kernels.cuh"
 
 #include <type_traits>
@@ -334,9 +334,9 @@ __global__ void __launch_bounds__(kNormThreads, BACK || S > 1 ? 4 : 6) norm_rota
                 const int l = e & (lanes - 1), i = e / lanes;
                 const Slot c = slot_of<V>(l + k * lanes, paired, p.rot);
                 const int channel = i < V ? c.a + i : c.b + i - V;
-                float sum = 0.0f;
+                double sum = 0.0;
                 for (int g = 0; g < kNormThreads / lanes; ++g) sum += reduced[i * kNormThreads + g * lanes + l];
-                if (channel < p.d) s.partial[static_cast<long long>(block) * p.d + channel] = sum;
+                if (channel < p.d) s.partial[static_cast<long long>(block) * p.d + channel] = static_cast<float>(sum);
             }
         }
     }
@@ -347,11 +347,11 @@ template <typename T>
 __global__ void __launch_bounds__(1024) norm_weight_kernel(const NormParams p)
 {
     chain_begin();
-    __shared__ float sums[32][33];
+    __shared__ double sums[32][33];
     const NormSide &s = p.side[blockIdx.y];
     if (s.partial == nullptr) return;
     const int c = blockIdx.x * 32 + threadIdx.x;
-    float sum = 0.0f;
+    double sum = 0.0;
     if (c < p.d)
         for (int i = threadIdx.y; i < s.blocks; i += 32) sum += s.partial[static_cast<long long>(i) * p.d + c];
     sums[threadIdx.y][threadIdx.x] = sum;
@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(1024) norm_weight_kernel(const NormParams p)
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const int out = blockIdx.x * 32 + threadIdx.y;
     if (threadIdx.x == 0 && out < p.d) {
-        if (p.w32) static_cast<float *>(s.dw)[out] = sum;
-        else store_one<T>(static_cast<T *>(s.dw) + out, sum);
+        if (p.w32) static_cast<float *>(s.dw)[out] = static_cast<float>(sum);
+        else store_one<T>(static_cast<T *>(s.dw) + out, static_cast<float>(sum));
     }
 }
 
