@@ -355,7 +355,8 @@ MATCHATTN_API int matchattn_flow_init(const void *correlation, void *prob, void 
  * lengths[b] - N + n: the last query at the last key.  It sees key j if j exists, and (with causal) j is not behind its own
  * position or j < prefix[b], and (with documents) both ids are equal and not negative.  dx, dy: columns and rows between the
  * two positions on a map `width` tokens wide (width 1: their distance in a sequence).
- * What no query may see does not reach a result, infinite and NaN values included.
+ * What no query may see does not reach a result, infinite, NaN and large finite values included; a value that a query sees does, whatever its
+ * weight.  A query whose visible scores are all minus infinity counts as one that sees nothing.
  *
  *   q [B, N, h, d], k and v [B, M, hk, d] with the strides given (elements; item, token, head; channels are contiguous)
  *   out [B, N, h, d], contiguous, written.  h is a multiple of hk: query heads [i*h/hk, (i+1)*h/hk) share key head i.
@@ -364,7 +365,8 @@ MATCHATTN_API int matchattn_flow_init(const void *correlation, void *prob, void 
  *     of d_out * out would lose half their digits without it; may be NULL (not used in float32)
  *   d <= MATCHATTN_MAX_DENSE_D; 0 <= M <= 2^24; 0 < N <= 2^24; scale > 0; cap >= 0 (0: none), both and scale / cap between
  *   2^-126 and 2.3e38; prefix needs causal.
- * Scores, softmax and sums are float32.  The sums do not depend on timing: equal calls give equal bits.
+ * Scores, softmax and sums are float32.  The sums do not depend on timing: equal calls give equal bits.  Every wait of the kernels for their
+ * own copies and products has a limit (2 s; none lasts longer than microseconds); results of a block that ran into it are NaN.
  */
 #define MATCHATTN_MAX_DENSE_D 256
 typedef struct matchattn_global_args {

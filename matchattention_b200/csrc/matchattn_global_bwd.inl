@@ -10,7 +10,7 @@
 //
 // A block has a fixed pair of tiles (keys: K, V; queries: Q, dO) and a moving pair (Q, dO; K, V).  The scores and dP of
 // fixed by moving rows come to tensor memory; a thread holds a fixed row and 32 of the 128 moving ones (warps 0-15), and puts P over S
-// and dS over dP, rounded to the type, as first operands of the products that add up the moving rows.  Order of the
+// and dS over dP, rounded to the type (which the matrix unit asks for), as first operands of the products that add up the moving rows.  Order of the
 // matrix unit: dV(i-1), S(i), dK(i-1), dP(i): while threads take exponentials of tile i it forms dK(i-1) and dP(i), while
 // they form dS(i) it forms dV(i) and S(i+1).
 //
@@ -19,8 +19,8 @@
 // the sums exactly.  The bound knows only tokens of visible pairs (global_levels_kernel): what is hidden, another item, another key
 // head, or a tile that the block never meets, however large, takes no digits from a sum.
 //
-// Measured, one B200: 2 x 4096 tokens, 16 heads x 128 on 4 key heads, bfloat16, causal and capped 369 us (dK, dV) and 323 us (dQ); 8160
-// tokens, 8 heads x 16, float16, map bias 681 and 560.  Bound by the steps that a tile goes through one after another (scores, P,
+// Measured, one B200: 2 x 4096 tokens, 16 heads x 128 on 4 key heads, bfloat16, causal and capped 371 us (dK, dV) and 320 us (dQ); 8160
+// tokens, 8 heads x 16, float16, map bias 686 and 526.  Bound by the steps that a tile goes through one after another (scores, P,
 // dP, dS); with eight warps of 64 rows each and the rows' figures fetched within the tile 497 + 407 and 843 + 650.
 //
 // As in the forward pass, tiles that are partly hidden are looked through for infinite and NaN values, and added term by term

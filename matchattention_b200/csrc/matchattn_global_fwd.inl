@@ -11,15 +11,15 @@
 // tensor memory is hardly ever touched between products, and nothing waits for a maximum.  float16 has few exponents: P, the sum and O are
 // held times 2^7 there, the room that the type leaves above 2^8, and over keys without end, whose small weights add up, times 2^11,
 // with a reference that moves at 2^4 (for every call that would cost: 48 x 48 tokens with a map bias 62 us for 51).
-// P is rounded to the type of V (a half step of it, relative, as torch rounds a softmax's result); scores, reference, sums and O are
-// float32.  For training O is divided by the sum of the rounded probabilities: their errors then weigh differences of values and not
+// P is rounded to the type of V (a half step of it, relative, as torch rounds a softmax's result; the matrix unit takes both operands in one
+// type, and a second term of P would be a product more); scores, reference, sums and O are float32.  For training O is divided by the sum of the rounded probabilities: their errors then weigh differences of values and not
 // the values (8160 tokens of 8 heads x 16, float16: 2.8e-4 from the exact result, 2.9e-4 without), which the row sums of the backward
 // pass build on.  Elsewhere by the sum itself: the second sum costs 5 to 10 %.
 //
-// Measured, one B200: 8192 tokens, 32 heads x 128 on 8 key heads, bfloat16, causal 566 us (0.97 PFLOP/s, 0.59 of the measured rate of a
-// library product).  With the softmax taken out the same products and copies take 467: scores read both of their operands from shared
-// memory at its full rate, beside the copies into it.  48 x 48 tokens x 2, 4 heads x 32, float16, map bias 50 us: one tile per block and SM,
-// eighteen dependent steps of 2.8 us.
+// Measured, one B200: 8192 tokens, 32 heads x 128 on 8 key heads, bfloat16, causal 617 us a call (0.89 PFLOP/s, 0.54 of the measured rate of a
+// library product).  Calls of one input in a row took 566, and 467 with the softmax taken out: scores read both of their operands from
+// shared memory at its full rate, beside the copies into it.  48 x 48 tokens x 2, 4 heads x 32, float16, map bias 51 us: one tile per
+// block and SM, eighteen dependent steps of 2.8 us.
 //
 // A probability that the mask makes zero meets V all the same in the product, and 0 * NaN is NaN: where a tile is partly
 // hidden, its V is looked through first, and one with infinite or NaN values is added term by term.

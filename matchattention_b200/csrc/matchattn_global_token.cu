@@ -11,8 +11,10 @@
 // a lane's eight neighbouring channels of V are its column of eight column tiles (pairs of keys are put together by a byte
 // permute).  The next run's keys are on their way while a run is computed.
 //
-// Measured, one B200: 8 items of 2048 to 8192 keys, 32 heads on 8 key heads x 128, bfloat16 44 us (2.4 TB/s), the join 8; one item of 317
-// keys, 8 heads x 64, float16 4.6 us.  255 registers hold 8 KB per warp on their way, eight warps per SM.
+// Measured, one B200: 8 items of 2048 to 8192 keys, 32 heads on 8 key heads x 128, bfloat16 47 us (DRAM at half its rate), the join 8; one item
+// of 317 keys, 8 heads x 64, float16 4.9 us.  255 registers hold 8 KB per warp on their way, eight warps per SM: an SM with two full
+// shares reads near its part of the memory's rate.  But the shares are cut from M, not from an item's own length: behind the shorter
+// lengths blocks have nothing to read, and the longest share takes 1.4 to 1.7 times the mean.
 //
 // Each warp keeps its own maximum, sum and output; the warps are joined in shared memory, the shares of the keys by a second
 // kernel.  Everything is float32 but the probabilities, which meet V as two terms of the type (rounded to it once they would make the largest

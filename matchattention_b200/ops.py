@@ -548,7 +548,7 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
     ``lengths[b] - N + n``: new tokens at the end of a cache, or a whole sequence when N is its length.  ``causal`` hides keys
     behind the query's position, except those below ``prefix[b]`` (int32 [B]).  ``documents``: int32 ids of the tokens, [B,N] for
     N == M, or a pair for queries and keys; a query sees keys of its own id, and a negative id sees and shows nothing.
-    A query that sees no key gives zeros.  What no query sees, NaN included, does not reach a result.
+    A query that sees no key (or scores of minus infinity alone) gives zeros.  What no query sees, NaN included, does not reach a result.
 
     Scores, softmax and sums are float32.  16-bit calls round the probabilities to the type for the products with v and its gradient,
     and the scores' gradients for theirs; calls of at most sixteen query rows per key head (N * h / hk) take the probabilities as two terms.

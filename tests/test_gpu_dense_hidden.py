@@ -150,3 +150,24 @@ def test_a_value_that_is_seen_with_hardly_any_weight(ahead, N, dtype):
     for name, g, w in zip(NAMES, got, want):
         assert torch.equal(g.isnan(), w.isnan()), name
     assert_within(got[0], want[0], bound[0], "out")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [2, 150])
+@pytest.mark.parametrize("options", [dict(), dict(causal=True), dict(slopes=True)], ids=str)
+def test_rows_of_scores_of_minus_infinity(options, N, dtype):
+    """Scores that overflow: a query that has no other sees nothing, gives zeros and takes part in no gradient."""
+    M, h, d = 200, 2, 64
+    q, k, v, dout = make(37, 1, N, M, h, h, d, dtype)
+    options = dict(options, slopes=torch.ones(h, device="cuda")) if "slopes" in options else options
+    q[:], k[:] = 0.0, -100.0
+    q[:, ::2] = 100.0
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = ma().global_attention(*leaves, scale=1e35, **options)
+    grads = torch.autograd.grad(out, leaves, dout)
+    assert bool((out[:, ::2] == 0).all()) and bool(torch.isfinite(out).all()) and bool((out[:, 1::2] != 0).any())
+    assert bool((grads[0][:, ::2] == 0).all())
+    rest = v.detach().clone().requires_grad_()
+    (dv,) = torch.autograd.grad(ma().global_attention(q.detach()[:, 1::2], k.detach(), rest, scale=1e35, causal=False), rest, dout[:, 1::2].contiguous())
+    if not options:
+        assert torch.allclose(grads[2].float(), dv.float(), rtol=4 * torch.finfo(dtype).eps, atol=2.0 ** -10)
