@@ -6,12 +6,14 @@
 //
 // Two passes of one kernel, each recomputing S and P: for keys (a block owns 128 keys of a key head, walks the queries of all
 // heads that share it, and keeps dK and dV in tensor memory) and for queries (128 queries, walks the keys, keeps dQ).  That is seven
-// products where one pass with dQ added up in global memory has five, but the sums have one order and no atomics.
+// products (one of them in two terms) where one pass with dQ added up in global memory has five, but the sums have one order and no atomics.
 //
 // A block has a fixed pair of tiles (keys: K, V; queries: Q, dO) and a moving pair (Q, dO; K, V).  The scores and dP of
 // fixed by moving rows come to tensor memory; a thread holds a fixed row and 32 of the 128 moving ones (warps 0-15), and puts P over S
-// and dS over dP, rounded to the type (which the matrix unit asks for), as first operands of the products that add up the moving rows.  Order of the
-// matrix unit: dV(i-1), S(i), dK(i-1), dP(i): while threads take exponentials of tile i it forms dK(i-1) and dP(i), while
+// and dS over dP, rounded to the type (which the matrix unit asks for), as first operands of the products that add up the moving rows.
+// dQ takes dS as two terms, cut to the type and what that left, in two products: rounded once, its error beside those of delta and of the
+// result made dQ 1.41 to 1.5 times as far from the exact gradient as the result's own rounding; it is 1.01 to 1.05 times now (dK and
+// dV stand at 1.35 to 1.45 times), for 570 us in place of 526 in the second case below.  Order of the matrix unit: dV(i-1), S(i), dK(i-1), dP(i): while threads take exponentials of tile i it forms dK(i-1) and dP(i), while
 // they form dS(i) it forms dV(i) and S(i+1).
 //
 // float16 has few exponents: P is held times 2^12 (P of a row of 10^5 tokens is not subnormal), dS times the power of two that
@@ -19,8 +21,8 @@
 // the sums exactly.  The bound knows only tokens of visible pairs (global_levels_kernel): what is hidden, another item, another key
 // head, or a tile that the block never meets, however large, takes no digits from a sum.
 //
-// Measured, one B200: 2 x 4096 tokens, 16 heads x 128 on 4 key heads, bfloat16, causal and capped 371 us (dK, dV) and 320 us (dQ); 8160
-// tokens, 8 heads x 16, float16, map bias 686 and 526.  Bound by the steps that a tile goes through one after another (scores, P,
+// Measured, one B200: 2 x 4096 tokens, 16 heads x 128 on 4 key heads, bfloat16, causal and capped 345 us (dK, dV) and 322 us (dQ); 8160
+// tokens, 8 heads x 16, float16, map bias 686 and 570.  Bound by the steps that a tile goes through one after another (scores, P,
 // dP, dS); with eight warps of 64 rows each and the rows' figures fetched within the tile 497 + 407 and 843 + 650.
 //
 // As in the forward pass, tiles that are partly hidden are looked through for infinite and NaN values, and added term by term
@@ -38,7 +40,7 @@ struct BackShared {
     static constexpr int kStages = DP == 128 ? 2 : 3;
     uint8_t fixed[2][kTileBytes<DP>];
     uint8_t moving[kStages][2][kTileBytes<DP>];
-    float4 lse[16][8], delta[16][8], across[16][8], down[16][8];      // per warp, for its 32 moving rows; column and row on the map
+    float4 lse[16][8], delta[16][8], across[16][8], down[16][8];      // per warp, for its 32 moving rows; less delta; column and row on the map
     int4 docs[16][8];
     uint64_t fixed_full, full[kStages], empty[kStages], s_full, p_full, dp_full, ds_full, done, looked, stored;
     uint32_t tmem;
@@ -174,7 +176,10 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 good = good && barrier_wait(&sh.ds_full, n & 1, &sh.broken);
                 if (!good) return;
                 tmem_after();
-                if (!*static_cast<volatile int *>(&sh.by_hand[1])) add_up(sum_k, slopes, moving(by_row, n, 0), n > 0);
+                if (!*static_cast<volatile int *>(&sh.by_hand[1])) {
+                    add_up(sum_k, slopes, moving(by_row, n, 0), n > 0);
+                    if (!KEYS) add_up(sum_k, slopes + 16, moving(by_row, n, 0), true);        // the second terms of dS
+                }
                 products_done(&sh.empty[n % STAGES]);
             };
             for (int r = r_begin; r < rounds && good; ++r)
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 const int m0 = t * kTile + w * kPart;                           // first of the warp's moving rows
                 if (KEYS) {
                     reinterpret_cast<float *>(sh.lse[warp])[lane] = next_lse;
-                    reinterpret_cast<float *>(sh.delta[warp])[lane] = next_delta;
+                    reinterpret_cast<float *>(sh.delta[warp])[lane] = -next_delta;
                 }
                 if (p.q_docs) reinterpret_cast<int *>(sh.docs[warp])[lane] = next_doc;
                 if (lane == 0) sh.begin[warp] = t * kTile;
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                 if (!good) break;
                 tmem_after();
                 {
-                    uint32_t dp[32], packed[16];
+                    uint32_t dp[32], packed[KEYS ? 16 : 32];
                     tmem_load32(my_slopes, dp);
                     tmem_loaded32(dp);
 #pragma unroll
@@ -362,10 +367,23 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                         if (KEYS) row_delta = sh.delta[warp][e / 4];
                         float value[4];
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const int at = e + u;
-                            const float off = __uint_as_float(dp[e + u]) - (KEYS ? element(row_delta, u) : delta);
-                            value[u] = prob[at] * (HALF ? off * hold : off);
+                        for (int u = 0; u < 4; u += 2) {
+                            Pair off = pair_add(Pair(__uint_as_float(dp[e + u]), __uint_as_float(dp[e + u + 1])),
+                                                KEYS ? Pair(element(row_delta, u), element(row_delta, u + 1)) : Pair(-delta, -delta));
+                            if (HALF) off = pair_mul(off, Pair(hold, hold));
+                            pair_mul(Pair(prob[e + u], prob[e + u + 1]), off).get(value[u], value[u + 1]);
+                        }
+                        if (!KEYS) {
+                            // cut to the digits of the type, and what that leaves
+#pragma unroll
+                            for (int u = 0; u < 4; u += 2) {
+                                const Pair whole(value[u], value[u + 1]);
+                                float rest[2];
+                                value[u] = __uint_as_float(__float_as_uint(value[u]) & (HALF ? 0xffffe000u : 0xffff0000u));
+                                value[u + 1] = __uint_as_float(__float_as_uint(value[u + 1]) & (HALF ? 0xffffe000u : 0xffff0000u));
+                                pair_fma(Pair(value[u], value[u + 1]), Pair(-1.0f, -1.0f), whole).get(rest[0], rest[1]);
+                                packed[16 + (e + u) / 2] = pack_two<T>(rest[0], rest[1]);
+                            }
                         }
                         packed[e / 2] = pack_two<T>(value[0], value[1]);
                         packed[e / 2 + 1] = pack_two<T>(value[2], value[3]);
@@ -380,11 +398,15 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
 #pragma unroll
                             for (int u = 0; u < 4; ++u) {
                                 const bool seen = (KEYS ? e + u >= begin : e + u < begin) && (!p.q_docs || element(docs, u) == doc);
-                                if (!seen) packed[(e + u) / 2] &= u & 1 ? 0x0000ffffu : 0xffff0000u;
+                                if (!seen) {
+                                    packed[(e + u) / 2] &= u & 1 ? 0x0000ffffu : 0xffff0000u;
+                                    if (!KEYS) packed[16 + (e + u) / 2] &= u & 1 ? 0x0000ffffu : 0xffff0000u;
+                                }
                             }
                         }
                     }
-                    tmem_store16(my_slopes, packed);
+                    if (KEYS) tmem_store16(my_slopes, packed);
+                    else tmem_store32(my_slopes, packed);
                 }
                 tmem_stored();
                 if (hand_k) {
@@ -393,7 +415,10 @@ __global__ void __launch_bounds__(kBackThreads, 1) global_backward_kernel(const 
                     good = barrier_wait(&sh.stored, stores & 1, &sh.broken);
                     tmem_after();
                     ++stores;
-                    if (w == 1) add_rows<T, DP, kPart>(sum_k + lanes, slopes + lanes, sh.moving[i % STAGES][0], i > 0, seen_rows());
+                    if (w == 1) {
+                        add_rows<T, DP, kPart>(sum_k + lanes, slopes + lanes, sh.moving[i % STAGES][0], i > 0, seen_rows());
+                        if (!KEYS) add_rows<T, DP, kPart>(sum_k + lanes, slopes + 16 + lanes, sh.moving[i % STAGES][0], true, seen_rows());
+                    }
                 }
                 if (tid == 0) sh.by_hand[1] = hand_k;
                 tmem_before();

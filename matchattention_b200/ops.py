@@ -551,7 +551,8 @@ def global_attention(q, k, v, *, scale: Optional[float] = None, cap: float = 0.0
     A query that sees no key (or scores of minus infinity alone) gives zeros.  What no query sees, NaN included, does not reach a result.
 
     Scores, softmax and sums are float32.  16-bit calls round the probabilities to the type for the products with v and its gradient,
-    and the scores' gradients for theirs; calls of at most sixteen query rows per key head (N * h / hk) take the probabilities as two terms.
+    and the scores' gradients for that of k (that of q takes them as two terms, and so do calls of at most sixteen query rows per key
+    head, N * h / hk, the probabilities).
     Equal calls give equal bits (a call that forms gradients divides by the sum of the rounded probabilities, and can differ from one
     that does not in the last place)."""
     q_docs, k_docs = documents if isinstance(documents, (tuple, list)) and len(documents) == 2 else (documents, documents)

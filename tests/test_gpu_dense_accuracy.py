@@ -50,3 +50,20 @@ def test_infinite_values_that_all_see(N, h, hk, dtype):
     # one key of weight one: its second term is nothing but the sign
     one = ma().global_attention(q, k[:, 77:78], v[:, 1:2])
     assert torch.equal(one, v[:, 1:2].repeat_interleave(h // hk, 2).expand_as(one))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("N,h,hk,d,options", [(1500, 4, 4, 16, dict(slopes=True, width=40)), (700, 4, 1, 64, dict(causal=True)), (500, 2, 2, 128, dict(causal=True, cap=20.0))],
+                         ids=str)
+def test_gradients_of_queries_lose_nothing_to_rounded_terms(N, h, hk, d, options, dtype):
+    """dS enters the sum over the keys as two terms: what is left beside the rounding of the result itself is what the rounding of the forward's
+    probabilities does to delta, a tenth of it (rounded once, dS would put its own error beside the result's: the square root of two)."""
+    q, k, v, dout = make(43, 1, N, N, h, hk, d, dtype)
+    if "slopes" in options:
+        options = dict(options, slopes=(0.5 * 2.0 ** -(8 * torch.arange(h, dtype=torch.float32) / h)).cuda())
+    want = _dense.attention(q, k, v, dout=dout, **options)[0][1]
+    q.requires_grad_()
+    (got,) = torch.autograd.grad(ma().global_attention(q, k, v, **options), q, dout)
+    far = (got.double() - want).square().mean().sqrt()
+    rounding = (want.to(dtype).double() - want).square().mean().sqrt()
+    assert float(far / rounding) <= 1.2
