@@ -13,8 +13,8 @@
 // and dS over dP, rounded to the type (which the matrix unit asks for), as first operands of the products that add up the moving rows.
 // dQ takes dS as two terms, cut to the type and what that left, in two products: rounded once, its error beside those of delta and of the
 // result made dQ 1.41 to 1.5 times as far from the exact gradient as the result's own rounding; it is 1.01 to 1.05 times now (dK and
-// dV stand at 1.35 to 1.45 times), for 570 us in place of 526 in the second case below.  Order of the matrix unit: dV(i-1), S(i), dK(i-1), dP(i): while threads take exponentials of tile i it forms dK(i-1) and dP(i), while
-// they form dS(i) it forms dV(i) and S(i+1).
+// dV stand at 1.35 to 1.45 times), for 570 us in place of 526 in the second case below.  Order of the matrix unit: dV(i-1), S(i),
+// dK(i-1), dP(i): while threads take exponentials of tile i it forms dK(i-1) and dP(i), while they form dS(i) it forms dV(i) and S(i+1).
 //
 // float16 has few exponents: P is held times 2^12 (P of a row of 10^5 tokens is not subnormal), dS times the power of two that
 // brings the largest value that |dS| <= |dO| |V| + |delta| allows over the tiles that the block meets to between 2^14 and 2^15; both leave
